@@ -1465,3 +1465,650 @@ extern "C" int32_t hoic_mlp_value_loss(int32_t M, const float* d_v, const float*
   MCHK(hipGetLastError());
   return HOIC_OK;
 }
+
+// ================================================================================================ learning operators
+// The second half of a training step on any list of tensors: the clipped policy loss with a KL term (value and gradient), the
+// norm of a list of gradients, and AdamW over many tensors with states in 32 or in 8 bits.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));            // four elements at the alignment of one
+typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 b4u __attribute__((ext_vector_type(4), aligned(2)));
+template <class T> struct vec4;
+template <> struct vec4<float> { typedef f4u type; };
+template <> struct vec4<_Float16> { typedef h4u type; };
+template <> struct vec4<__bf16> { typedef b4u type; };
+
+// four elements from x on, of which the first `left` exist (the rest read as 0)
+template <class T> __device__ __forceinline__ f32x4 load4(const T* __restrict__ x, int left) {
+  f32x4 r = {0.f, 0.f, 0.f, 0.f};
+  if (left >= 4) {
+    r = __builtin_convertvector(*(const typename vec4<T>::type*)x, f32x4);
+  } else {
+    if (left > 0) r.x = (float)x[0];
+    if (left > 1) r.y = (float)x[1];
+    if (left > 2) r.z = (float)x[2];
+  }
+  return r;
+}
+template <class T> __device__ __forceinline__ void store4(T* __restrict__ x, int left, f32x4 r) {
+  if (left >= 4) {
+    *(typename vec4<T>::type*)x = __builtin_convertvector(r, typename vec4<T>::type);
+  } else {
+    if (left > 0) x[0] = (T)r.x;
+    if (left > 1) x[1] = (T)r.y;
+    if (left > 2) x[2] = (T)r.z;
+  }
+}
+__device__ __forceinline__ f32x4 load4_any(const void* x, long long i, int left, int type) {
+  if (type == HOIC_F32) return load4((const float*)x + i, left);
+  if (type == HOIC_F16) return load4((const _Float16*)x + i, left);
+  return load4((const __bf16*)x + i, left);
+}
+__device__ __forceinline__ void store4_any(void* x, long long i, int left, int type, f32x4 r) {
+  if (type == HOIC_F32) store4((float*)x + i, left, r);
+  else if (type == HOIC_F16) store4((_Float16*)x + i, left, r);
+  else store4((__bf16*)x + i, left, r);
+}
+
+// ---------------------------------------------------------------------------------------------- clipped policy loss with a KL term
+// rows m, action dimensions j; mu, s = log sigma, action a, advantage A, old log-probability l0, reference policy (mu0, s0):
+//   l = sum_j [-(a - mu)^2 / (2 e^{2s}) - s - log(2 pi) / 2],   r = e^{l - l0}   (r = 1 without l0: the old policy is this one)
+//   S = -min(r A, clip(r) A),   K = KL(reference || policy) = sum_j [s - s0 + (e^{2 s0} + (mu - mu0)^2) / (2 e^{2s}) - 1/2]
+//   L = sum over the valid rows of (S + c K) / n
+//   dS/dl = -A r where the row passes its gradient (r A < clip(r) A, or r inside the closed interval), else 0
+// Everything per row is in 64 bits: a row whose ratio lies within a float32 rounding of a clip border would otherwise have its
+// whole gradient or none by chance (|l| is 50 and more, so float32 leaves the ratio 1e-5 wide); on this GPU a 64-bit FMA
+// issues at the rate of a float32 one, and the kernel waits for memory.
+// A row is handled by `lpr` lanes of four dimensions each (lpr = the power of two >= dims / 4), a wavefront takes 64 / lpr rows.
+struct PolicyLossArgs {
+  hoic_policy_loss_args a;
+  int lpr_log2;
+  const int* counts; int ncounts;        // partial counts of the valid rows (gradient with a mask)
+  double* part;                          // [blocks][dims + 3]
+};
+#define PL_NT 256
+
+__global__ __launch_bounds__(256) void hoic_count_valid_kernel(const unsigned char* __restrict__ valid, long long rows, long long per_block, int* __restrict__ counts) {
+  __shared__ int red[4];
+  const long long r0 = (long long)blockIdx.x * per_block, r1 = r0 + per_block < rows ? r0 + per_block : rows;
+  int c = 0;
+  for (long long r = r0 + threadIdx.x; r < r1; r += 256) c += valid[r] != 0;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+__device__ __forceinline__ void policy_loss_scalars(const hoic_policy_loss_args& a, double surr, double kl, double clipped, double n) {
+  const double d = n > 0. ? n : 1.;
+  surr /= d; kl /= d;
+  a.out[0] = (float)(surr + a.kl_coef * kl);
+  a.out[1] = (float)surr; a.out[2] = (float)kl; a.out[3] = (float)(clipped / d); a.out[4] = (float)n; a.out[5] = 0.f;
+  *(double*)(a.out + 6) = n;
+}
+
+template <class TM, class TA> __global__ __launch_bounds__(PL_NT) void hoic_policy_loss_kernel(PolicyLossArgs k) {
+  const hoic_policy_loss_args& a = k.a;
+  __shared__ double red[PL_NT * 4];
+  __shared__ double tail[3][PL_NT / 64];
+  __shared__ int wcount[PL_NT / 64];
+  const int lpr = 1 << k.lpr_log2, sub = threadIdx.x & (lpr - 1), j = sub * 4, left = a.dims - j;
+  const int rpb = PL_NT >> k.lpr_log2, rg = threadIdx.x >> k.lpr_log2;
+  const bool grad = a.d_mean != nullptr, kl_on = a.ref_mean != nullptr, shared_std = a.ld_std == 0, sum_ls = grad && a.d_log_std && shared_std;
+  double n = (double)a.rows;
+  if (grad && a.valid) {
+    if (a.count) {
+      n = *a.count;
+    } else {
+      int c = 0;
+      for (int i = threadIdx.x; i < k.ncounts; i += PL_NT) c += k.counts[i];
+#pragma unroll
+      for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
+      if ((threadIdx.x & 63) == 0) wcount[threadIdx.x >> 6] = c;
+      __syncthreads();
+      n = 0.;
+      for (int w = 0; w < PL_NT / 64; w++) n += (double)wcount[w];
+    }
+  }
+  const double scale = grad ? a.weight * (a.upstream ? (double)*a.upstream : 1.) / (n > 0. ? n : 1.) : 0.;
+  const double lo = 1. - a.clip_lo, hi = 1. + a.clip_hi, klw = a.kl_coef * scale;
+  double iv[4], lc[4], kc[4], ke[4];            // 1 / sigma^2, -s - log(2 pi) / 2, the KL's part without the means, e^{2 (s0 - s)}
+  auto std_terms = [&](f32x4 s, f32x4 s0) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const double sd = (double)s[e], s0d = (double)s0[e];
+      iv[e] = e < left ? exp(-2. * sd) : 0.;
+      lc[e] = e < left ? -sd - 0.91893853320467274178 : 0.;
+      ke[e] = kl_on && e < left ? exp(2. * (s0d - sd)) : 0.;
+      kc[e] = kl_on && e < left ? sd - s0d + 0.5 * ke[e] - 0.5 : 0.;
+    }
+  };
+  const bool once = shared_std && (!kl_on || a.ld_ref_std == 0);
+  if (once) std_terms(load4_any(a.log_std, j, left, a.t_std), kl_on ? load4_any(a.ref_log_std, j, left, a.t_std) : f32x4{0.f, 0.f, 0.f, 0.f});
+  double dls[4] = {0., 0., 0., 0.}, acc_s = 0., acc_k = 0., acc_c = 0., acc_n = 0.;
+  const long long nchunks = (a.rows + rpb - 1) / rpb;
+  for (long long c = blockIdx.x; c < nchunks; c += gridDim.x) {
+    const long long row = c * rpb + rg;
+    const bool in = row < a.rows, ok = in && (!a.valid || a.valid[row]);
+    const int l = ok ? left : 0;
+    f32x4 mu = load4((const TM*)a.mean + (ok ? row * a.ld_mean + j : 0), l), x = load4((const TA*)a.act + (ok ? row * a.ld_act + j : 0), l);
+    f32x4 mu0 = kl_on ? load4((const TM*)a.ref_mean + (ok ? row * a.ld_ref_mean + j : 0), l) : f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!once) std_terms(load4_any(a.log_std, ok ? row * a.ld_std + j : 0, l, a.t_std),
+                         kl_on ? load4_any(a.ref_log_std, ok ? row * a.ld_ref_std + j : 0, l, a.t_std) : f32x4{0.f, 0.f, 0.f, 0.f});
+    const double A = ok ? (double)a.adv[row] : 0., l0 = ok && a.fixed ? (double)a.fixed[row] : 0.;
+    double d[4], dk[4], lp = 0., kl = 0.;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      d[e] = (double)x[e] - (double)mu[e];
+      dk[e] = kl_on ? (double)mu[e] - (double)mu0[e] : 0.;
+      lp += lc[e] - 0.5 * d[e] * d[e] * iv[e];
+      kl += kc[e] + 0.5 * dk[e] * dk[e] * iv[e];
+    }
+    for (int o = lpr >> 1; o; o >>= 1) { lp += __shfl_xor(lp, o, 64); kl += __shfl_xor(kl, o, 64); }
+    const double r = a.fixed ? exp(lp - l0) : 1.;
+    const double s1 = r * A, s2 = (r < lo ? lo : r > hi ? hi : r) * A;
+    const bool pass = s1 < s2 || (r >= lo && r <= hi) || r != r;      // (a NaN is passed on)
+    if (ok && sub == 0) {
+      acc_s -= s1 < s2 || s1 != s1 ? s1 : s2;
+      acc_k += kl;
+      acc_c += pass ? 0. : 1.;
+      acc_n += 1.;
+    }
+    if (a.log_probs && in && sub == 0) a.log_probs[row] = ok ? (float)lp : 0.f;
+    if (grad && in) {
+      const double dlp = ok && pass ? -scale * s1 : 0.;
+      f32x4 g, gs;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const double gm = ok ? (dlp * d[e] + klw * dk[e]) * iv[e] : 0.;
+        const double gl = ok ? dlp * (d[e] * d[e] * iv[e] - 1.) + (kl_on ? klw * (1. - ke[e] - dk[e] * dk[e] * iv[e]) : 0.) : 0.;
+        g[e] = (float)gm; gs[e] = (float)gl;
+        if (sum_ls) dls[e] += gl;
+      }
+      store4((TM*)a.d_mean + row * a.ld_dmean + j, left, g);
+      if (a.d_log_std && !shared_std) store4_any(a.d_log_std, row * a.dims + j, left, a.t_std, gs);
+    }
+  }
+  // the block's sums in fixed order: the gradient of a shared log-deviation over the block's row groups, then the scalars
+  const int ps = a.dims + 4;
+  double* part = k.part + (long long)blockIdx.x * ps;
+  if (sum_ls) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) red[rg * (lpr * 4) + j + e] = dls[e];
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) { acc_s += __shfl_xor(acc_s, o, 64); acc_k += __shfl_xor(acc_k, o, 64); acc_c += __shfl_xor(acc_c, o, 64); acc_n += __shfl_xor(acc_n, o, 64); }
+  if ((threadIdx.x & 63) == 0) { const int w = threadIdx.x >> 6; tail[0][w] = acc_s; tail[1][w] = acc_k; tail[2][w] = acc_c; wcount[w] = (int)acc_n; }
+  __syncthreads();
+  if (sum_ls && threadIdx.x < a.dims) {
+    double t = 0.;
+    for (int q = 0; q < rpb; q++) t += red[q * (lpr * 4) + threadIdx.x];
+    part[threadIdx.x] = t;
+  }
+  if (threadIdx.x == 0 && !a.count) {
+    double t[4] = {0., 0., 0., 0.};
+    for (int w = 0; w < PL_NT / 64; w++) { t[0] += tail[0][w]; t[1] += tail[1][w]; t[2] += tail[2][w]; t[3] += (double)wcount[w]; }
+    for (int q = 0; q < 4; q++) part[a.dims + q] = t[q];
+  }
+}
+
+// sums of the blocks' parts: workgroup 0 the scalars, the others eight dimensions each (32 lanes a column, fixed order)
+__global__ __launch_bounds__(256) void hoic_policy_loss_finish_kernel(PolicyLossArgs k, int nb) {
+  const hoic_policy_loss_args& a = k.a;
+  const int ps = a.dims + 4, col = threadIdx.x & 7, q = threadIdx.x >> 3;
+  const int j = blockIdx.x == 0 ? (col < 4 ? a.dims + col : -1) : ((int)blockIdx.x - 1) * 8 + col;
+  const bool on = blockIdx.x == 0 ? col < 4 && !a.count : j < a.dims;       // (with a.count the forward call wrote the scalars)
+  __shared__ double red[32][9];
+  double t = 0.;
+  if (on) for (int b = q; b < nb; b += 32) t += k.part[(long long)b * ps + j];
+  red[q][col] = t;
+  __syncthreads();
+  if (threadIdx.x < 8) {
+    double s = 0.;
+    for (int i = 0; i < 32; i++) s += red[i][threadIdx.x];
+    red[0][threadIdx.x] = s;
+    if (blockIdx.x > 0 && on) {
+      if (a.t_std == HOIC_F32) ((float*)a.d_log_std)[j] = (float)s;
+      else if (a.t_std == HOIC_F16) ((_Float16*)a.d_log_std)[j] = (_Float16)(float)s;
+      else ((__bf16*)a.d_log_std)[j] = (__bf16)(float)s;
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0 && !a.count) policy_loss_scalars(a, red[0][0], red[0][1], red[0][2], red[0][3]);
+}
+
+#define PL_BLOCKS 512
+#define PL_COUNTS 256
+extern "C" int64_t hoic_policy_loss_scratch_bytes(int32_t dims) { return dims <= 0 ? 0 : (int64_t)PL_BLOCKS * (dims + 4) * 8 + PL_COUNTS * 4; }
+template <class TM, class TA> static void launch_policy_loss(const PolicyLossArgs& k, int nb, hipStream_t st) {
+  hipLaunchKernelGGL((hoic_policy_loss_kernel<TM, TA>), dim3(nb), dim3(PL_NT), 0, st, k);
+}
+extern "C" int32_t hoic_policy_loss(const hoic_policy_loss_args* p, void* stream) {
+  if (!p) { hoic_set_error("hoic_policy_loss: no arguments"); return HOIC_ERR_ARG; }
+  const hoic_policy_loss_args& a = *p;
+  auto type_ok = [](int t) { return t == HOIC_F32 || t == HOIC_F16 || t == HOIC_BF16; };
+  if (a.rows < 0 || a.dims <= 0 || a.dims > 256 || !type_ok(a.t_mean) || !type_ok(a.t_act) || !type_ok(a.t_std) || (a.t_act != a.t_mean && a.t_act != HOIC_F32)
+      || (a.t_std != a.t_mean && a.t_std != HOIC_F32)) {
+    hoic_set_error("hoic_policy_loss: 1 .. 256 dimensions; actions and log_std in float32 or in the mean's type"); return HOIC_ERR_ARG;
+  }
+  if (!a.scratch || (!a.count && !a.out) || !a.log_std || (a.rows > 0 && (!a.mean || !a.act || !a.adv)) || (!a.ref_mean) != (!a.ref_log_std) || (a.d_log_std && !a.d_mean)
+      || (a.count && !a.d_mean)) {
+    hoic_set_error("hoic_policy_loss: missing tensors"); return HOIC_ERR_ARG;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  PolicyLossArgs k;
+  k.a = a;
+  k.lpr_log2 = 0;
+  while ((4 << k.lpr_log2) < a.dims) k.lpr_log2++;
+  k.part = (double*)a.scratch;
+  int* counts = (int*)((char*)a.scratch + (int64_t)PL_BLOCKS * (a.dims + 4) * 8);
+  k.counts = counts; k.ncounts = 0;
+  if (a.d_mean && a.valid && !a.count && a.rows > 0) {
+    long long per = (a.rows + PL_COUNTS - 1) / PL_COUNTS;
+    if (per < 4096) per = 4096;
+    k.ncounts = (int)((a.rows + per - 1) / per);
+    hipLaunchKernelGGL(hoic_count_valid_kernel, dim3(k.ncounts), dim3(256), 0, st, a.valid, (long long)a.rows, per, counts);
+  }
+  const int rpb = PL_NT >> k.lpr_log2;
+  const int nb = (int)std::max<long long>(1, std::min<long long>(PL_BLOCKS, (a.rows + rpb - 1) / rpb));
+  if (a.t_mean == HOIC_F32) launch_policy_loss<float, float>(k, nb, st);
+  else if (a.t_mean == HOIC_F16) { if (a.t_act == HOIC_F32) launch_policy_loss<_Float16, float>(k, nb, st); else launch_policy_loss<_Float16, _Float16>(k, nb, st); }
+  else { if (a.t_act == HOIC_F32) launch_policy_loss<__bf16, float>(k, nb, st); else launch_policy_loss<__bf16, __bf16>(k, nb, st); }
+  const bool sum_ls = a.d_log_std && a.ld_std == 0;
+  if (!a.count || sum_ls) {
+    hipLaunchKernelGGL(hoic_policy_loss_finish_kernel, dim3(sum_ls ? 1 + (a.dims + 7) / 8 : 1), dim3(256), 0, st, k, nb);
+  }
+  MCHK(hipGetLastError());
+  return HOIC_OK;
+}
+
+// ---------------------------------------------------------------------------------------------- lists of tensors
+// A list's tensors travel in the kernel arguments (<= LIST_MAX a launch), so that a call needs no table in device memory, no
+// copy to it, and can be captured into a graph as it is.  A workgroup takes one chunk of one tensor.
+template <class E, int MAXT> __device__ __forceinline__ int list_find(const E (&t)[MAXT], int nt, int block) {
+  int lo = 0, hi = nt - 1;
+  while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (t[mid].first <= block) lo = mid; else hi = mid - 1; }
+  return lo;
+}
+
+// sqrt(sum g^2) over a list: 64-bit partial sums per workgroup, joined in fixed order by one workgroup; the factor
+// min(1, bound / (norm + 1e-6)) beside it.
+struct NormEntry { const void* g; long long n; int first; };
+#define NORM_MAX 120
+struct NormArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; double* part; };
+template <class T> __device__ __forceinline__ double sumsq(const T* g, long long i0, long long i1) {
+  double s = 0.;
+  for (long long i = i0 + threadIdx.x * 4; i < i1; i += 1024) {
+    const long long l = i1 - i;
+    const f32x4 x = load4(g + i, l < 4 ? (int)l : 4);
+#pragma unroll
+    for (int e = 0; e < 4; e++) s = fma((double)x[e], (double)x[e], s);
+  }
+  return s;
+}
+__global__ __launch_bounds__(256) void hoic_sumsq_kernel(NormArgs a) {
+  __shared__ double red[4];
+  const int t = list_find(a.t, a.nt, blockIdx.x);
+  const long long i0 = (long long)(blockIdx.x - a.t[t].first) * a.chunk, i1 = i0 + a.chunk < a.t[t].n ? i0 + a.chunk : a.t[t].n;
+  double s = a.type == HOIC_F32 ? sumsq((const float*)a.t[t].g, i0, i1) : a.type == HOIC_F16 ? sumsq((const _Float16*)a.t[t].g, i0, i1) : sumsq((const __bf16*)a.t[t].g, i0, i1);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) a.part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+__global__ __launch_bounds__(1024) void hoic_norm_finish_kernel(const double* __restrict__ part, long long nparts, double bound, double* __restrict__ clip, float* __restrict__ norm) {
+  __shared__ double red[16];
+  double s = 0.;
+  for (long long i = threadIdx.x; i < nparts; i += 1024) s += part[i];
+#pragma unroll
+  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.;
+    for (int w = 0; w < 16; w++) t += red[w];
+    t = sqrt(t);
+    const double c = bound / (t + 1e-6);
+    clip[0] = t;
+    clip[1] = c > 1. ? 1. : c;       // (a NaN norm leaves a NaN factor)
+    *norm = (float)t;
+  }
+}
+// g *= factor where it is not 1
+struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; const double* clip; };
+template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, float c) {
+  for (long long i = i0 + threadIdx.x * 4; i < i1; i += 1024) {
+    const int l = i1 - i < 4 ? (int)(i1 - i) : 4;
+    f32x4 x = load4(g + i, l);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] *= c;
+    store4(g + i, l, x);
+  }
+}
+__global__ __launch_bounds__(256) void hoic_scale_kernel(ScaleArgs a) {
+  const double c = a.clip[1];
+  if (c == 1.) return;
+  const int t = list_find(a.t, a.nt, blockIdx.x);
+  const long long i0 = (long long)(blockIdx.x - a.t[t].first) * a.chunk, i1 = i0 + a.chunk < a.t[t].n ? i0 + a.chunk : a.t[t].n;
+  if (a.type == HOIC_F32) scale_list((float*)a.t[t].g, i0, i1, (float)c);
+  else if (a.type == HOIC_F16) scale_list((_Float16*)a.t[t].g, i0, i1, (float)c);
+  else scale_list((__bf16*)a.t[t].g, i0, i1, (float)c);
+}
+// elements a workgroup: at least 8192, at most ~2048 workgroups (= parts) a list beyond one per tensor
+static long long norm_chunk(const int64_t* n, int32_t nt) {
+  long long tot = 0;
+  for (int i = 0; i < nt; i++) tot += n[i];
+  const long long c = (tot + 2047) / 2048;
+  return std::max<long long>(8192, (c + 1023) / 1024 * 1024);
+}
+static long long norm_parts(const int64_t* n, int32_t nt, long long chunk) {
+  long long p = 0;
+  for (int i = 0; i < nt; i++) p += (n[i] + chunk - 1) / chunk;
+  return p;
+}
+static int32_t norm_check(const char* who, const void* const* g, const int64_t* n, int32_t nt, int32_t type) {
+  if (nt < 0 || (nt > 0 && (!g || !n)) || (type != HOIC_F32 && type != HOIC_F16 && type != HOIC_BF16)) { hoic_set_error(std::string(who) + ": bad list or type"); return HOIC_ERR_ARG; }
+  for (int i = 0; i < nt; i++) if (n[i] < 0 || (n[i] > 0 && !g[i])) { hoic_set_error(std::string(who) + ": a tensor without memory or with a negative size"); return HOIC_ERR_ARG; }
+  return HOIC_OK;
+}
+extern "C" int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt) {
+  if (nt < 0 || (nt > 0 && !n)) return -1;
+  return norm_parts(n, nt, norm_chunk(n, nt));
+}
+extern "C" int32_t hoic_grad_norm_partial(const void* const* g, const int64_t* n, int32_t nt, int32_t type, double* d_part, void* stream) {
+  const int32_t rc = norm_check("hoic_grad_norm_partial", g, n, nt, type);
+  if (rc != HOIC_OK) return rc;
+  if (!d_part) { hoic_set_error("hoic_grad_norm_partial: no place for the partial sums"); return HOIC_ERR_ARG; }
+  NormArgs a;
+  a.type = type; a.chunk = norm_chunk(n, nt); a.part = d_part;
+  for (int i = 0; i < nt;) {
+    long long blocks = 0;
+    for (a.nt = 0; i < nt && a.nt < NORM_MAX; i++) {
+      if (n[i] == 0) continue;
+      a.t[a.nt].g = g[i]; a.t[a.nt].n = n[i]; a.t[a.nt].first = (int)blocks; a.nt++;
+      blocks += (n[i] + a.chunk - 1) / a.chunk;
+    }
+    if (blocks) hipLaunchKernelGGL(hoic_sumsq_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+    a.part += blocks;
+  }
+  MCHK(hipGetLastError());
+  return HOIC_OK;
+}
+extern "C" int32_t hoic_grad_norm_finish(const double* d_part, int64_t nparts, double bound, double* d_clip, float* d_norm, void* stream) {
+  if (nparts < 0 || (nparts > 0 && !d_part) || !d_clip || !d_norm || !(bound >= 0.)) { hoic_set_error("hoic_grad_norm_finish: bad arguments"); return HOIC_ERR_ARG; }
+  hipLaunchKernelGGL(hoic_norm_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, d_part, (long long)nparts, bound, d_clip, d_norm);
+  MCHK(hipGetLastError());
+  return HOIC_OK;
+}
+extern "C" int32_t hoic_scale_list(void* const* g, const int64_t* n, int32_t nt, int32_t type, const double* d_clip, void* stream) {
+  const int32_t rc = norm_check("hoic_scale_list", (const void* const*)g, n, nt, type);
+  if (rc != HOIC_OK) return rc;
+  if (!d_clip) { hoic_set_error("hoic_scale_list: no factor"); return HOIC_ERR_ARG; }
+  ScaleArgs a;
+  a.type = type; a.chunk = norm_chunk(n, nt); a.clip = d_clip;
+  for (int i = 0; i < nt;) {
+    long long blocks = 0;
+    for (a.nt = 0; i < nt && a.nt < NORM_MAX; i++) {
+      if (n[i] == 0) continue;
+      a.t[a.nt].g = g[i]; a.t[a.nt].n = n[i]; a.t[a.nt].first = (int)blocks; a.nt++;
+      blocks += (n[i] + a.chunk - 1) / a.chunk;
+    }
+    if (blocks) hipLaunchKernelGGL(hoic_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+  }
+  MCHK(hipGetLastError());
+  return HOIC_OK;
+}
+
+// ---------------------------------------------------------------------------------------------- AdamW
+//   m' = b1 m + (1 - b1) c g,   v' = b2 v + (1 - b2) (c g)^2,
+//   p' = p - (lr wd p + lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps))
+// (the weight decay is part of the subtracted step: 1 - lr wd itself, rounded to float32, would lose most of a small lr wd).
+// c: the clipping factor; a norm that is not finite leaves parameters and states as they are.
+//
+// 8-bit states: blocks of 256 elements in storage order, one power-of-two scale k per block and state,
+//   m: sign + e4m3 (value / k below 2^8, smallest step 2^-9),  v: e5m3 without sign (below 2^16, smallest step 2^-17).
+// Stochastic rounding: v moves by 0.1 % a step at b2 = 0.999 and a 3-bit mantissa by 6 to 12 %, so that nearest rounding would hold
+// it for ever; rounding up with the probability of the part cut off keeps its mean.  A power-of-two scale leaves stored values on
+// the grid when the block's maximum moves, so that only the step's change is rounded.  v > 0 is never stored as 0 (m / eps
+// would follow).  The random numbers are a hash of (seed, step, tensor, element): the same on every rank and in every replay.
+// m', v' and the place of a value between two codes are in 64 bits: a float32 rounding there moves a value by a whole code.
+// Codes of values that are not finite: m 0x7f, v 0xff (such an element does not touch its block's scale).
+struct AdamEntry { void* p; const void* g; void* m; void* v; float* ms; float* vs; long long n; float size, rroot; unsigned key; int first; };
+#define ADAM_MAX 48
+struct AdamArgs {
+  AdamEntry t[ADAM_MAX];
+  int nt, at;                    // entries of this launch; place of the first one in the call's list
+  float b1, c1, b2, c2, eps, lrwd;
+  double b1d, c1d, b2d, c2d;
+  const double* clip;            // {norm, factor} or NULL
+  const float* consts;           // {step size, 1 / sqrt(1 - b2^t), key, lr * wd} per entry of the call (step on the device), or NULL
+};
+__host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
+  x ^= x >> 17; x *= 0x743b8c43u;
+  x ^= x >> 12; x *= 0xab2209abu;
+  return x ^ (x >> 15);
+}
+__host__ __device__ __forceinline__ unsigned adam_key(unsigned seed, unsigned step, unsigned ordinal) { return mix32(mix32(mix32(seed) + step) + ordinal); }
+struct AdamConsts { float size, rroot, lrwd; unsigned key; };
+__device__ __forceinline__ AdamConsts adam_consts(const AdamArgs& a, int t) {
+  AdamConsts c;
+  if (a.consts) {
+    const float* k = a.consts + 4 * (a.at + t);
+    c.size = k[0]; c.rroot = k[1]; c.key = __builtin_bit_cast(unsigned, k[2]); c.lrwd = k[3];
+  } else {
+    c.size = a.t[t].size; c.rroot = a.t[t].rroot; c.key = a.t[t].key; c.lrwd = a.lrwd;
+  }
+  return c;
+}
+__device__ __forceinline__ float adam_param(float p, float m, float v, const AdamConsts& c, float eps) {
+  const float u = c.size * m / fmaf(sqrtf(v), c.rroot, eps);
+  return p - fmaf(c.lrwd, p, u);
+}
+#define ADAM32_CHUNK 4096
+template <class T> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(AdamArgs a) {
+  const int t = list_find(a.t, a.nt, blockIdx.x);
+  float cl = 1.f;
+  if (a.clip) { if (!(a.clip[0] < INFINITY)) return; cl = (float)a.clip[1]; }
+  const AdamConsts c = adam_consts(a, t);
+  T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; float* m = (float*)a.t[t].m; float* v = (float*)a.t[t].v;
+  const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM32_CHUNK, left = a.t[t].n - i0;
+#pragma unroll
+  for (int u = 0; u < ADAM32_CHUNK / 1024; u++) {
+    const long long o = u * 1024 + threadIdx.x * 4;
+    if (o >= left) break;
+    const int l = left - o < 4 ? (int)(left - o) : 4;
+    const long long i = i0 + o;
+    f32x4 pp = load4(p + i, l), gg = load4(g + i, l), mm = load4(m + i, l), vv = load4(v + i, l);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float x = gg[e] * cl;
+      mm[e] = fmaf(a.b1, mm[e], a.c1 * x);
+      vv[e] = fmaf(a.b2, vv[e], a.c2 * x * x);
+      pp[e] = adam_param(pp[e], mm[e], vv[e], c, a.eps);
+    }
+    store4(m + i, l, mm); store4(v + i, l, vv); store4(p + i, l, pp);
+  }
+}
+__device__ __forceinline__ unsigned hi32(double x) { return (unsigned)(__builtin_bit_cast(unsigned long long, x) >> 32); }
+__device__ __forceinline__ double pow2d(int e) { return __builtin_bit_cast(double, (unsigned long long)(1023 + e) << 52); }
+__device__ __forceinline__ float pow2f(int e) { return __builtin_bit_cast(float, (unsigned)(127 + e) << 23); }
+// A code's value: exponent field and 3 mantissa bits moved to a float32's places, then the difference of the biases (exact, the
+// smallest codes included: they are float32 subnormals before the multiplication).
+__device__ __forceinline__ float m_value(unsigned c) {
+  const float x = __builtin_bit_cast(float, (c & 0x7f) << 20) * pow2f(120);
+  return (c & 0x7f) == 0x7f ? __builtin_nanf("") : (c & 0x80) ? -x : x;
+}
+__device__ __forceinline__ float v_value(unsigned c) { return c == 0xff ? __builtin_nanf("") : __builtin_bit_cast(float, c << 20) * pow2f(112); }
+// y >= 0 in units of the scale -> code, rounded up with the probability of the part cut off: 20 mantissa bits are in the
+// high word, 3 stay, the 17 below them plus (2 r + 1) of 2^17 carry or do not (r: 16 random bits).  Below the smallest normal
+// 2^low one 2^low is added: the step there is the same as in the binade above, the code counts from 0.
+__device__ __forceinline__ unsigned code8(double y, int low, unsigned r16) {
+  const bool sub = y < pow2d(low);
+  const double z = sub ? y + pow2d(low) : y;
+  return ((hi32(z) + 2 * r16 + 1) >> 17) - (unsigned)(1023 + low - (sub ? 0 : 1)) * 8;
+}
+#define ADAM8_CHUNK 4096
+template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(AdamArgs a) {
+  const int t = list_find(a.t, a.nt, blockIdx.x);
+  double cl = 1.;
+  if (a.clip) { if (!(a.clip[0] < INFINITY)) return; cl = a.clip[1]; }
+  const AdamConsts c = adam_consts(a, t);
+  T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; unsigned char* m = (unsigned char*)a.t[t].m; unsigned char* v = (unsigned char*)a.t[t].v;
+  const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM8_CHUNK, left = a.t[t].n - i0;
+  const unsigned key = mix32(c.key + (unsigned)(i0 >> 32));
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int u = 0; u < ADAM8_CHUNK / 1024; u++) {
+    const long long ob = (u * 4 + wave) * 256;
+    if (ob >= left) break;                                          // (wavefront-uniform)
+    const long long o = ob + lane * 4, i = i0 + o, blk = (i0 + ob) >> 8;
+    const int l = left - o >= 4 ? 4 : left - o > 0 ? (int)(left - o) : 0;
+    f32x4 pp = load4(p + (l ? i : 0), l), gg = load4(g + (l ? i : 0), l);
+    unsigned cm = 0, cv = 0;
+    if (l == 4) { cm = *(const unsigned*)(m + i); cv = *(const unsigned*)(v + i); }
+    else for (int e = 0; e < l; e++) { cm |= (unsigned)m[i + e] << (8 * e); cv |= (unsigned)v[i + e] << (8 * e); }
+    const double km = (double)a.t[t].ms[blk], kv = (double)a.t[t].vs[blk];
+    double mm[4], vv[4];
+    unsigned hm = 0, hv = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const double x = (double)gg[e] * cl;
+      mm[e] = fma(a.b1d, (double)m_value((cm >> (8 * e)) & 0xff) * km, a.c1d * x);
+      vv[e] = fma(a.b2d, (double)v_value((cv >> (8 * e)) & 0xff) * kv, a.c2d * x * x);
+      if (vv[e] > 3.4028234663852886e38 && vv[e] < INFINITY) vv[e] = 3.4028234663852886e38;
+      const unsigned am = hi32(mm[e]) & 0x7fffffffu, av = hi32(vv[e]);
+      if (am < 0x7ff00000u && am > hm) hm = am;
+      if (av < 0x7ff00000u && av > hv) hv = av;
+      pp[e] = adam_param(pp[e], (float)mm[e], (float)vv[e], c, a.eps);
+    }
+#pragma unroll
+    for (int q = 32; q; q >>= 1) { hm = max(hm, (unsigned)__shfl_xor((int)hm, q, 64)); hv = max(hv, (unsigned)__shfl_xor((int)hv, q, 64)); }
+    const int em = max((int)(hm >> 20) - 1023 - 7, -126), ev = max((int)(hv >> 20) - 1023 - 15, -126);
+    const double rm = pow2d(-em), rv = pow2d(-ev);
+    unsigned om = 0, ov = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const unsigned h = mix32((unsigned)(i + e) + key);
+      unsigned qm = code8(fabs(mm[e]) * rm, -6, h & 0xffff) | (mm[e] < 0. ? 0x80u : 0u);
+      unsigned qv = code8(vv[e] * rv, -14, h >> 16);
+      qv = qv == 0 && vv[e] > 0. ? 1u : qv;
+      qm = (hi32(mm[e]) & 0x7ff00000u) == 0x7ff00000u ? 0x7fu : qm;
+      qv = (hi32(vv[e]) & 0x7ff00000u) == 0x7ff00000u ? 0xffu : qv;
+      om |= qm << (8 * e); ov |= qv << (8 * e);
+    }
+    if (l == 4) { *(unsigned*)(m + i) = om; *(unsigned*)(v + i) = ov; }
+    else for (int e = 0; e < l; e++) { m[i + e] = (unsigned char)(om >> (8 * e)); v[i + e] = (unsigned char)(ov >> (8 * e)); }
+    store4(p + i, l, pp);
+    if (lane == 0) { a.t[t].ms[blk] = pow2f(em); a.t[t].vs[blk] = pow2f(ev); }
+  }
+}
+// the float32 values of 8-bit states: p, g of an entry are the places of m's and v's values
+__global__ __launch_bounds__(256) void hoic_adamw_values_kernel(AdamArgs a) {
+  const int t = list_find(a.t, a.nt, blockIdx.x);
+  float* om = (float*)a.t[t].p; float* ov = (float*)(uintptr_t)a.t[t].g;
+  const unsigned char* m = (const unsigned char*)a.t[t].m; const unsigned char* v = (const unsigned char*)a.t[t].v;
+  const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM8_CHUNK, left = a.t[t].n - i0;
+#pragma unroll
+  for (int u = 0; u < ADAM8_CHUNK / 1024; u++) {
+    const long long o = u * 1024 + threadIdx.x * 4, i = i0 + o;
+    if (o >= left) break;
+    const int l = left - o < 4 ? (int)(left - o) : 4;
+    unsigned cm = 0, cv = 0;
+    if (l == 4) { cm = *(const unsigned*)(m + i); cv = *(const unsigned*)(v + i); }
+    else for (int e = 0; e < l; e++) { cm |= (unsigned)m[i + e] << (8 * e); cv |= (unsigned)v[i + e] << (8 * e); }
+    const float km = a.t[t].ms[i >> 8], kv = a.t[t].vs[i >> 8];
+    f32x4 x, y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) { x[e] = m_value((cm >> (8 * e)) & 0xff) * km; y[e] = v_value((cv >> (8 * e)) & 0xff) * kv; }
+    store4(om + i, l, x); store4(ov + i, l, y);
+  }
+}
+// a captured step counts on the device: step += 1, then the constants that depend on it
+struct AdamCount { int* step[ADAM_MAX]; unsigned ordinal[ADAM_MAX]; int nt, at; double lr; const float* d_lr; double b1, b2, wd; unsigned seed; float* consts; };
+__global__ __launch_bounds__(64) void hoic_adamw_count_kernel(AdamCount a) {
+  const int t = threadIdx.x;
+  if (t >= a.nt) return;
+  const int s = *a.step[t] + 1;
+  *a.step[t] = s;
+  const double lr = a.d_lr ? (double)*a.d_lr : a.lr;
+  float* k = a.consts + 4 * (a.at + t);
+  k[0] = (float)(lr / (1. - pow(a.b1, (double)s)));
+  k[1] = (float)(1. / sqrt(1. - pow(a.b2, (double)s)));
+  k[2] = __builtin_bit_cast(float, adam_key(a.seed, (unsigned)s, a.ordinal[t]));
+  k[3] = (float)(lr * a.wd);
+}
+extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic_adamw_args* x, void* stream) {
+  if (nt < 0 || (nt > 0 && !t) || !x || (x->type != HOIC_F32 && x->type != HOIC_F16 && x->type != HOIC_BF16) || (x->state_bits != 32 && x->state_bits != 8)
+      || !(x->b1 >= 0. && x->b1 < 1.) || !(x->b2 >= 0. && x->b2 < 1.) || !(x->eps >= 0.)) {
+    hoic_set_error("hoic_adamw: bad list, type, state_bits (8 or 32), betas or eps"); return HOIC_ERR_ARG;
+  }
+  for (int i = 0; i < nt; i++) {
+    const hoic_adamw_tensor& e = t[i];
+    if (e.n < 0 || (e.n > 0 && (!e.p || !e.g || !e.m || !e.v || (x->state_bits == 8 && (!e.m_scale || !e.v_scale)))) || (x->d_consts ? !e.d_step : e.step < 1)
+        || (e.n + ADAM32_CHUNK - 1) / ADAM32_CHUNK > 0x7fffffff / ADAM_MAX) {
+      hoic_set_error("hoic_adamw: a tensor without memory, state or step count, or too large"); return HOIC_ERR_ARG;
+    }
+  }
+  static_assert(ADAM8_CHUNK == ADAM32_CHUNK, "one chunk size for the launch below");
+  hipStream_t st = (hipStream_t)stream;
+  AdamArgs a;
+  a.b1 = (float)x->b1; a.c1 = (float)(1. - x->b1); a.b2 = (float)x->b2; a.c2 = (float)(1. - x->b2); a.eps = (float)x->eps; a.lrwd = (float)(x->lr * x->weight_decay);
+  a.b1d = x->b1; a.c1d = 1. - x->b1; a.b2d = x->b2; a.c2d = 1. - x->b2; a.clip = x->d_clip; a.consts = x->d_consts;
+  a.at = 0;
+  for (int i = 0; i < nt;) {
+    long long blocks = 0;
+    AdamCount cnt;
+    for (a.nt = 0; i < nt && a.nt < ADAM_MAX; i++) {
+      const hoic_adamw_tensor& e = t[i];
+      if (e.n == 0) continue;
+      AdamEntry& o = a.t[a.nt];
+      o.p = e.p; o.g = e.g; o.m = e.m; o.v = e.v; o.ms = e.m_scale; o.vs = e.v_scale; o.n = e.n; o.first = (int)blocks;
+      if (x->d_consts) { o.size = o.rroot = 0.f; o.key = 0; cnt.step[a.nt] = e.d_step; cnt.ordinal[a.nt] = (unsigned)e.ordinal; }
+      else {
+        o.size = (float)(x->lr / (1. - pow(x->b1, (double)e.step)));
+        o.rroot = (float)(1. / sqrt(1. - pow(x->b2, (double)e.step)));
+        o.key = adam_key(x->seed, (unsigned)e.step, (unsigned)e.ordinal);
+      }
+      blocks += (e.n + ADAM32_CHUNK - 1) / ADAM32_CHUNK;
+      a.nt++;
+    }
+    if (!blocks) continue;
+    if (x->d_consts) {
+      cnt.nt = a.nt; cnt.at = a.at; cnt.lr = x->lr; cnt.d_lr = x->d_lr; cnt.b1 = x->b1; cnt.b2 = x->b2; cnt.wd = x->weight_decay; cnt.seed = x->seed; cnt.consts = x->d_consts;
+      hipLaunchKernelGGL(hoic_adamw_count_kernel, dim3(1), dim3(64), 0, st, cnt);
+    }
+    const dim3 grid((unsigned)blocks), block(256);
+    if (x->state_bits == 32) {
+      if (x->type == HOIC_F32) hipLaunchKernelGGL(hoic_adamw32_kernel<float>, grid, block, 0, st, a);
+      else if (x->type == HOIC_F16) hipLaunchKernelGGL(hoic_adamw32_kernel<_Float16>, grid, block, 0, st, a);
+      else hipLaunchKernelGGL(hoic_adamw32_kernel<__bf16>, grid, block, 0, st, a);
+    } else {
+      if (x->type == HOIC_F32) hipLaunchKernelGGL(hoic_adamw8_kernel<float>, grid, block, 0, st, a);
+      else if (x->type == HOIC_F16) hipLaunchKernelGGL(hoic_adamw8_kernel<_Float16>, grid, block, 0, st, a);
+      else hipLaunchKernelGGL(hoic_adamw8_kernel<__bf16>, grid, block, 0, st, a);
+    }
+    a.at += a.nt;
+  }
+  MCHK(hipGetLastError());
+  return HOIC_OK;
+}
+extern "C" int32_t hoic_adamw_values(const hoic_adamw_tensor* t, int32_t nt, void* stream) {
+  if (nt < 0 || (nt > 0 && !t)) { hoic_set_error("hoic_adamw_values: bad list"); return HOIC_ERR_ARG; }
+  for (int i = 0; i < nt; i++)
+    if (t[i].n < 0 || (t[i].n > 0 && (!t[i].p || !t[i].g || !t[i].m || !t[i].v || !t[i].m_scale || !t[i].v_scale)) || (t[i].n + ADAM8_CHUNK - 1) / ADAM8_CHUNK > 0x7fffffff / ADAM_MAX) {
+      hoic_set_error("hoic_adamw_values: a tensor without memory, or too large"); return HOIC_ERR_ARG;
+    }
+  AdamArgs a;
+  for (int i = 0; i < nt;) {
+    long long blocks = 0;
+    for (a.nt = 0; i < nt && a.nt < ADAM_MAX; i++) {
+      if (t[i].n == 0) continue;
+      AdamEntry& o = a.t[a.nt++];
+      o.p = t[i].p; o.g = t[i].g; o.m = t[i].m; o.v = t[i].v; o.ms = t[i].m_scale; o.vs = t[i].v_scale; o.n = t[i].n; o.first = (int)blocks;
+      blocks += (t[i].n + ADAM8_CHUNK - 1) / ADAM8_CHUNK;
+    }
+    if (blocks) hipLaunchKernelGGL(hoic_adamw_values_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+  }
+  MCHK(hipGetLastError());
+  return HOIC_OK;
+}

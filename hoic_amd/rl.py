@@ -9,6 +9,7 @@ and the PPO-clip loss (uhc/khrylib/rl/agents/agent_ppo.py:58-64).
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -173,6 +174,204 @@ def ppo_loss(policy, states, actions, advantages, fixed_log_probs, clip_epsilon,
     surr1 = ratio * advantages
     surr2 = torch.clamp(ratio, 1.0 - clip_epsilon, 1.0 + clip_epsilon) * advantages
     return -torch.min(surr1, surr2).mean()
+
+
+class PolicyLoss(NamedTuple):
+    """``loss`` scalar; ``info`` [4]: surrogate, KL, share of rows without gradient (clipped), number of valid rows;
+    ``log_probs`` [M, 1] when no old ones were given"""
+    loss: torch.Tensor
+    info: torch.Tensor
+    log_probs: torch.Tensor | None
+
+
+class PolicyLossGrad(NamedTuple):
+    """PolicyLoss with the gradients of weight * loss"""
+    loss: torch.Tensor
+    info: torch.Tensor
+    d_mean: torch.Tensor
+    d_log_std: torch.Tensor
+    log_probs: torch.Tensor | None
+
+
+_LOSS_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}         # enum hoic_type
+
+
+def _loss_inputs(mean, log_std, actions, advantages, fixed, clip_epsilon, ref_mean, ref_log_std, kl_coef, valid):
+    """Checks of the policy loss's arguments; row tensors come back with unit stride along the dimensions, vectors flat."""
+    if mean.dim() != 2 or mean.shape[1] < 1:
+        raise ValueError(f"mean must be [rows, dimensions], not {tuple(mean.shape)}")
+    M, N = mean.shape
+    dev = mean.device
+
+    def rows(t, name, types, shared=False):
+        if shared and t.dim() == 1:
+            t = t[None]
+        if t.dim() != 2 or t.shape[1] != N or (t.shape[0] != M and not (shared and t.shape[0] == 1)):
+            raise ValueError(f"{name}: {tuple(t.shape)} for means of {(M, N)}")
+        if t.device != dev or t.dtype not in types:
+            raise ValueError(f"{name}: {t.dtype} on {t.device}; wanted {' or '.join(str(x) for x in types)} on {dev}")
+        if shared and t.shape[0] > 1 and t.stride(0) == 0:
+            t = t.contiguous()                     # a row expanded over the batch: its gradient has a value per row
+        return t if t.stride(1) == 1 or N == 1 else t.contiguous()
+
+    def flat(t, name, types):
+        if t.numel() != M or t.device != dev or t.dtype not in types:
+            raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device} for {M} rows on {dev}")
+        return t.reshape(-1).contiguous()
+
+    f32 = torch.float32 if mean.dtype != torch.float64 else torch.float64
+    own, wide = (mean.dtype,), (mean.dtype, f32)
+    if not mean.dtype.is_floating_point:
+        raise ValueError(f"mean: a floating type, not {mean.dtype}")
+    if (ref_mean is None) != (ref_log_std is None):
+        raise ValueError("the reference policy is ref_mean and ref_log_std together")
+    if ref_mean is None and kl_coef:
+        raise ValueError("kl_coef needs a reference policy (ref_mean, ref_log_std)")
+    lo, hi = clip_epsilon if isinstance(clip_epsilon, (tuple, list)) else (clip_epsilon, clip_epsilon)
+    if not (0.0 <= lo < math.inf and 0.0 <= hi < math.inf and math.isfinite(kl_coef)):
+        raise ValueError(f"clip_epsilon {clip_epsilon} (>= 0) or kl_coef {kl_coef}")
+    mean, actions = rows(mean, "mean", own), rows(actions, "actions", wide)
+    log_std = rows(log_std, "log_std", wide, True)
+    advantages = flat(advantages, "advantages", (f32,))
+    fixed = None if fixed is None else flat(fixed, "fixed_log_probs", (f32,))
+    if ref_mean is not None:
+        ref_mean, ref_log_std = rows(ref_mean, "ref_mean", own).detach(), rows(ref_log_std, "ref_log_std", (log_std.dtype,), True).detach()
+    valid = None if valid is None else flat(valid, "valid", (torch.bool, torch.uint8))
+    return mean, log_std, actions, advantages, fixed, (float(lo), float(hi)), ref_mean, ref_log_std, valid
+
+
+def _policy_loss_launch(x, kl_coef, weight, grad, upstream=None, count=None):
+    """hoic_policy_loss on checked inputs -> (out [8] or None, d_mean, d_log_std [1 or M, N], log_probs)"""
+    from . import lib
+    import ctypes as C
+    mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid = x
+    M, N = mean.shape
+    if N > 256:
+        raise ValueError(f"the policy loss's kernel takes up to 256 action dimensions, not {N}")
+    L, dev = lib.load(), mean.device
+    if M == 0:
+        zeros = lambda *shape, dtype=torch.float32: torch.zeros(shape, dtype=dtype, device=dev)
+        return (zeros(8) if count is None else None, zeros(0, N, dtype=mean.dtype) if grad else None,
+                zeros(*log_std.shape, dtype=log_std.dtype) if grad else None, zeros(0, 1) if fixed is None and count is None else None)
+    a = lib.PolicyLossArgs()
+    new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=dev)
+    scratch = new((int(L.hoic_policy_loss_scratch_bytes(N)),), torch.uint8)
+    out = new((8,), torch.float32) if count is None else None
+    d_mean = new((M, N), mean.dtype) if grad else None
+    d_log_std = new(log_std.shape, log_std.dtype) if grad else None
+    log_probs = new((M, 1), torch.float32) if fixed is None and count is None else None
+    a.rows, a.dims = M, N
+    a.t_mean, a.t_act, a.t_std = _LOSS_TYPES[mean.dtype], _LOSS_TYPES[actions.dtype], _LOSS_TYPES[log_std.dtype]
+    # (a leading 1 is a shared row: stride 0; so is [M, N] = [1, N])
+    ld = lambda t: 0 if t.shape[0] == 1 else t.stride(0)
+    for name, t in (("mean", mean), ("act", actions), ("log_std", log_std), ("ref_mean", ref_mean), ("ref_log_std", ref_log_std), ("adv", advantages),
+                    ("fixed", fixed), ("valid", valid), ("upstream", upstream), ("count", count), ("d_mean", d_mean), ("d_log_std", d_log_std),
+                    ("log_probs", log_probs), ("out", out), ("scratch", scratch)):
+        setattr(a, name, None if t is None else t.data_ptr())
+    a.ld_mean, a.ld_act, a.ld_std, a.ld_dmean = mean.stride(0), actions.stride(0), ld(log_std), N
+    if ref_mean is not None:
+        a.ld_ref_mean, a.ld_ref_std = ref_mean.stride(0), ld(ref_log_std)
+    (a.clip_lo, a.clip_hi), a.kl_coef, a.weight = clip, float(kl_coef), float(weight)
+    with torch.cuda.device(dev):
+        rc = L.hoic_policy_loss(C.byref(a), C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+    if rc != 0:
+        raise lib.HoicError(f"hoic_policy_loss failed ({rc}): {L.hoic_last_error().decode()}")
+    return out, d_mean, d_log_std, log_probs
+
+
+class _ClippedPolicyLoss(torch.autograd.Function):
+    """Value in the forward call; the backward call makes the gradients from the same inputs, scaled by the incoming one on the
+    device (a gradient made in the forward call would have to be written, read and written again)."""
+
+    @staticmethod
+    def forward(ctx, kl_coef, clip, mean, log_std, *rest):
+        actions, advantages, fixed, ref_mean, ref_log_std, valid = rest
+        out, _, _, log_probs = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0, False)
+        ctx.save_for_backward(mean, log_std, *rest)
+        ctx.consts, ctx.count = (kl_coef, clip), out[6:].view(torch.float64)
+        loss, info = out[0], out[1:5]
+        ctx.mark_non_differentiable(*((info,) if log_probs is None else (info, log_probs)))
+        return loss, info, log_probs
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, *_):
+        mean, log_std, actions, advantages, fixed, ref_mean, ref_log_std, valid = ctx.saved_tensors
+        kl_coef, clip = ctx.consts
+        _, d_mean, d_log_std, _ = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0,
+                                                      True, upstream=g.float().contiguous(), count=ctx.count)
+        return (None, None, d_mean, d_log_std) + (None,) * 6
+
+
+def _policy_loss_tensors(x, kl_coef):
+    """The loss as tensor operations (CPU and float64 tensors; what the kernel computes, row by row)"""
+    mean, log_std, actions, advantages, fixed, (lo, hi), ref_mean, ref_log_std, valid = x
+    if valid is not None:                          # rows outside the batch may hold anything: they are left out, not multiplied by 0
+        keep = valid.bool()
+        cut = lambda t: t if t is None or (t.shape[0] != keep.shape[0]) else t[keep]
+        shared = log_std.shape[0] == 1
+        mean, actions, advantages, fixed, ref_mean = cut(mean), cut(actions), cut(advantages), cut(fixed), cut(ref_mean)
+        log_std, ref_log_std = log_std if shared else cut(log_std), ref_log_std if ref_log_std is None or ref_log_std.shape[0] == 1 else cut(ref_log_std)
+    n = max(mean.shape[0], 1)
+    mean_, s = (t.float() if t.dtype != torch.float64 else t for t in (mean, log_std))
+    lp = (-((actions.to(mean_.dtype) - mean_) ** 2) / (2 * torch.exp(2 * s)) - s - 0.5 * math.log(2 * math.pi)).sum(1)
+    r = torch.exp(lp - (lp.detach() if fixed is None else fixed))
+    s1, s2 = r * advantages, torch.clamp(r, 1.0 - lo, 1.0 + hi) * advantages
+    surr = -torch.min(s1, s2).sum() / n
+    kl = torch.zeros_like(surr)
+    if ref_mean is not None:
+        s0 = ref_log_std.to(s.dtype)
+        kl = (s - s0 + (torch.exp(2 * s0) + (mean_ - ref_mean.to(mean_.dtype)) ** 2) / (2 * torch.exp(2 * s)) - 0.5).sum() / n
+    with torch.no_grad():
+        clipped = (~((s1 < s2) | ((r >= 1.0 - lo) & (r <= 1.0 + hi)))).to(surr.dtype).sum() / n
+        log_probs = None
+        if fixed is None:
+            log_probs = lp.detach()[:, None]
+            if valid is not None:
+                log_probs = torch.zeros(valid.shape[0], 1, dtype=lp.dtype, device=lp.device).masked_scatter_(valid.bool()[:, None], log_probs)
+    info = torch.stack([surr.detach(), kl.detach(), clipped, torch.full_like(surr, float(mean.shape[0]))])
+    return PolicyLoss(surr + kl_coef * kl, info, log_probs)
+
+
+def _on_kernel(mean):
+    return mean.is_cuda and mean.dtype in _LOSS_TYPES
+
+
+def clipped_policy_loss(mean, log_std, actions, advantages, fixed_log_probs=None, clip_epsilon=0.2, *, ref_mean=None, ref_log_std=None,
+                        kl_coef=0.0, valid=None):
+    """PPO's clipped surrogate (``ppo_loss``; agent_ppo.py:58-64) plus ``kl_coef`` times KL(reference || policy), the mean over the
+    valid rows; differentiable in ``mean`` and ``log_std``.
+
+    mean, ref_mean [M, N] (N <= 256); actions [M, N] in the mean's type or float32; log_std [N] / [1, N] (shared by the rows: its
+    gradient is summed) or [M, N], float32 or the mean's type, ref_log_std alike; advantages, fixed_log_probs [M] or [M, 1]
+    float32; ``valid`` [M] bool: rows outside it take no part, whatever they hold.  ``fixed_log_probs`` None: the old policy
+    is this one (ratio 1), the log-probabilities come back for the later epochs.  ``clip_epsilon``: eps, or (lower, upper).
+    On the GPU one pass over the batch for the value and one for the gradient (hoic_policy_loss), per-row arithmetic and sums in
+    64 bits in a fixed order; CPU and float64 tensors take the tensor form.  Returns a ``PolicyLoss``."""
+    x = _loss_inputs(mean, log_std, actions, advantages, fixed_log_probs, clip_epsilon, ref_mean, ref_log_std, kl_coef, valid)
+    if not _on_kernel(mean):
+        return _policy_loss_tensors(x, kl_coef)
+    mean2, log_std2, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid = x
+    const = [None if t is None else t.detach() for t in (actions, advantages, fixed, ref_mean, ref_log_std, valid)]
+    return PolicyLoss(*_ClippedPolicyLoss.apply(float(kl_coef), clip, mean2, log_std2, *const))
+
+
+def clipped_policy_loss_grad(mean, log_std, actions, advantages, fixed_log_probs=None, clip_epsilon=0.2, *, ref_mean=None, ref_log_std=None,
+                             kl_coef=0.0, valid=None, weight=1.0):
+    """``clipped_policy_loss`` and the gradients of ``weight`` times it in one pass over the batch, without autograd.  Returns a
+    ``PolicyLossGrad``; d_log_std has log_std's shape."""
+    args = (actions, advantages, fixed_log_probs, clip_epsilon, ref_mean, ref_log_std, kl_coef, valid)
+    if not _on_kernel(mean):
+        _loss_inputs(mean, log_std, *args)
+        mu, s = mean.detach().requires_grad_(), log_std.detach().requires_grad_()
+        with torch.enable_grad():
+            loss, info, log_probs = _policy_loss_tensors(_loss_inputs(mu, s, *args), kl_coef)
+            d_mean, d_log_std = torch.autograd.grad(loss * weight, (mu, s))
+        return PolicyLossGrad(loss.detach(), info, d_mean, d_log_std, log_probs)
+    with torch.no_grad():
+        x = _loss_inputs(mean, log_std, *args)
+        out, d_mean, d_log_std, log_probs = _policy_loss_launch(x, kl_coef, weight, True)
+        return PolicyLossGrad(out[0], out[1:5], d_mean, d_log_std.view(log_std.shape), log_probs)
 
 
 # ----------------------------------------------------------------------------- observation filter

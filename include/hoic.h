@@ -343,6 +343,76 @@ int32_t hoic_mlp_slab_reduce(const float* d_slabs, int32_t S, int32_t rows, int3
 int32_t hoic_mlp_rowsum_packed(const void* d_P, int32_t rows, int32_t Cp, float* d_out, const int32_t* d_exps, int32_t slot,
                                void* stream);
 
+/* ---- the second half of a training step on any list of tensors: policy loss -> gradient norm -> AdamW.  No handle; every call
+ * is asynchronous on `stream`, launches on the current device and can be captured into a HIP graph. */
+enum hoic_type { HOIC_F32 = 0, HOIC_F16 = 1, HOIC_BF16 = 2 };
+/* hoic_policy_loss: the clipped policy loss of a Gaussian policy with a KL term (agent_ppo.py:46-64 with policy_gaussian.py:27-33,
+ * distributions.py:11-22; the KL term is PPO's penalty form, which the reference does not have).  Rows m, dimensions j < dims
+ * <= 256; s = log_std, l = sum_j log N(act; mean, e^s), r = e^(l - fixed) (fixed NULL: r = 1, the old policy is this one),
+ *   S = -min(r adv, clip(r, 1 - clip_lo, 1 + clip_hi) adv),  K = KL(reference || policy),  L = sum over valid rows (S + kl_coef K) / n,
+ * n = number of valid rows (valid NULL: all; no valid row: L = 0 and no gradient).  Rows outside `valid` may hold anything.
+ *   mean, ref_mean  t_mean, row strides ld_* in elements;  act  t_mean or float32;
+ *   log_std, ref_log_std  float32 or t_mean, row stride 0: one row shared by all;  ref_* both or neither
+ *   adv, fixed [rows] float32;  valid [rows] bytes
+ *   d_mean  NULL: value only;  else weight * upstream * dL/dmean (t_mean; upstream: device scalar, NULL = 1)
+ *   d_log_std  (with d_mean) t_std: [dims] summed over the rows when ld_std is 0, else [rows][dims] contiguous
+ *   log_probs [rows]: l (0 outside `valid`) or NULL
+ *   out [8] float32: L (unweighted), mean S, mean K, share of rows without gradient (clipped), n, 0, and n as a double in out[6..7]
+ *   count  device double: the n of an earlier call's out + 6 (gradient alone: the scalars are not computed, out is not written)
+ *   scratch  hoic_policy_loss_scratch_bytes(dims) bytes, aligned to 8 */
+typedef struct hoic_policy_loss_args {
+  int64_t rows;
+  int32_t dims, t_mean, t_act, t_std;
+  const void *mean, *act, *log_std, *ref_mean, *ref_log_std;
+  int64_t ld_mean, ld_act, ld_std, ld_ref_mean, ld_ref_std, ld_dmean;
+  const float *adv, *fixed;
+  const uint8_t* valid;
+  const float* upstream;
+  const double* count;
+  double clip_lo, clip_hi, kl_coef, weight;
+  void *d_mean, *d_log_std;
+  float *log_probs, *out;
+  void* scratch;
+} hoic_policy_loss_args;
+int64_t hoic_policy_loss_scratch_bytes(int32_t dims);
+int32_t hoic_policy_loss(const hoic_policy_loss_args* a, void* stream);
+/* The norm of a list of gradients (the learner clips the policy's at 40: agent_handmimic.py:67) in two steps: hoic_grad_norm_partial
+ * writes hoic_grad_norm_parts(n, nt) partial sums of squares of nt contiguous tensors of one type (once per type, behind one
+ * another); hoic_grad_norm_finish joins them in fixed order: d_clip[0] = norm, d_clip[1] = min(1, bound / (norm + 1e-6)) in
+ * 64 bits, d_norm[0] = norm.  hoic_scale_list: g *= d_clip[1] (a factor of 1 touches nothing).  The lists are HOST arrays. */
+int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt);
+int32_t hoic_grad_norm_partial(const void* const* g, const int64_t* n, int32_t nt, int32_t type, double* d_part, void* stream);
+int32_t hoic_grad_norm_finish(const double* d_part, int64_t nparts, double bound, double* d_clip, float* d_norm, void* stream);
+int32_t hoic_scale_list(void* const* g, const int64_t* n, int32_t nt, int32_t type, const double* d_clip, void* stream);
+/* hoic_adamw: one AdamW step over nt tensors of one type (in the place of the optimiser step of agent_ppo.py:46-56 / agent_pg.py:18-25;
+ * list in HOST memory).  m' = b1 m + (1 - b1) c g, v' = b2 v + (1 - b2) (c g)^2, p' = p - (lr wd p + lr / (1 - b1^t) m' / (sqrt(v' / (1 - b2^t))
+ * + eps)).  d_clip: {norm, factor c} or NULL (c = 1); a norm that is not finite leaves everything as it is.
+ *   state_bits 32: m, v float32 [n];  8: m, v bytes [n], m_scale, v_scale float32 [ceil(n / 256)]: blocks of 256 in storage order, a
+ *   power-of-two scale each; m sign + e4m3 (bias 7), v e5m3 (bias 15) without sign; rounded up with the probability of the part cut
+ *   off by a hash of (seed, t, ordinal, element); 0x7f / 0xff stand for values that are not finite
+ *   t = step (>= 1, this step's) -- or, with d_consts (4 nt floats of scratch), counted on the device: *d_step += 1 first; lr then
+ *   comes from d_lr (device float) when given.  Bytes of 8-bit states aligned to 4.
+ * hoic_adamw_values: the float32 values of 8-bit states: p receives m's, g v's (both float32 [n]). */
+typedef struct hoic_adamw_tensor {
+  void* p;
+  const void* g;
+  void *m, *v;
+  float *m_scale, *v_scale;
+  int64_t n, step;
+  int32_t* d_step;
+  int64_t ordinal;
+} hoic_adamw_tensor;
+typedef struct hoic_adamw_args {
+  int32_t type, state_bits;
+  double lr, b1, b2, eps, weight_decay;
+  const float* d_lr;
+  const double* d_clip;
+  float* d_consts;
+  uint32_t seed, reserved;
+} hoic_adamw_args;
+int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic_adamw_args* a, void* stream);
+int32_t hoic_adamw_values(const hoic_adamw_tensor* t, int32_t nt, void* stream);
+
 /* hoic_step is two launches: the substep kernel (15 fused substeps, the dominant kernel) and the post-step
  * kernel (contact averaging, residual-force QP, termination, reward, observation).  Durations in milliseconds of
  * the most recent launches, measured with HIP events on the launch stream (negative if timing was not enabled
