@@ -1940,13 +1940,38 @@ __device__ __forceinline__ float m_value(unsigned c) {
   return (c & 0x7f) == 0x7f ? __builtin_nanf("") : (c & 0x80) ? -x : x;
 }
 __device__ __forceinline__ float v_value(unsigned c) { return c == 0xff ? __builtin_nanf("") : __builtin_bit_cast(float, c << 20) * pow2f(112); }
-// y >= 0 in units of the scale -> code, rounded up with the probability of the part cut off: 20 mantissa bits are in the
-// high word, 3 stay, the 17 below them plus (2 r + 1) of 2^17 carry or do not (r: 16 random bits).  Below the smallest normal
-// 2^low one 2^low is added: the step there is the same as in the binade above, the code counts from 0.
-__device__ __forceinline__ unsigned code8(double y, int low, unsigned r16) {
-  const bool sub = y < pow2d(low);
-  const double z = sub ? y + pow2d(low) : y;
-  return ((hi32(z) + 2 * r16 + 1) >> 17) - (unsigned)(1023 + low - (sub ? 0 : 1)) * 8;
+// Where a value lies between two codes is a matter of its last bits now and then: with b1 = 0.9 one value in 10^7 or so is a decimal
+// fraction that lies exactly on the border between up and down.  So that it falls where the same formula lets it fall in 64-bit
+// tensor operations, the operations are theirs, unfused and in their order, down to 2^e: tensor operations take it from the math
+// library's pow, which gives the next smaller number for some e.  Those e (bit e + 126), and what that makes of
+//   a code's value (8 + man) 2^(e - 10 | e - 18): one unit in the last place down for these exponent fields (bit = field),
+//   a / k: one up,     y 2^(3 - ey): one down for these ey (bit ey + 14).
+__device__ const unsigned POW_DOWN[8] = {0x00a02000u, 0x08084010u, 0x40000424u, 0x04252800u, 0x28080200u, 0x02100420u, 0x04000908u, 0x090a0210u};
+#define M_DOWN 0x43u
+#define V_DOWN 0x20004253u
+#define Y_DOWN 0x24200040u
+__device__ __forceinline__ double nudge(double x, int units) { return __builtin_bit_cast(double, __builtin_bit_cast(long long, x) + units); }
+__device__ __forceinline__ bool pow_down(int e) { return (POW_DOWN[(e + 126) >> 5] >> ((e + 126) & 31)) & 1; }
+// a product that is rounded by itself (this unit is compiled with contraction everywhere)
+__device__ __forceinline__ double rounded(double x) { asm("" : "+v"(x)); return x; }
+__device__ __forceinline__ double m_old(unsigned c, double k) {
+  const double x = (double)m_value(c) * k;
+  return (c & 0x7f) && (M_DOWN >> ((c & 0x7f) >> 3)) & 1 ? nudge(x, -1) : x;
+}
+__device__ __forceinline__ double v_old(unsigned c, double k) {
+  const double x = (double)v_value(c) * k;
+  return c && (V_DOWN >> (c >> 3)) & 1 ? nudge(x, -1) : x;
+}
+// a >= 0 -> code: y = a / k in eighths of its binade 2^ey (of 2^low below the smallest normal one), the part below one of them up
+// with its probability (r16: 16 random bits); r = 1 / k, up: 1 where pow's 2^e is small
+__device__ __forceinline__ unsigned code8(double a, double r, int up, int low, unsigned r16) {
+  double y = a * r;
+  y = a > 0. ? nudge(y, up) : 0.;
+  const int ey = min(max((int)(hi32(y) >> 20) - 1023, low), 16);        // (16: what is not finite; its code is set afterwards)
+  const double u = fma((double)r16, 1. / 65536., 0.5 / 65536.);
+  double q = y * pow2d(3 - ey);
+  q = y > 0. && (Y_DOWN >> (ey + 14)) & 1 ? nudge(q, -1) : q;
+  return (unsigned)(q + u) + (unsigned)(ey - low) * 8u;
 }
 #define ADAM8_CHUNK 4096
 template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(AdamArgs a) {
@@ -1973,8 +1998,8 @@ template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(Ada
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const double x = (double)gg[e] * cl;
-      mm[e] = fma(a.b1d, (double)m_value((cm >> (8 * e)) & 0xff) * km, a.c1d * x);
-      vv[e] = fma(a.b2d, (double)v_value((cv >> (8 * e)) & 0xff) * kv, a.c2d * x * x);
+      mm[e] = rounded(a.b1d * m_old((cm >> (8 * e)) & 0xff, km)) + rounded(a.c1d * x);
+      vv[e] = rounded(a.b2d * v_old((cv >> (8 * e)) & 0xff, kv)) + rounded(a.c2d * x * x);
       if (vv[e] > 3.4028234663852886e38 && vv[e] < INFINITY) vv[e] = 3.4028234663852886e38;
       const unsigned am = hi32(mm[e]) & 0x7fffffffu, av = hi32(vv[e]);
       if (am < 0x7ff00000u && am > hm) hm = am;
@@ -1985,12 +2010,13 @@ template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(Ada
     for (int q = 32; q; q >>= 1) { hm = max(hm, (unsigned)__shfl_xor((int)hm, q, 64)); hv = max(hv, (unsigned)__shfl_xor((int)hv, q, 64)); }
     const int em = max((int)(hm >> 20) - 1023 - 7, -126), ev = max((int)(hv >> 20) - 1023 - 15, -126);
     const double rm = pow2d(-em), rv = pow2d(-ev);
+    const int um = pow_down(em), uv = pow_down(ev);
     unsigned om = 0, ov = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const unsigned h = mix32((unsigned)(i + e) + key);
-      unsigned qm = code8(fabs(mm[e]) * rm, -6, h & 0xffff) | (mm[e] < 0. ? 0x80u : 0u);
-      unsigned qv = code8(vv[e] * rv, -14, h >> 16);
+      unsigned qm = code8(fabs(mm[e]), rm, um, -6, h & 0xffff) | (mm[e] < 0. ? 0x80u : 0u);
+      unsigned qv = code8(vv[e], rv, uv, -14, h >> 16);
       qv = qv == 0 && vv[e] > 0. ? 1u : qv;
       qm = (hi32(mm[e]) & 0x7ff00000u) == 0x7ff00000u ? 0x7fu : qm;
       qv = (hi32(vv[e]) & 0x7ff00000u) == 0x7ff00000u ? 0xffu : qv;

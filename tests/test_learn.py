@@ -574,6 +574,56 @@ def test_adamw8_matches_float64(sizes, dtype, clip):
             p.grad = (p.grad.float() * 0.7 + 1e-3).to(dtype)
 
 
+def tensor_form8(x, signed, bits):
+    """store8 and its values as float64 tensor operations on the GPU (blocks of 256 throughout)"""
+    top, low = (7, -6) if signed else (15, -14)
+    b = x.abs().view(-1, 256)
+    e = torch.clamp(torch.frexp(b.max(1).values)[1] - 1 - top, min=-126)
+    k = torch.ldexp(torch.ones((), dtype=torch.float64, device=x.device), e)
+    y = (b / k[:, None]).view(-1)
+    ey = torch.clamp(torch.where(y > 0, torch.frexp(y)[1] - 1, low), min=low)
+    code = torch.floor(torch.ldexp(y, 3 - ey) + (bits.double() + 0.5) / 65536.0).long() + (ey.long() - low) * 8
+    code = code + 128 * (x < 0).long() if signed else torch.where(x > 0, torch.clamp(code, min=1), code)
+    return code.to(torch.uint8), k.float()
+
+
+def tensor_form8_values(code, k, signed):
+    low = -6 if signed else -14
+    c = torch.arange(256, device=code.device)
+    e, man = (c & 127 if signed else c) >> 3, c & 7
+    v = torch.where(e == 0, torch.ldexp(man.double(), torch.full_like(e, low - 3)), torch.ldexp(man.double() + 8.0, e - 1 + low - 3))
+    v = torch.where(c >= 128, -v, v) if signed else v
+    return v[code.long()] * k.double().repeat_interleave(256)
+
+
+@gpu
+@pytest.mark.parametrize("seed", [0, 1])
+def test_adamw8_borders_fall_as_in_tensor_operations(seed):
+    """Decimal fractions that lie exactly between up and down come up once in 10^7 values at b1 = 0.9: 2^26 elements, gradients with few
+    bits so that they come up often, a first step and one on states of every code: the same codes as the float64 tensor form"""
+    n = 1 << 26
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    g = torch.randint(1, 4096, (n,), device="cuda", generator=gen).float() * (2.0 ** torch.randint(-20, -10, (n,), device="cuda", generator=gen))
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda")); p.grad = g
+    opt = optim.AdamW([p], lr=0.0, state_bits=8, seed=seed)
+    i = torch.arange(n, device="cuda")
+    def mix(x):
+        x = x ^ (x >> 17); x = (x * 0x743B8C43) & 0xFFFFFFFF
+        x = x ^ (x >> 12); x = (x * 0xAB2209AB) & 0xFFFFFFFF
+        return x ^ (x >> 15)
+    m = v = torch.zeros(n, dtype=torch.float64, device="cuda")
+    for t in (1, 2):
+        opt.step()
+        m = 0.9 * m + (1.0 - 0.9) * g.double(); v = 0.999 * v + (1.0 - 0.999) * g.double() * g.double()
+        h = mix((i + mix(mix(mix(mix(seed) + t & 0xFFFFFFFF) + 0) + 0 & 0xFFFFFFFF)) & 0xFFFFFFFF)
+        s = opt.state[p]
+        for key, x, signed, r in (("exp_avg", m, True, h & 0xFFFF), ("exp_avg_sq", v, False, h >> 16)):
+            code, k = tensor_form8(x, signed, r)
+            assert int((code != s[key]).sum()) == 0 and torch.equal(k, s[key + "_scale"]), (key, t)
+        m, v = tensor_form8_values(s["exp_avg"], s["exp_avg_scale"], True), tensor_form8_values(s["exp_avg_sq"], s["exp_avg_sq_scale"], False)
+        p.grad = g = -g.flip(0)
+
+
 @gpu
 def test_adamw8_extreme_values():
     """zero blocks, single large and tiny values, non-finite gradients (their own element only), squares past float32's range"""
