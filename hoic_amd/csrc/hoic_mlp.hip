@@ -1731,8 +1731,28 @@ template <class E, int MAXT> __device__ __forceinline__ int list_find(const E (&
   return lo;
 }
 
-// sqrt(sum g^2) over a list: 64-bit partial sums per workgroup, joined in fixed order by one workgroup; the factor
-// min(1, bound / (norm + 1e-6)) beside it.
+// sqrt(sum g^2) over a list: 64-bit partial sums per workgroup, then joined in fixed order, with the factor
+// min(1, bound / (norm + 1e-6)) beside it -- by a workgroup of its own, or, in lists of few parts, by every workgroup of the launch
+// that uses the factor (Joint): that saves the launch between.
+struct Joint { const double* parts; int nparts; double bound; float* norm; };      // parts NULL: no clipping; nparts 0: parts = {norm, factor}
+__device__ __forceinline__ double2 norm_factor(double sum, double bound) {
+  const double t = sqrt(sum), c = bound / (t + 1e-6);
+  return make_double2(t, c > 1. ? 1. : c);       // (a NaN norm leaves a NaN factor)
+}
+// all of a 256-lane workgroup: {norm, factor}
+__device__ __forceinline__ double2 join_norm(const Joint& j) {
+  if (j.nparts == 0) return make_double2(j.parts[0], j.parts[1]);
+  __shared__ double red[4];
+  double s = 0.;
+  for (int i = threadIdx.x; i < j.nparts; i += 256) s += j.parts[i];
+#pragma unroll
+  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  const double2 r = norm_factor((red[0] + red[1]) + (red[2] + red[3]), j.bound);
+  if (j.norm && blockIdx.x == 0 && threadIdx.x == 0) *j.norm = (float)r.x;
+  return r;
+}
 struct NormEntry { const void* g; long long n; int first; };
 #define NORM_MAX 120
 struct NormArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; double* part; };
@@ -1757,26 +1777,13 @@ __global__ __launch_bounds__(256) void hoic_sumsq_kernel(NormArgs a) {
   __syncthreads();
   if (threadIdx.x == 0) a.part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
-__global__ __launch_bounds__(1024) void hoic_norm_finish_kernel(const double* __restrict__ part, long long nparts, double bound, double* __restrict__ clip, float* __restrict__ norm) {
-  __shared__ double red[16];
-  double s = 0.;
-  for (long long i = threadIdx.x; i < nparts; i += 1024) s += part[i];
-#pragma unroll
-  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double t = 0.;
-    for (int w = 0; w < 16; w++) t += red[w];
-    t = sqrt(t);
-    const double c = bound / (t + 1e-6);
-    clip[0] = t;
-    clip[1] = c > 1. ? 1. : c;       // (a NaN norm leaves a NaN factor)
-    *norm = (float)t;
-  }
+// parts -> clip = {norm, factor}, norm in float32
+__global__ __launch_bounds__(256) void hoic_norm_finish_kernel(Joint j, double* __restrict__ clip) {
+  const double2 r = join_norm(j);
+  if (threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
 }
 // g *= factor where it is not 1
-struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; const double* clip; };
+struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; Joint clip; };
 template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, float c) {
   for (long long i = i0 + threadIdx.x * 4; i < i1; i += 1024) {
     const int l = i1 - i < 4 ? (int)(i1 - i) : 4;
@@ -1787,7 +1794,7 @@ template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0
   }
 }
 __global__ __launch_bounds__(256) void hoic_scale_kernel(ScaleArgs a) {
-  const double c = a.clip[1];
+  const double c = join_norm(a.clip).y;
   if (c == 1.) return;
   const int t = list_find(a.t, a.nt, blockIdx.x);
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * a.chunk, i1 = i0 + a.chunk < a.t[t].n ? i0 + a.chunk : a.t[t].n;
@@ -1802,60 +1809,80 @@ static long long norm_chunk(const int64_t* n, int32_t nt) {
   const long long c = (tot + 2047) / 2048;
   return std::max<long long>(8192, (c + 1023) / 1024 * 1024);
 }
-static long long norm_parts(const int64_t* n, int32_t nt, long long chunk) {
-  long long p = 0;
-  for (int i = 0; i < nt; i++) p += (n[i] + chunk - 1) / chunk;
-  return p;
-}
-static int32_t norm_check(const char* who, const void* const* g, const int64_t* n, int32_t nt, int32_t type) {
-  if (nt < 0 || (nt > 0 && (!g || !n)) || (type != HOIC_F32 && type != HOIC_F16 && type != HOIC_BF16)) { hoic_set_error(std::string(who) + ": bad list or type"); return HOIC_ERR_ARG; }
-  for (int i = 0; i < nt; i++) if (n[i] < 0 || (n[i] > 0 && !g[i])) { hoic_set_error(std::string(who) + ": a tensor without memory or with a negative size"); return HOIC_ERR_ARG; }
+#define JOIN_PARTS 2048          // up to so many parts are joined by the workgroups that use them
+static int32_t norm_check(const char* who, const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt) {
+  if (nt < 0 || (nt > 0 && (!g || !n || !type))) { hoic_set_error(std::string(who) + ": bad list"); return HOIC_ERR_ARG; }
+  for (int i = 0; i < nt; i++)
+    if (n[i] < 0 || (n[i] > 0 && !g[i]) || type[i] > HOIC_BF16) { hoic_set_error(std::string(who) + ": a tensor without memory, with a negative size or of another type"); return HOIC_ERR_ARG; }
   return HOIC_OK;
 }
 extern "C" int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt) {
   if (nt < 0 || (nt > 0 && !n)) return -1;
-  return norm_parts(n, nt, norm_chunk(n, nt));
+  const long long chunk = norm_chunk(n, nt);
+  long long p = 0;
+  for (int i = 0; i < nt; i++) p += (n[i] + chunk - 1) / chunk;
+  return p;
 }
-extern "C" int32_t hoic_grad_norm_partial(const void* const* g, const int64_t* n, int32_t nt, int32_t type, double* d_part, void* stream) {
-  const int32_t rc = norm_check("hoic_grad_norm_partial", g, n, nt, type);
-  if (rc != HOIC_OK) return rc;
-  if (!d_part) { hoic_set_error("hoic_grad_norm_partial: no place for the partial sums"); return HOIC_ERR_ARG; }
+// launches over a list, type by type: f(entries so far, blocks) for every NORM_MAX of them
+template <class A, class F> static void norm_launches(A& a, const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, F launch) {
+  a.chunk = norm_chunk(n, nt);
+  for (int ty = HOIC_F32; ty <= HOIC_BF16; ty++) {
+    a.type = ty; a.nt = 0;
+    long long blocks = 0;
+    for (int i = 0; i < nt; i++) {
+      if (type[i] == ty && n[i] > 0) {
+        a.t[a.nt].g = g[i]; a.t[a.nt].n = n[i]; a.t[a.nt].first = (int)blocks; a.nt++;
+        blocks += (n[i] + a.chunk - 1) / a.chunk;
+      }
+      if (blocks && (a.nt == NORM_MAX || i == nt - 1)) { launch(blocks); a.nt = 0; blocks = 0; }
+    }
+  }
+}
+static void norm_partial(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* part, hipStream_t st) {
   NormArgs a;
-  a.type = type; a.chunk = norm_chunk(n, nt); a.part = d_part;
-  for (int i = 0; i < nt;) {
-    long long blocks = 0;
-    for (a.nt = 0; i < nt && a.nt < NORM_MAX; i++) {
-      if (n[i] == 0) continue;
-      a.t[a.nt].g = g[i]; a.t[a.nt].n = n[i]; a.t[a.nt].first = (int)blocks; a.nt++;
-      blocks += (n[i] + a.chunk - 1) / a.chunk;
-    }
-    if (blocks) hipLaunchKernelGGL(hoic_sumsq_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+  a.part = part;
+  norm_launches(a, g, n, type, nt, [&](long long blocks) {
+    hipLaunchKernelGGL(hoic_sumsq_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
     a.part += blocks;
-  }
-  MCHK(hipGetLastError());
-  return HOIC_OK;
+  });
 }
-extern "C" int32_t hoic_grad_norm_finish(const double* d_part, int64_t nparts, double bound, double* d_clip, float* d_norm, void* stream) {
-  if (nparts < 0 || (nparts > 0 && !d_part) || !d_clip || !d_norm || !(bound >= 0.)) { hoic_set_error("hoic_grad_norm_finish: bad arguments"); return HOIC_ERR_ARG; }
-  hipLaunchKernelGGL(hoic_norm_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, d_part, (long long)nparts, bound, d_clip, d_norm);
-  MCHK(hipGetLastError());
-  return HOIC_OK;
+// d_buf = {norm, factor, parts ...}; what a launch that uses the factor is given: the parts, or {norm, factor} after a join
+static Joint norm_join(double* d_buf, long long nparts, double bound, float* d_norm, bool now, hipStream_t st) {
+  Joint j = {d_buf + 2, (int)nparts, bound, d_norm};
+  if (nparts <= JOIN_PARTS && !now) return j;
+  hipLaunchKernelGGL(hoic_norm_finish_kernel, dim3(1), dim3(256), 0, st, j, d_buf);
+  return Joint{d_buf, 0, bound, nullptr};
 }
-extern "C" int32_t hoic_scale_list(void* const* g, const int64_t* n, int32_t nt, int32_t type, const double* d_clip, void* stream) {
-  const int32_t rc = norm_check("hoic_scale_list", (const void* const*)g, n, nt, type);
+extern "C" int32_t hoic_grad_norm(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* d_buf, float* d_norm, void* stream) {
+  const int32_t rc = norm_check("hoic_grad_norm", g, n, type, nt);
   if (rc != HOIC_OK) return rc;
-  if (!d_clip) { hoic_set_error("hoic_scale_list: no factor"); return HOIC_ERR_ARG; }
+  const long long np = hoic_grad_norm_parts(n, nt);
+  if (!d_buf || !d_norm || np == 0 || np > 0x7fffffff) { hoic_set_error("hoic_grad_norm: an empty list, or no place for the sums"); return HOIC_ERR_ARG; }
+  norm_partial(g, n, type, nt, d_buf + 2, (hipStream_t)stream);
+  norm_join(d_buf, np, INFINITY, d_norm, true, (hipStream_t)stream);
+  MCHK(hipGetLastError());
+  return HOIC_OK;
+}
+extern "C" int32_t hoic_grad_norm_partial(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* d_buf, void* stream) {
+  const int32_t rc = norm_check("hoic_grad_norm_partial", g, n, type, nt);
+  if (rc != HOIC_OK) return rc;
+  if (!d_buf) { hoic_set_error("hoic_grad_norm_partial: no place for the sums"); return HOIC_ERR_ARG; }
+  norm_partial(g, n, type, nt, d_buf + 2, (hipStream_t)stream);
+  MCHK(hipGetLastError());
+  return HOIC_OK;
+}
+extern "C" int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double bound, double* d_buf, float* d_norm, void* stream) {
+  const int32_t rc = norm_check("hoic_clip_grads", (const void* const*)g, n, type, nt);
+  if (rc != HOIC_OK) return rc;
+  const long long np = hoic_grad_norm_parts(n, nt);
+  if (!d_buf || !d_norm || np == 0 || np > 0x7fffffff || !(bound >= 0.)) { hoic_set_error("hoic_clip_grads: an empty list, no place for the sums, or a bound below 0"); return HOIC_ERR_ARG; }
+  hipStream_t st = (hipStream_t)stream;
+  norm_partial((const void* const*)g, n, type, nt, d_buf + 2, st);
   ScaleArgs a;
-  a.type = type; a.chunk = norm_chunk(n, nt); a.clip = d_clip;
-  for (int i = 0; i < nt;) {
-    long long blocks = 0;
-    for (a.nt = 0; i < nt && a.nt < NORM_MAX; i++) {
-      if (n[i] == 0) continue;
-      a.t[a.nt].g = g[i]; a.t[a.nt].n = n[i]; a.t[a.nt].first = (int)blocks; a.nt++;
-      blocks += (n[i] + a.chunk - 1) / a.chunk;
-    }
-    if (blocks) hipLaunchKernelGGL(hoic_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
-  }
+  a.clip = norm_join(d_buf, np, bound, d_norm, false, st);
+  norm_launches(a, (const void* const*)g, n, type, nt, [&](long long blocks) {
+    hipLaunchKernelGGL(hoic_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  });
   MCHK(hipGetLastError());
   return HOIC_OK;
 }
@@ -1881,7 +1908,7 @@ struct AdamArgs {
   int nt, at;                    // entries of this launch; place of the first one in the call's list
   float b1, c1, b2, c2, eps, lrwd;
   double b1d, c1d, b2d, c2d;
-  const double* clip;            // {norm, factor} or NULL
+  Joint clip;
   const float* consts;           // {step size, 1 / sqrt(1 - b2^t), key, lr * wd} per entry of the call (step on the device), or NULL
 };
 __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
@@ -1906,10 +1933,15 @@ __device__ __forceinline__ float adam_param(float p, float m, float v, const Ada
   return p - fmaf(c.lrwd, p, u);
 }
 #define ADAM32_CHUNK 4096
+#define JOIN_BLOCKS 4096         // a launch of more workgroups is given the joined factor
 template <class T> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   float cl = 1.f;
-  if (a.clip) { if (!(a.clip[0] < INFINITY)) return; cl = (float)a.clip[1]; }
+  if (a.clip.parts) {
+    const double2 f = join_norm(a.clip);
+    if (!(f.x < INFINITY)) return;
+    cl = (float)f.y;
+  }
   const AdamConsts c = adam_consts(a, t);
   T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; float* m = (float*)a.t[t].m; float* v = (float*)a.t[t].v;
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM32_CHUNK, left = a.t[t].n - i0;
@@ -1977,7 +2009,11 @@ __device__ __forceinline__ unsigned code8(double a, double r, int up, int low, u
 template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   double cl = 1.;
-  if (a.clip) { if (!(a.clip[0] < INFINITY)) return; cl = a.clip[1]; }
+  if (a.clip.parts) {
+    const double2 f = join_norm(a.clip);
+    if (!(f.x < INFINITY)) return;
+    cl = f.y;
+  }
   const AdamConsts c = adam_consts(a, t);
   T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; unsigned char* m = (unsigned char*)a.t[t].m; unsigned char* v = (unsigned char*)a.t[t].v;
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM8_CHUNK, left = a.t[t].n - i0;
@@ -2065,8 +2101,9 @@ __global__ __launch_bounds__(64) void hoic_adamw_count_kernel(AdamCount a) {
 }
 extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic_adamw_args* x, void* stream) {
   if (nt < 0 || (nt > 0 && !t) || !x || (x->type != HOIC_F32 && x->type != HOIC_F16 && x->type != HOIC_BF16) || (x->state_bits != 32 && x->state_bits != 8)
+      || (x->d_norm_buf && (x->norm_parts <= 0 || x->norm_parts > 0x7fffffff || !x->d_norm || !(x->bound >= 0.)))
       || !(x->b1 >= 0. && x->b1 < 1.) || !(x->b2 >= 0. && x->b2 < 1.) || !(x->eps >= 0.)) {
-    hoic_set_error("hoic_adamw: bad list, type, state_bits (8 or 32), betas or eps"); return HOIC_ERR_ARG;
+    hoic_set_error("hoic_adamw: bad list, type, state_bits (8 or 32), betas, eps or norm"); return HOIC_ERR_ARG;
   }
   for (int i = 0; i < nt; i++) {
     const hoic_adamw_tensor& e = t[i];
@@ -2079,8 +2116,12 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
   hipStream_t st = (hipStream_t)stream;
   AdamArgs a;
   a.b1 = (float)x->b1; a.c1 = (float)(1. - x->b1); a.b2 = (float)x->b2; a.c2 = (float)(1. - x->b2); a.eps = (float)x->eps; a.lrwd = (float)(x->lr * x->weight_decay);
-  a.b1d = x->b1; a.c1d = 1. - x->b1; a.b2d = x->b2; a.c2d = 1. - x->b2; a.clip = x->d_clip; a.consts = x->d_consts;
+  a.b1d = x->b1; a.c1d = 1. - x->b1; a.b2d = x->b2; a.c2d = 1. - x->b2; a.consts = x->d_consts;
   a.at = 0;
+  long long total = 0;
+  for (int i = 0; i < nt; i++) total += (t[i].n + ADAM32_CHUNK - 1) / ADAM32_CHUNK;
+  a.clip = Joint{nullptr, 0, 0., nullptr};
+  if (x->d_norm_buf) a.clip = norm_join(x->d_norm_buf, x->norm_parts, x->bound, x->d_norm, total > JOIN_BLOCKS, st);
   for (int i = 0; i < nt;) {
     long long blocks = 0;
     AdamCount cnt;
@@ -2114,6 +2155,7 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
       else hipLaunchKernelGGL(hoic_adamw8_kernel<__bf16>, grid, block, 0, st, a);
     }
     a.at += a.nt;
+    a.clip.norm = nullptr;       // (written by the first launch)
   }
   MCHK(hipGetLastError());
   return HOIC_OK;

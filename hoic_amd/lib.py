@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import subprocess
 
 import numpy as np
@@ -38,20 +39,9 @@ class RewardParams(C.Structure):
     _fields_ = [("wk", C.c_float * 16), ("end_reward", C.c_float), ("use_end_reward", C.c_int32)]
 
 
-class PolicyLossArgs(C.Structure):
-    """hoic_policy_loss_args (include/hoic.h)"""
-    _fields_ = ([("rows", C.c_int64)] + [(n, C.c_int32) for n in ("dims", "t_mean", "t_act", "t_std")]
-                + [(n, C.c_void_p) for n in ("mean", "act", "log_std", "ref_mean", "ref_log_std")]
-                + [(n, C.c_int64) for n in ("ld_mean", "ld_act", "ld_std", "ld_ref_mean", "ld_ref_std", "ld_dmean")]
-                + [(n, C.c_void_p) for n in ("adv", "fixed", "valid", "upstream", "count")]
-                + [(n, C.c_double) for n in ("clip_lo", "clip_hi", "kl_coef", "weight")]
-                + [(n, C.c_void_p) for n in ("d_mean", "d_log_std", "log_probs", "out", "scratch")])
-
-
-class AdamWArgs(C.Structure):
-    """hoic_adamw_args (include/hoic.h)"""
-    _fields_ = ([("type", C.c_int32), ("state_bits", C.c_int32)] + [(n, C.c_double) for n in ("lr", "b1", "b2", "eps", "weight_decay")]
-                + [(n, C.c_void_p) for n in ("d_lr", "d_clip", "d_consts")] + [("seed", C.c_uint32), ("reserved", C.c_uint32)])
+# hoic_policy_loss_args and hoic_adamw_args (include/hoic.h) as struct formats: one pack() is the whole argument block
+POLICY_LOSS_ARGS = struct.Struct("@q4i5P6q5P4d5P")
+ADAMW_ARGS = struct.Struct("@2i5d4Pdq2I")
 
 
 EXPORTS = ["hoic_create", "hoic_destroy", "hoic_num_envs", "hoic_obs_dim", "hoic_action_dim", "hoic_last_error", "hoic_build_id",
@@ -62,8 +52,8 @@ EXPORTS = ["hoic_create", "hoic_destroy", "hoic_num_envs", "hoic_obs_dim", "hoic
            "hoic_mlp_gemm", "hoic_mlp_slab_reduce", "hoic_mlp_rowsum_packed", "hoic_mlp_set_pipeline", "hoic_mlp_gemm_tn",
            "hoic_mlp_colsum_packed", "hoic_mlp_amax_colsum", "hoic_mlp_colpart_finish", "hoic_mlp_update_exps_rel", "hoic_mlp_pack_tiled", "hoic_mlp_forward_tiled",
            "hoic_set_async_reward", "hoic_sync_rewards", "hoic_set_cu_reserve", "hoic_mlp_head", "hoic_mlp_head_backward", "hoic_mlp_ppo_loss",
-           "hoic_mlp_value_loss", "hoic_policy_loss", "hoic_policy_loss_scratch_bytes", "hoic_grad_norm_parts", "hoic_grad_norm_partial",
-           "hoic_grad_norm_finish", "hoic_scale_list", "hoic_adamw", "hoic_adamw_values"]
+           "hoic_mlp_value_loss", "hoic_policy_loss", "hoic_policy_loss_scratch_bytes", "hoic_grad_norm_parts", "hoic_grad_norm",
+           "hoic_grad_norm_partial", "hoic_clip_grads", "hoic_adamw", "hoic_adamw_values"]
 
 
 def build(force: bool = False) -> str:
@@ -134,15 +124,15 @@ def load():
     if hasattr(L, "hoic_zfilter_absorb"):
         L.hoic_zfilter_absorb.argtypes = [i32, vp, C.POINTER(vp), i32, vp, vp]
     if hasattr(L, "hoic_policy_loss"):
-        L.hoic_policy_loss.argtypes = [C.POINTER(PolicyLossArgs), vp]
+        L.hoic_policy_loss.argtypes = [vp, vp]
         L.hoic_policy_loss_scratch_bytes.argtypes = [i32]
         L.hoic_policy_loss_scratch_bytes.restype = C.c_int64
         L.hoic_grad_norm_parts.argtypes = [vp, i32]
         L.hoic_grad_norm_parts.restype = C.c_int64
-        L.hoic_grad_norm_partial.argtypes = [vp, vp, i32, i32, vp, vp]
-        L.hoic_grad_norm_finish.argtypes = [vp, C.c_int64, C.c_double, vp, vp, vp]
-        L.hoic_scale_list.argtypes = [vp, vp, i32, i32, vp, vp]
-        L.hoic_adamw.argtypes = [vp, i32, C.POINTER(AdamWArgs), vp]       # the list: n x 10 int64 (hoic_adamw_tensor is 80 bytes of 8-byte fields)
+        L.hoic_grad_norm.argtypes = [vp, vp, vp, i32, vp, vp, vp]
+        L.hoic_grad_norm_partial.argtypes = [vp, vp, vp, i32, vp, vp]
+        L.hoic_clip_grads.argtypes = [vp, vp, vp, i32, C.c_double, vp, vp, vp]
+        L.hoic_adamw.argtypes = [vp, i32, vp, vp]       # the list: n x 10 int64 (hoic_adamw_tensor is 80 bytes of 8-byte fields)
         L.hoic_adamw_values.argtypes = [vp, i32, vp]
     for n in EXPORTS:
         if os.environ.get("HOIC_LIB") and not hasattr(L, n):

@@ -10,20 +10,13 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+import torch.optim.optimizer as _opt
 
 from . import lib
 
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}         # enum hoic_type
 BLOCK = 256                                                             # elements per block of an 8-bit state
 _EMPTY_SCALE = 2.0 ** -126                                              # the scale of a block whose values are all zero
-
-
-def _ptr(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
-
-
-def _stream(dev):
-    return C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _strides(t):
@@ -43,7 +36,7 @@ def _dense(t):
 
 
 def _check(t, what):
-    if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
+    if not isinstance(t, torch.Tensor) or t.layout is not torch.strided:
         raise ValueError(f"{what}: a dense tensor is needed")
     if not t.is_cuda:
         raise lib.HoicError(f"{what}: the kernels run on the GPU only, this tensor is on {t.device}")
@@ -51,30 +44,36 @@ def _check(t, what):
         raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
 
 
-def _norm(grads, bound):
-    """(norm: float32 scalar, float64 [2] = {norm, min(1, bound / (norm + 1e-6))}) of dense CUDA tensors of one device"""
-    dev = grads[0].device
-    by_type = {}
+class _Launch:
+    """``with _Launch(device) as stream``: the device current (switched only when another one is), its current stream's handle.  Every
+    entry point launches on the stream that it is given and carries no device ordinal."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, dev):
+        self.index = dev.index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.before)
+
+
+def _norm_list(grads):
+    """The arguments of the hoic_grad_norm family for CUDA tensors of one device: ((pointers, sizes, types, count), parts, tensors held)"""
+    dev, n = grads[0].device, len(grads)
     for g in grads:
         if g.device != dev:
             raise ValueError(f"one norm over gradients on several devices ({dev}, {g.device})")
-        if g.numel():
-            by_type.setdefault(g.dtype, []).append(g if _dense(g) else g.contiguous())
-    L = lib.load()
-    lists, parts = [], 0
-    for dt, gs in by_type.items():
-        sizes = (C.c_int64 * len(gs))(*[g.numel() for g in gs])
-        lists.append((dt, gs, (C.c_void_p * len(gs))(*[g.data_ptr() for g in gs]), sizes, parts))
-        parts += L.hoic_grad_norm_parts(sizes, len(gs))
-    buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    base = buf.data_ptr() + 16
-    with torch.cuda.device(dev):
-        st = _stream(dev)
-        for dt, gs, ptrs, sizes, at in lists:
-            lib._chk(L.hoic_grad_norm_partial(ptrs, sizes, len(gs), TYPES[dt], C.c_void_p(base + 8 * at), st), "hoic_grad_norm_partial")
-        lib._chk(L.hoic_grad_norm_finish(C.c_void_p(base), parts, float(bound), _ptr(buf), _ptr(norm), st), "hoic_grad_norm_finish")
-    return norm, buf, lists
+    grads = [g if _dense(g) else g.contiguous() for g in grads]
+    sizes = (C.c_int64 * n)(*[g.numel() for g in grads])
+    args = ((C.c_void_p * n)(*[g.data_ptr() for g in grads]), sizes, bytes([TYPES[g.dtype] for g in grads]), n)
+    return args, lib.load().hoic_grad_norm_parts(sizes, n), grads
 
 
 def _bound(max_norm):
@@ -93,7 +92,15 @@ def grad_norm(tensors):
     if not tensors:
         return torch.zeros(())
     with torch.no_grad():
-        return _norm(tensors, float("inf"))[0]
+        args, parts, held = _norm_list(tensors)
+        dev = held[0].device
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        if parts == 0:
+            return norm.zero_()
+        buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
+        with _Launch(dev) as st:
+            lib._chk(lib.load().hoic_grad_norm(*args, buf.data_ptr(), norm.data_ptr(), st), "hoic_grad_norm")
+    return norm
 
 
 def clip_grad_norm_(parameters, max_norm):
@@ -101,7 +108,7 @@ def clip_grad_norm_(parameters, max_norm):
     place, the norm before clipping returned as a float32 scalar on the device.  A factor of 1 reads and writes nothing; a norm
     that is not finite gives the factor that the formula gives (0 or NaN)."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
     b = _bound(max_norm)
     for g in grads:
         _check(g, "clip_grad_norm_")
@@ -109,14 +116,15 @@ def clip_grad_norm_(parameters, max_norm):
             raise ValueError("clip_grad_norm_: a gradient whose elements do not fill their memory cannot be scaled in place")
     if not grads:
         return torch.zeros(())
-    with torch.no_grad():
-        norm, clip, lists = _norm(grads, b)
-        L, dev = lib.load(), grads[0].device
-        with torch.cuda.device(dev):
-            for dt, gs, ptrs, sizes, _ in lists:
-                lib._chk(L.hoic_scale_list(ptrs, sizes, len(gs), TYPES[dt], _ptr(clip), _stream(dev)), "hoic_scale_list")
-        for g in grads:
-            torch.autograd.graph.increment_version(g)
+    args, parts, _ = _norm_list(grads)
+    dev = grads[0].device
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    if parts == 0:
+        return norm.zero_()
+    buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
+    with _Launch(dev) as st:
+        lib._chk(lib.load().hoic_clip_grads(*args, b, buf.data_ptr(), norm.data_ptr(), st), "hoic_clip_grads")
+    torch.autograd.graph.increment_version(grads)
     return norm
 
 
@@ -205,106 +213,115 @@ class AdamW(torch.optim.Optimizer):
             g.update(fixed)
         self.state.update(states)
 
-    @torch.no_grad()
     def step(self, closure=None, *, max_norm=None):
+        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _opt._global_optimizer_pre_hooks
+                or _opt._global_optimizer_post_hooks or torch.autograd.profiler._is_profiler_enabled):
+            return self._step_hooked(closure, max_norm=max_norm)
+        return self._step(closure, max_norm=max_norm)
+
+    step.hooked = True          # (hooks and profiler ranges are taken care of above; the base class would add 6 us to every step)
+
+    def _step(self, closure=None, *, max_norm=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        capturable = self.defaults["capturable"]
         bound = None if max_norm is None else _bound(max_norm)
-        ordinal, work, capturing = -1, {}, None
+        bits, capturable = self.defaults["state_bits"], self.defaults["capturable"]
+        # rows of the list (hoic_adamw_tensor) per device, group and type
+        ordinal, work, grads, params, fresh = -1, {}, [], [], []
         for gi, group in enumerate(self.param_groups):
             for p in group["params"]:
                 ordinal += 1
                 g = p.grad
                 if g is None:
                     continue
-                if g.dtype != p.dtype or g.layout != torch.strided:
-                    raise ValueError(f"AdamW: a {g.dtype} gradient (dense ones only) of a {p.dtype} parameter")
-                if not ((p.is_contiguous() and g.is_contiguous()) or _strides(g) == _strides(p)):
-                    g = torch.empty_like(p).copy_(g)                   # the parameter's order of elements
-                work.setdefault((p.device, gi, p.dtype), []).append((ordinal, p, g))
-        self.grad_norm = None
-        clip = None
-        if work:
-            for dev in {k[0] for k in work}:
-                with torch.cuda.device(dev):
-                    capturing = torch.cuda.is_current_stream_capturing()
-                if capturing and not capturable:
-                    raise lib.HoicError("AdamW: a captured step needs capturable=True (its step count would stand still)")
-                if capturing and any(not self.state[p] for k in work if k[0] == dev for _, p, _ in work[k]):
-                    raise lib.HoicError("AdamW: take one eager step before a capture (the states would be made anew at every replay)")
-        if bound is not None:
-            if work:
-                self.grad_norm, clip, _ = _norm([g for todo in work.values() for _, _, g in todo], bound)
-            else:
-                self.grad_norm = torch.zeros(())
-        L = lib.load()
-        bits = self.defaults["state_bits"]
-        for (dev, gi, dtype), todo in work.items():
-            group = self.param_groups[gi]
-            flat = []
-            for o, p, g in todo:
+                dtype = p.dtype
+                if g.dtype is not dtype or g.layout is not torch.strided:
+                    raise ValueError(f"AdamW: a {g.dtype} gradient (dense ones only) of a {dtype} parameter")
+                if not (p.is_contiguous() and g.is_contiguous()) and _strides(g) != _strides(p):
+                    g = torch.empty_like(p).copy_(g.detach())          # the parameter's order of elements
+                params.append(p)
+                grads.append(g)
                 s = self.state[p]
                 if not s:
-                    s.update(self._make_state(p))
+                    fresh.append(p)
+                todo = work.get((p.device, gi, dtype))
+                if todo is None:
+                    todo = work[(p.device, gi, dtype)] = []
+                todo.append((p, g, s, ordinal))
+        self.grad_norm = None
+        if not work:
+            if bound is not None:
+                self.grad_norm = torch.zeros(())
+            return loss
+        if torch.cuda.is_current_stream_capturing():
+            if not capturable:
+                raise lib.HoicError("AdamW: a captured step needs capturable=True (its step count would stand still)")
+            if fresh:
+                raise lib.HoicError("AdamW: take one eager step before a capture (the states would be made anew at every replay)")
+        for p in fresh:
+            self.state[p].update(self._make_state(p))
+        L = lib.load()
+        buf_ptr = norm_ptr = parts = 0
+        if bound is not None:
+            args, parts, held = _norm_list(grads)
+            dev = held[0].device
+            self.grad_norm = norm = torch.empty((), dtype=torch.float32, device=dev)
+            if parts:
+                buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
+                buf_ptr, norm_ptr = buf.data_ptr(), norm.data_ptr()
+                with _Launch(dev) as st:
+                    lib._chk(L.hoic_grad_norm_partial(*args, buf_ptr, st), "hoic_grad_norm_partial")
+            else:
+                norm.zero_()
+        for (dev, gi, dtype), todo in work.items():
+            group = self.param_groups[gi]
+            lr, (b1, b2) = group["lr"], group["betas"]
+            lr_ptr = 0
+            if isinstance(lr, torch.Tensor):
+                if not capturable or lr.device != dev or lr.dtype != torch.float32 or lr.numel() != 1:
+                    raise ValueError("lr: a float, or with capturable=True a float32 tensor of one element on the parameters' device")
+                lr, lr_ptr = 0.0, lr.data_ptr()
+            flat, t, d_step, ms, vs = [], 0, 0, 0, 0
+            for p, g, s, o in todo:
                 if capturable:
-                    t, d_step = 0, s["step"].data_ptr()
+                    d_step = s["step"].data_ptr()
                 else:
                     s["step"] = t = s["step"] + 1
-                    d_step = 0
-                ms, vs = (s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr()) if bits == 8 else (0, 0)
+                if bits == 8:
+                    ms, vs = s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr()
                 flat += (p.data_ptr(), g.data_ptr(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), ms, vs, p.numel(), t, d_step, o)
-            a = lib.AdamWArgs()
-            lr = group["lr"]
-            a.type, a.state_bits = TYPES[dtype], bits
-            if isinstance(lr, torch.Tensor):
-                if not capturable or lr.device != dev or lr.dtype != torch.float32:
-                    raise ValueError("lr: a float, or with capturable=True a float32 tensor on the parameters' device")
-                a.lr, a.d_lr = 0.0, lr.data_ptr()
-            else:
-                a.lr = float(lr)
-            (a.b1, a.b2), a.eps, a.weight_decay, a.seed = group["betas"], group["eps"], group["weight_decay"], group["seed"]
             consts = torch.empty(4 * len(todo), dtype=torch.float32, device=dev) if capturable else None
-            a.d_clip = None if clip is None else clip.data_ptr()
-            a.d_consts = None if consts is None else consts.data_ptr()
-            with torch.cuda.device(dev):
-                lib._chk(L.hoic_adamw((C.c_int64 * len(flat))(*flat), len(todo), C.byref(a), _stream(dev)), "hoic_adamw")
-            for _, p, _ in todo:
-                torch.autograd.graph.increment_version(p)
+            a = lib.ADAMW_ARGS.pack(TYPES[dtype], bits, lr, b1, b2, group["eps"], group["weight_decay"], lr_ptr,
+                                    0 if consts is None else consts.data_ptr(), buf_ptr, norm_ptr, bound or 0.0, parts, group["seed"], 0)
+            with _Launch(dev) as st:
+                lib._chk(L.hoic_adamw((C.c_int64 * len(flat))(*flat), len(todo), a, st), "hoic_adamw")
+        torch.autograd.graph.increment_version(params)
         return loss
 
-    @torch.no_grad()
     def state_values(self):
         """([m, ...], [v, ...]): both moments of every parameter in float32 (8-bit states: the values that their codes stand for, made
         anew by one launch per 48 tensors; 32-bit ones: the states themselves); zeros where a parameter has no state yet."""
-        params = [p for g in self.param_groups for p in g["params"]]
-        if self.defaults["state_bits"] == 32:
-            get = lambda key: [self.state[p][key] if p in self.state and self.state[p] else torch.zeros_like(p, dtype=torch.float32) for p in params]
-            return get("exp_avg"), get("exp_avg_sq")
-        L, out, work = lib.load(), ({}, {}), {}
-        for p in params:
-            work.setdefault(p.device, []).append(p)
-        for dev, ps in work.items():
-            with torch.cuda.device(dev):
-                # one buffer for all values: each tensor's stretch starts at a multiple of 4 elements
-                at, ends = [], 0
-                for p in ps:
-                    at.append(ends)
-                    ends += (p.numel() + 3) // 4 * 4
-                bufs = (torch.empty(ends, dtype=torch.float32, device=dev), torch.empty(ends, dtype=torch.float32, device=dev))
-                flat, n = [], 0
-                for p, i in zip(ps, at):
-                    for o, b in zip(out, bufs):
-                        o[p] = b.as_strided(p.shape, p.stride(), i)
-                    s = self.state.get(p)
-                    if not s:
-                        out[0][p].zero_(), out[1][p].zero_()
-                        continue
-                    flat += (bufs[0].data_ptr() + 4 * i, bufs[1].data_ptr() + 4 * i, s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(),
-                             s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr(), p.numel(), 1, 0, 0)
-                    n += 1
-                lib._chk(L.hoic_adamw_values((C.c_int64 * len(flat))(*flat), n, _stream(dev)), "hoic_adamw_values")
-        return [out[0][p] for p in params], [out[1][p] for p in params]
+        ms, vs, work = [], [], {}
+        bits = self.defaults["state_bits"]
+        for group in self.param_groups:
+            for p in group["params"]:
+                s = self.state.get(p)
+                if not s:
+                    m, v = torch.zeros_like(p, dtype=torch.float32, requires_grad=False), torch.zeros_like(p, dtype=torch.float32, requires_grad=False)
+                elif bits == 32:
+                    m, v = s["exp_avg"], s["exp_avg_sq"]
+                else:
+                    m, v = torch.empty_like(p, dtype=torch.float32, requires_grad=False), torch.empty_like(p, dtype=torch.float32, requires_grad=False)
+                    work.setdefault(p.device, []).extend((m.data_ptr(), v.data_ptr(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(),
+                                                          s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr(), p.numel(), 1, 0, 0))
+                ms.append(m)
+                vs.append(v)
+        for dev, flat in work.items():
+            with _Launch(dev) as st:
+                lib._chk(lib.load().hoic_adamw_values((C.c_int64 * len(flat))(*flat), len(flat) // 10, st), "hoic_adamw_values")
+        return ms, vs
 
+
+AdamW._step_hooked = torch.optim.Optimizer.profile_hook_step(AdamW._step)

@@ -196,84 +196,86 @@ class PolicyLossGrad(NamedTuple):
 _LOSS_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}         # enum hoic_type
 
 
+def _loss_rows(t, name, M, N, dev, types, shared=False):
+    """[M, N] (``shared``: or one row for all) of the right type and place, with unit stride along the dimensions"""
+    if shared and t.dim() == 1:
+        t = t[None]
+    if t.dim() != 2 or t.shape[1] != N or (t.shape[0] != M and not (shared and t.shape[0] == 1)):
+        raise ValueError(f"{name}: {tuple(t.shape)} for means of {(M, N)}")
+    if t.dtype not in types or t.device != dev:
+        raise ValueError(f"{name}: {t.dtype} on {t.device}; wanted {' or '.join(str(x) for x in types)} on {dev}")
+    if t.is_contiguous():
+        return t
+    if shared and t.shape[0] > 1 and t.stride(0) == 0:
+        return t.contiguous()                      # a row expanded over the batch: its gradient has a value per row
+    return t if t.stride(1) == 1 or N == 1 else t.contiguous()
+
+
+def _loss_flat(t, name, M, dev, types):
+    if t.numel() != M or t.dtype not in types or t.device != dev:
+        raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device} for {M} rows on {dev}")
+    return t if t.is_contiguous() else t.reshape(-1).contiguous()
+
+
 def _loss_inputs(mean, log_std, actions, advantages, fixed, clip_epsilon, ref_mean, ref_log_std, kl_coef, valid):
-    """Checks of the policy loss's arguments; row tensors come back with unit stride along the dimensions, vectors flat."""
+    """Checks of the policy loss's arguments; row tensors come back with unit stride along the dimensions, vectors contiguous."""
     if mean.dim() != 2 or mean.shape[1] < 1:
         raise ValueError(f"mean must be [rows, dimensions], not {tuple(mean.shape)}")
     M, N = mean.shape
-    dev = mean.device
-
-    def rows(t, name, types, shared=False):
-        if shared and t.dim() == 1:
-            t = t[None]
-        if t.dim() != 2 or t.shape[1] != N or (t.shape[0] != M and not (shared and t.shape[0] == 1)):
-            raise ValueError(f"{name}: {tuple(t.shape)} for means of {(M, N)}")
-        if t.device != dev or t.dtype not in types:
-            raise ValueError(f"{name}: {t.dtype} on {t.device}; wanted {' or '.join(str(x) for x in types)} on {dev}")
-        if shared and t.shape[0] > 1 and t.stride(0) == 0:
-            t = t.contiguous()                     # a row expanded over the batch: its gradient has a value per row
-        return t if t.stride(1) == 1 or N == 1 else t.contiguous()
-
-    def flat(t, name, types):
-        if t.numel() != M or t.device != dev or t.dtype not in types:
-            raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device} for {M} rows on {dev}")
-        return t.reshape(-1).contiguous()
-
-    f32 = torch.float32 if mean.dtype != torch.float64 else torch.float64
-    own, wide = (mean.dtype,), (mean.dtype, f32)
-    if not mean.dtype.is_floating_point:
-        raise ValueError(f"mean: a floating type, not {mean.dtype}")
-    if (ref_mean is None) != (ref_log_std is None):
+    dev, dtype = mean.device, mean.dtype
+    if not dtype.is_floating_point:
+        raise ValueError(f"mean: a floating type, not {dtype}")
+    f32 = torch.float32 if dtype is not torch.float64 else dtype
+    if (ref_mean is None) is not (ref_log_std is None):
         raise ValueError("the reference policy is ref_mean and ref_log_std together")
     if ref_mean is None and kl_coef:
         raise ValueError("kl_coef needs a reference policy (ref_mean, ref_log_std)")
     lo, hi = clip_epsilon if isinstance(clip_epsilon, (tuple, list)) else (clip_epsilon, clip_epsilon)
     if not (0.0 <= lo < math.inf and 0.0 <= hi < math.inf and math.isfinite(kl_coef)):
         raise ValueError(f"clip_epsilon {clip_epsilon} (>= 0) or kl_coef {kl_coef}")
-    mean, actions = rows(mean, "mean", own), rows(actions, "actions", wide)
-    log_std = rows(log_std, "log_std", wide, True)
-    advantages = flat(advantages, "advantages", (f32,))
-    fixed = None if fixed is None else flat(fixed, "fixed_log_probs", (f32,))
+    wide = (dtype, f32)
+    mean, actions = _loss_rows(mean, "mean", M, N, dev, wide), _loss_rows(actions, "actions", M, N, dev, wide)
+    log_std = _loss_rows(log_std, "log_std", M, N, dev, wide, True)
+    advantages = _loss_flat(advantages, "advantages", M, dev, (f32,))
+    if fixed is not None:
+        fixed = _loss_flat(fixed, "fixed_log_probs", M, dev, (f32,))
     if ref_mean is not None:
-        ref_mean, ref_log_std = rows(ref_mean, "ref_mean", own).detach(), rows(ref_log_std, "ref_log_std", (log_std.dtype,), True).detach()
-    valid = None if valid is None else flat(valid, "valid", (torch.bool, torch.uint8))
+        ref_mean = _loss_rows(ref_mean, "ref_mean", M, N, dev, (dtype,))
+        ref_log_std = _loss_rows(ref_log_std, "ref_log_std", M, N, dev, (log_std.dtype,), True)
+    if valid is not None:
+        valid = _loss_flat(valid, "valid", M, dev, (torch.bool, torch.uint8))
     return mean, log_std, actions, advantages, fixed, (float(lo), float(hi)), ref_mean, ref_log_std, valid
 
 
 def _policy_loss_launch(x, kl_coef, weight, grad, upstream=None, count=None):
     """hoic_policy_loss on checked inputs -> (out [8] or None, d_mean, d_log_std [1 or M, N], log_probs)"""
     from . import lib
-    import ctypes as C
+    from .optim import _Launch
     mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid = x
     M, N = mean.shape
     if N > 256:
         raise ValueError(f"the policy loss's kernel takes up to 256 action dimensions, not {N}")
-    L, dev = lib.load(), mean.device
+    L, dev, f32, empty = lib.load(), mean.device, torch.float32, torch.empty
+    out = empty(8, dtype=f32, device=dev) if count is None else None
+    d_mean = empty((M, N), dtype=mean.dtype, device=dev) if grad else None
+    d_log_std = empty(log_std.shape, dtype=log_std.dtype, device=dev) if grad else None
+    log_probs = empty((M, 1), dtype=f32, device=dev) if fixed is None and count is None else None
     if M == 0:
-        zeros = lambda *shape, dtype=torch.float32: torch.zeros(shape, dtype=dtype, device=dev)
-        return (zeros(8) if count is None else None, zeros(0, N, dtype=mean.dtype) if grad else None,
-                zeros(*log_std.shape, dtype=log_std.dtype) if grad else None, zeros(0, 1) if fixed is None and count is None else None)
-    a = lib.PolicyLossArgs()
-    new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=dev)
-    scratch = new((int(L.hoic_policy_loss_scratch_bytes(N)),), torch.uint8)
-    out = new((8,), torch.float32) if count is None else None
-    d_mean = new((M, N), mean.dtype) if grad else None
-    d_log_std = new(log_std.shape, log_std.dtype) if grad else None
-    log_probs = new((M, 1), torch.float32) if fixed is None and count is None else None
-    a.rows, a.dims = M, N
-    a.t_mean, a.t_act, a.t_std = _LOSS_TYPES[mean.dtype], _LOSS_TYPES[actions.dtype], _LOSS_TYPES[log_std.dtype]
-    # (a leading 1 is a shared row: stride 0; so is [M, N] = [1, N])
-    ld = lambda t: 0 if t.shape[0] == 1 else t.stride(0)
-    for name, t in (("mean", mean), ("act", actions), ("log_std", log_std), ("ref_mean", ref_mean), ("ref_log_std", ref_log_std), ("adv", advantages),
-                    ("fixed", fixed), ("valid", valid), ("upstream", upstream), ("count", count), ("d_mean", d_mean), ("d_log_std", d_log_std),
-                    ("log_probs", log_probs), ("out", out), ("scratch", scratch)):
-        setattr(a, name, None if t is None else t.data_ptr())
-    a.ld_mean, a.ld_act, a.ld_std, a.ld_dmean = mean.stride(0), actions.stride(0), ld(log_std), N
-    if ref_mean is not None:
-        a.ld_ref_mean, a.ld_ref_std = ref_mean.stride(0), ld(ref_log_std)
-    (a.clip_lo, a.clip_hi), a.kl_coef, a.weight = clip, float(kl_coef), float(weight)
-    with torch.cuda.device(dev):
-        rc = L.hoic_policy_loss(C.byref(a), C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+        for t in (out, d_log_std):
+            if t is not None:
+                t.zero_()
+        return out, d_mean, d_log_std, log_probs
+    scratch = empty(L.hoic_policy_loss_scratch_bytes(N), dtype=torch.uint8, device=dev)
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    ld = lambda t: 0 if t is None or t.shape[0] == 1 else t.stride(0)          # (one row is a shared one: stride 0)
+    args = lib.POLICY_LOSS_ARGS.pack(
+        M, N, _LOSS_TYPES[mean.dtype], _LOSS_TYPES[actions.dtype], _LOSS_TYPES[log_std.dtype],
+        mean.data_ptr(), actions.data_ptr(), log_std.data_ptr(), ptr(ref_mean), ptr(ref_log_std),
+        mean.stride(0), actions.stride(0), ld(log_std), 0 if ref_mean is None else ref_mean.stride(0), ld(ref_log_std), N,
+        advantages.data_ptr(), ptr(fixed), ptr(valid), ptr(upstream), ptr(count), clip[0], clip[1], kl_coef, weight,
+        ptr(d_mean), ptr(d_log_std), ptr(log_probs), ptr(out), scratch.data_ptr())
+    with _Launch(dev) as st:
+        rc = L.hoic_policy_loss(args, st)
     if rc != 0:
         raise lib.HoicError(f"hoic_policy_loss failed ({rc}): {L.hoic_last_error().decode()}")
     return out, d_mean, d_log_std, log_probs
@@ -306,6 +308,8 @@ class _ClippedPolicyLoss(torch.autograd.Function):
 def _policy_loss_tensors(x, kl_coef):
     """The loss as tensor operations (CPU and float64 tensors; what the kernel computes, row by row)"""
     mean, log_std, actions, advantages, fixed, (lo, hi), ref_mean, ref_log_std, valid = x
+    advantages, fixed, valid = (None if t is None else t.reshape(-1) for t in (advantages, fixed, valid))
+    ref_mean, ref_log_std = (None if t is None else t.detach() for t in (ref_mean, ref_log_std))
     if valid is not None:                          # rows outside the batch may hold anything: they are left out, not multiplied by 0
         keep = valid.bool()
         cut = lambda t: t if t is None or (t.shape[0] != keep.shape[0]) else t[keep]
@@ -368,10 +372,9 @@ def clipped_policy_loss_grad(mean, log_std, actions, advantages, fixed_log_probs
             loss, info, log_probs = _policy_loss_tensors(_loss_inputs(mu, s, *args), kl_coef)
             d_mean, d_log_std = torch.autograd.grad(loss * weight, (mu, s))
         return PolicyLossGrad(loss.detach(), info, d_mean, d_log_std, log_probs)
-    with torch.no_grad():
-        x = _loss_inputs(mean, log_std, *args)
-        out, d_mean, d_log_std, log_probs = _policy_loss_launch(x, kl_coef, weight, True)
-        return PolicyLossGrad(out[0], out[1:5], d_mean, d_log_std.view(log_std.shape), log_probs)
+    x = _loss_inputs(mean, log_std, *args)
+    out, d_mean, d_log_std, log_probs = _policy_loss_launch(x, float(kl_coef), float(weight), True)
+    return PolicyLossGrad(out[0], out[1:5], d_mean, d_log_std if log_std.dim() == 2 else d_log_std[0], log_probs)
 
 
 # ----------------------------------------------------------------------------- observation filter

@@ -376,17 +376,20 @@ typedef struct hoic_policy_loss_args {
 } hoic_policy_loss_args;
 int64_t hoic_policy_loss_scratch_bytes(int32_t dims);
 int32_t hoic_policy_loss(const hoic_policy_loss_args* a, void* stream);
-/* The norm of a list of gradients (the learner clips the policy's at 40: agent_handmimic.py:67) in two steps: hoic_grad_norm_partial
- * writes hoic_grad_norm_parts(n, nt) partial sums of squares of nt contiguous tensors of one type (once per type, behind one
- * another); hoic_grad_norm_finish joins them in fixed order: d_clip[0] = norm, d_clip[1] = min(1, bound / (norm + 1e-6)) in
- * 64 bits, d_norm[0] = norm.  hoic_scale_list: g *= d_clip[1] (a factor of 1 touches nothing).  The lists are HOST arrays. */
+/* The norm of a list of gradients (the learner clips the policy's at 40: agent_handmimic.py:67).  The lists are HOST arrays: nt
+ * pointers to contiguous tensors, their sizes and types (enum hoic_type, one byte each), not all empty.  Sums in 64 bits in a fixed
+ * order.  d_buf: hoic_grad_norm_parts(n, nt) + 2 doubles of scratch; d_norm: the norm in float32.
+ * hoic_grad_norm: the norm; d_buf[0..1] = {norm, 1} afterwards.
+ * hoic_grad_norm_partial: the parts alone, for hoic_adamw (d_norm_buf, norm_parts) to join.
+ * hoic_clip_grads: g *= min(1, bound / (norm + 1e-6)) in place (a factor of 1 touches nothing). */
 int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt);
-int32_t hoic_grad_norm_partial(const void* const* g, const int64_t* n, int32_t nt, int32_t type, double* d_part, void* stream);
-int32_t hoic_grad_norm_finish(const double* d_part, int64_t nparts, double bound, double* d_clip, float* d_norm, void* stream);
-int32_t hoic_scale_list(void* const* g, const int64_t* n, int32_t nt, int32_t type, const double* d_clip, void* stream);
+int32_t hoic_grad_norm(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* d_buf, float* d_norm, void* stream);
+int32_t hoic_grad_norm_partial(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* d_buf, void* stream);
+int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double bound, double* d_buf, float* d_norm, void* stream);
 /* hoic_adamw: one AdamW step over nt tensors of one type (in the place of the optimiser step of agent_ppo.py:46-56 / agent_pg.py:18-25;
  * list in HOST memory).  m' = b1 m + (1 - b1) c g, v' = b2 v + (1 - b2) (c g)^2, p' = p - (lr wd p + lr / (1 - b1^t) m' / (sqrt(v' / (1 - b2^t))
- * + eps)).  d_clip: {norm, factor c} or NULL (c = 1); a norm that is not finite leaves everything as it is.
+ * + eps)).  c = 1 without d_norm_buf; with it c = min(1, bound / (norm + 1e-6)) from the norm_parts parts of hoic_grad_norm_partial
+ * (the norm comes back in d_norm), and a norm that is not finite leaves everything as it is.
  *   state_bits 32: m, v float32 [n];  8: m, v bytes [n], m_scale, v_scale float32 [ceil(n / 256)]: blocks of 256 in storage order, a
  *   power-of-two scale each; m sign + e4m3 (bias 7), v e5m3 (bias 15) without sign; rounded up with the probability of the part cut
  *   off by a hash of (seed, t, ordinal, element); 0x7f / 0xff stand for values that are not finite
@@ -406,8 +409,11 @@ typedef struct hoic_adamw_args {
   int32_t type, state_bits;
   double lr, b1, b2, eps, weight_decay;
   const float* d_lr;
-  const double* d_clip;
   float* d_consts;
+  double* d_norm_buf;
+  float* d_norm;
+  double bound;
+  int64_t norm_parts;
   uint32_t seed, reserved;
 } hoic_adamw_args;
 int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic_adamw_args* a, void* stream);

@@ -325,22 +325,15 @@ def test_policy_loss_tensor_form_and_refusals():
 
 def test_policy_loss_entry_point_refuses_on_the_host():
     """hoic_policy_loss checks its arguments before any launch (no GPU is needed to see it)"""
-    import ctypes as C
     L = lib.load()
     assert L.hoic_policy_loss(None, None) == -1
-    a = lib.PolicyLossArgs()
-    buf = C.create_string_buffer(64)
-    at = C.cast(buf, C.c_void_p).value
-    def ok():
-        for n in ("mean", "act", "log_std", "adv", "out", "scratch"):
-            setattr(a, n, at)
-        a.rows, a.dims, a.t_mean, a.t_act, a.t_std, a.ref_mean, a.ref_log_std, a.d_mean, a.d_log_std, a.count = 4, 4, 0, 0, 0, None, None, None, None, None
-    for change in (dict(dims=0), dict(dims=257), dict(rows=-1), dict(t_mean=3), dict(t_mean=2, t_act=1), dict(t_std=1), dict(mean=None), dict(scratch=None), dict(out=None),
+    names = ("rows dims t_mean t_act t_std mean act log_std ref_mean ref_log_std ld_mean ld_act ld_std ld_ref_mean ld_ref_std ld_dmean adv fixed valid upstream count "
+             "clip_lo clip_hi kl_coef weight d_mean d_log_std log_probs out scratch").split()
+    at = 64
+    good = dict.fromkeys(names, 0) | dict(rows=4, dims=4, mean=at, act=at, log_std=at, adv=at, out=at, scratch=at)
+    for change in (dict(dims=0), dict(dims=257), dict(rows=-1), dict(t_mean=3), dict(t_mean=2, t_act=1), dict(t_std=1), dict(mean=0), dict(scratch=0), dict(out=0),
                    dict(ref_mean=at), dict(ref_log_std=at), dict(d_log_std=at), dict(count=at)):
-        ok()
-        for k, v in change.items():
-            setattr(a, k, v)
-        assert L.hoic_policy_loss(C.byref(a), None) == -1, change
+        assert L.hoic_policy_loss(lib.POLICY_LOSS_ARGS.pack(*(good | change).values()), None) == -1, change
     assert L.hoic_policy_loss_scratch_bytes(0) == 0
 
 
@@ -409,12 +402,16 @@ def test_norm_refusals():
         optim.clip_grad_norm_([p], 1.0)
     import ctypes as C
     L = lib.load()
-    one = (C.c_int64 * 1)(4)
-    null = (C.c_void_p * 1)(None)
+    one, none = (C.c_int64 * 1)(4), (C.c_int64 * 1)(0)
+    null, some = (C.c_void_p * 1)(None), (C.c_void_p * 1)(8)
     assert L.hoic_grad_norm_parts(None, 1) == -1 and L.hoic_grad_norm_parts(one, 1) == 1
-    assert L.hoic_grad_norm_partial(null, one, 1, 0, one, None) == -1 and L.hoic_grad_norm_partial(null, one, 1, 5, one, None) == -1
-    assert L.hoic_grad_norm_finish(None, 1, 1.0, one, one, None) == -1 and L.hoic_grad_norm_finish(one, 1, -1.0, one, one, None) == -1
-    assert L.hoic_scale_list(null, one, 1, 0, None, None) == -1
+    for g, n, t, nt, buf, norm in ((null, one, b"\0", 1, 8, 8), (some, one, b"\5", 1, 8, 8), (some, (C.c_int64 * 1)(-1), b"\0", 1, 8, 8), (some, one, None, 1, 8, 8),
+                                   (some, one, b"\0", -1, 8, 8), (some, one, b"\0", 1, None, 8)):
+        assert L.hoic_grad_norm(g, n, t, nt, buf, norm, None) == -1 and L.hoic_clip_grads(g, n, t, nt, 1.0, buf, norm, None) == -1
+        assert L.hoic_grad_norm_partial(g, n, t, nt, buf, None) == -1
+    for n, norm, bound in ((one, None, 1.0), (none, 8, 1.0), (one, 8, -1.0), (one, 8, math.nan)):
+        assert L.hoic_clip_grads(some, n, b"\0", 1, bound, 8, norm, None) == -1
+    assert L.hoic_grad_norm(some, none, b"\0", 1, 8, 8, None) == -1
 
 
 # ================================================================================================ AdamW
@@ -847,15 +844,13 @@ def test_adamw_refusals():
             optim.AdamW([torch.nn.Parameter(torch.zeros(3))], **kw)
     import ctypes as C
     L = lib.load()
-    def args(**kw):
-        a = lib.AdamWArgs()
-        a.type, a.state_bits, a.lr, a.b1, a.b2, a.eps = 0, 32, 1e-3, 0.9, 0.999, 1e-8
-        for k, v in kw.items():
-            setattr(a, k, v)
-        return C.byref(a)
+    fields = dict(type=0, state_bits=32, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, weight_decay=0.0, d_lr=0, d_consts=0, d_norm_buf=0, d_norm=0, bound=0.0, norm_parts=0, seed=0,
+                  reserved=0)
+    args = lambda **kw: lib.ADAMW_ARGS.pack(*(fields | kw).values())
     row = lambda **kw: (C.c_int64 * 10)(*[kw.get(k, d) for k, d in zip(("p", "g", "m", "v", "ms", "vs", "n", "step", "d_step", "ordinal"), (8, 8, 8, 8, 0, 0, 4, 1, 0, 0))])
     for a, t in ((args(type=3), row()), (args(state_bits=16), row()), (args(b1=1.0), row()), (args(eps=-1.0), row()), (args(), row(p=0)), (args(), row(g=0)), (args(), row(m=0)),
-                 (args(), row(v=0)), (args(), row(n=-1)), (args(), row(step=0)), (args(state_bits=8), row()), (args(d_consts=8), row()), (args(), row(n=1 << 60))):
+                 (args(), row(v=0)), (args(), row(n=-1)), (args(), row(step=0)), (args(state_bits=8), row()), (args(d_consts=8), row()), (args(), row(n=1 << 60)),
+                 (args(d_norm_buf=8, d_norm=8), row()), (args(d_norm_buf=8, norm_parts=1), row()), (args(d_norm_buf=8, d_norm=8, norm_parts=1, bound=-1.0), row())):
         assert L.hoic_adamw(t, 1, a, None) == -1
     assert L.hoic_adamw(None, 1, args(), None) == -1 and L.hoic_adamw(row(), 1, None, None) == -1 and L.hoic_adamw(row(), -1, args(), None) == -1
     assert L.hoic_adamw_values(row(), 1, None) == -1 and L.hoic_adamw_values(None, 1, None) == -1
