@@ -1928,9 +1928,22 @@ __device__ __forceinline__ AdamConsts adam_consts(const AdamArgs& a, int t) {
   }
   return c;
 }
+// The step of one parameter with the 1-ulp hardware square root and reciprocal (the precise forms cost 20 instructions more, a
+// fifth of the 8-bit kernel, and p rounds to far more than an ulp of its step).  The square root takes no subnormals: v is
+// scaled by 2^64 below 2^-96; the reciprocal's argument is not subnormal (host: eps is 0 or at least the smallest normal).
 __device__ __forceinline__ float adam_param(float p, float m, float v, const AdamConsts& c, float eps) {
-  const float u = c.size * m / fmaf(sqrtf(v), c.rroot, eps);
+  const bool small = v < 1.262177448e-29f;
+  const float root = __builtin_amdgcn_sqrtf(v * (small ? 18446744073709551616.f : 1.f)) * (small ? 2.328306437e-10f : 1.f);
+  const float u = c.size * m * __builtin_amdgcn_rcpf(fmaf(root, c.rroot, eps));
   return p - fmaf(c.lrwd, p, u);
+}
+// maximum over the wavefront, in a scalar register: four steps inside the rows of 16 lanes, two across them
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+#define DPP_MAX(ctrl, rows) x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false))
+  DPP_MAX(0x111, 0xf); DPP_MAX(0x112, 0xf); DPP_MAX(0x114, 0xf); DPP_MAX(0x118, 0xf);      // row_shr 1, 2, 4, 8
+  DPP_MAX(0x142, 0xa); DPP_MAX(0x143, 0xc);                                                 // row_bcast 15 (rows 1, 3), 31 (rows 2, 3)
+#undef DPP_MAX
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
 #define ADAM32_CHUNK 4096
 #define JOIN_BLOCKS 4096         // a launch of more workgroups is given the joined factor
@@ -2006,6 +2019,57 @@ __device__ __forceinline__ unsigned code8(double a, double r, int up, int low, u
   return (unsigned)(q + u) + (unsigned)(ey - low) * 8u;
 }
 #define ADAM8_CHUNK 4096
+// One block of 256 elements from element i0 + ob on in the tensor form's arithmetic (a wavefront): blocks in which a value lies next to a
+// border or is not finite.
+template <class T> __device__ __forceinline__ void adam8_block(const AdamArgs& a, int t, const AdamConsts& c, double cl, unsigned key, long long i0, long long ob, long long left,
+                                                               int lane) {
+  T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; unsigned char* m = (unsigned char*)a.t[t].m; unsigned char* v = (unsigned char*)a.t[t].v;
+  const long long o = ob + lane * 4, i = i0 + o, blk = (i0 + ob) >> 8;
+  const int l = left - o >= 4 ? 4 : left - o > 0 ? (int)(left - o) : 0;
+  f32x4 pp = load4(p + (l ? i : 0), l), gg = load4(g + (l ? i : 0), l);
+  unsigned cm = 0, cv = 0;
+  for (int e = 0; e < l; e++) { cm |= (unsigned)m[i + e] << (8 * e); cv |= (unsigned)v[i + e] << (8 * e); }
+  const double km = (double)a.t[t].ms[blk], kv = (double)a.t[t].vs[blk];
+  double mm[4], vv[4];
+  unsigned hm = 0, hv = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const double x = (double)gg[e] * cl;
+    mm[e] = rounded(a.b1d * m_old((cm >> (8 * e)) & 0xff, km)) + rounded(a.c1d * x);
+    vv[e] = rounded(a.b2d * v_old((cv >> (8 * e)) & 0xff, kv)) + rounded(a.c2d * x * x);
+    if (vv[e] > 3.4028234663852886e38 && vv[e] < INFINITY) vv[e] = 3.4028234663852886e38;
+    const unsigned am = hi32(mm[e]) & 0x7fffffffu, av = hi32(vv[e]);
+    if (am < 0x7ff00000u && am > hm) hm = am;
+    if (av < 0x7ff00000u && av > hv) hv = av;
+    pp[e] = adam_param(pp[e], (float)mm[e], (float)vv[e], c, a.eps);
+  }
+  hm = wave_max(hm); hv = wave_max(hv);
+  const int em = max((int)(hm >> 20) - 1023 - 7, -126), ev = max((int)(hv >> 20) - 1023 - 15, -126);
+  const double rm = pow2d(-em), rv = pow2d(-ev);
+  const int um = pow_down(em), uv = pow_down(ev);
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const unsigned h = mix32((unsigned)(i + e) + key);
+    unsigned qm = code8(fabs(mm[e]), rm, um, -6, h & 0xffff) | (mm[e] < 0. ? 0x80u : 0u);
+    unsigned qv = code8(vv[e], rv, uv, -14, h >> 16);
+    qv = qv == 0 && vv[e] > 0. ? 1u : qv;
+    qm = (hi32(mm[e]) & 0x7ff00000u) == 0x7ff00000u ? 0x7fu : qm;
+    qv = (hi32(vv[e]) & 0x7ff00000u) == 0x7ff00000u ? 0xffu : qv;
+    if (e < l) { m[i + e] = (unsigned char)qm; v[i + e] = (unsigned char)qv; }
+  }
+  store4(p + i, l, pp);
+  if (lane == 0) { a.t[t].ms[blk] = pow2f(em); a.t[t].vs[blk] = pow2f(ev); }
+}
+// The same code without the last bits: y = a / k by an exact product, below 2^low with 2^low added (the step there is that of the
+// binade above, the code counts from 0); of the high word's 20 mantissa bits 3 stay, the 17 below them carry with 2 r + 1 of
+// 2^17 or do not.  `near` falls under 2^16 where the sum is within 2^-17 of a step of its border.
+__device__ __forceinline__ unsigned code8_quick(double a, double r, int low, unsigned u17, unsigned& near) {
+  const double y = a * r;
+  const bool sub = y < pow2d(low);
+  const unsigned t = hi32(y + (sub ? pow2d(low) : 0.)) + u17;
+  near = min(near, (t << 15) + 0x8000u);
+  return (t >> 17) - (sub ? (unsigned)(1023 + low) * 8u : (unsigned)(1022 + low) * 8u);
+}
 template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   double cl = 1.;
@@ -2016,53 +2080,68 @@ template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(Ada
   }
   const AdamConsts c = adam_consts(a, t);
   T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; unsigned char* m = (unsigned char*)a.t[t].m; unsigned char* v = (unsigned char*)a.t[t].v;
+  float* ms = a.t[t].ms; float* vs = a.t[t].vs;
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM8_CHUNK, left = a.t[t].n - i0;
   const unsigned key = mix32(c.key + (unsigned)(i0 >> 32));
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int u = 0; u < ADAM8_CHUNK / 1024; u++) {
-    const long long ob = (u * 4 + wave) * 256;
-    if (ob >= left) break;                                          // (wavefront-uniform)
-    const long long o = ob + lane * 4, i = i0 + o, blk = (i0 + ob) >> 8;
-    const int l = left - o >= 4 ? 4 : left - o > 0 ? (int)(left - o) : 0;
-    f32x4 pp = load4(p + (l ? i : 0), l), gg = load4(g + (l ? i : 0), l);
-    unsigned cm = 0, cv = 0;
-    if (l == 4) { cm = *(const unsigned*)(m + i); cv = *(const unsigned*)(v + i); }
-    else for (int e = 0; e < l; e++) { cm |= (unsigned)m[i + e] << (8 * e); cv |= (unsigned)v[i + e] << (8 * e); }
-    const double km = (double)a.t[t].ms[blk], kv = (double)a.t[t].vs[blk];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  constexpr int U = ADAM8_CHUNK / 1024;
+  unsigned again = 0;               // blocks left to adam8_block, a tensor's last, partial one among them
+  // all loads of the wavefront's blocks first
+  f32x4 pp[U], gg[U];
+  unsigned cm[U], cv[U];
+  float km[U], kv[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const long long ob = (u * 4 + wave) * 256, i = i0 + ob + lane * 4;
+    if (ob + 256 > left) continue;
+    pp[u] = load4(p + i, 4); gg[u] = load4(g + i, 4);
+    cm[u] = *(const unsigned*)(m + i); cv[u] = *(const unsigned*)(v + i);
+    km[u] = ms[(i0 + ob) >> 8]; kv[u] = vs[(i0 + ob) >> 8];
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const long long ob = (u * 4 + wave) * 256, i = i0 + ob + lane * 4, blk = (i0 + ob) >> 8;
+    if (ob >= left) break;
+    if (ob + 256 > left) { again |= 1u << u; break; }
+    const double km1 = (double)km[u], kv1 = (double)kv[u], bm = a.b1d * km1, bv = a.b2d * kv1 * pow2d(112);
+    const f32x4 gu = gg[u];
+    const unsigned cmu = cm[u], cvu = cv[u];
     double mm[4], vv[4];
+    float mf[4], vf[4];
     unsigned hm = 0, hv = 0;
+    const float om_[4] = {__builtin_amdgcn_cvt_f32_fp8(cmu, 0), __builtin_amdgcn_cvt_f32_fp8(cmu, 1), __builtin_amdgcn_cvt_f32_fp8(cmu, 2), __builtin_amdgcn_cvt_f32_fp8(cmu, 3)};
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const double x = (double)gg[e] * cl;
-      mm[e] = rounded(a.b1d * m_old((cm >> (8 * e)) & 0xff, km)) + rounded(a.c1d * x);
-      vv[e] = rounded(a.b2d * v_old((cv >> (8 * e)) & 0xff, kv)) + rounded(a.c2d * x * x);
-      if (vv[e] > 3.4028234663852886e38 && vv[e] < INFINITY) vv[e] = 3.4028234663852886e38;
-      const unsigned am = hi32(mm[e]) & 0x7fffffffu, av = hi32(vv[e]);
-      if (am < 0x7ff00000u && am > hm) hm = am;
-      if (av < 0x7ff00000u && av > hv) hv = av;
-      pp[e] = adam_param(pp[e], (float)mm[e], (float)vv[e], c, a.eps);
+      const double x = (double)gu[e] * cl;
+      mm[e] = fma((double)om_[e], bm, a.c1d * x);
+      vv[e] = fma(a.c2d * x, x, (double)__builtin_bit_cast(float, ((cvu >> (8 * e)) & 0xff) << 20) * bv);
+      hm = max(hm, hi32(mm[e]) & 0x7fffffffu); hv = max(hv, hi32(vv[e]));
+      mf[e] = (float)mm[e]; vf[e] = (float)vv[e];
     }
-#pragma unroll
-    for (int q = 32; q; q >>= 1) { hm = max(hm, (unsigned)__shfl_xor((int)hm, q, 64)); hv = max(hv, (unsigned)__shfl_xor((int)hv, q, 64)); }
+    hm = wave_max(hm); hv = wave_max(hv);
     const int em = max((int)(hm >> 20) - 1023 - 7, -126), ev = max((int)(hv >> 20) - 1023 - 15, -126);
     const double rm = pow2d(-em), rv = pow2d(-ev);
-    const int um = pow_down(em), uv = pow_down(ev);
-    unsigned om = 0, ov = 0;
+    unsigned om = 0, ov = 0, near = 0xffffffffu;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const unsigned h = mix32((unsigned)(i + e) + key);
-      unsigned qm = code8(fabs(mm[e]), rm, um, -6, h & 0xffff) | (mm[e] < 0. ? 0x80u : 0u);
-      unsigned qv = code8(vv[e], rv, uv, -14, h >> 16);
-      qv = qv == 0 && vv[e] > 0. ? 1u : qv;
-      qm = (hi32(mm[e]) & 0x7ff00000u) == 0x7ff00000u ? 0x7fu : qm;
-      qv = (hi32(vv[e]) & 0x7ff00000u) == 0x7ff00000u ? 0xffu : qv;
-      om |= qm << (8 * e); ov |= qv << (8 * e);
+      const unsigned qm = code8_quick(fabs(mm[e]), rm, -6, ((h & 0xffff) << 1) | 1, near), qv = code8_quick(vv[e], rv, -14, (h >> 15) | 1, near);
+      om |= (qm | ((hi32(mm[e]) >> 24) & 0x80u)) << (8 * e);
+      ov |= max(qv, min(hi32(vv[e]), 1u)) << (8 * e);
     }
-    if (l == 4) { *(unsigned*)(m + i) = om; *(unsigned*)(v + i) = ov; }
-    else for (int e = 0; e < l; e++) { m[i + e] = (unsigned char)(om >> (8 * e)); v[i + e] = (unsigned char)(ov >> (8 * e)); }
-    store4(p + i, l, pp);
-    if (lane == 0) { a.t[t].ms[blk] = pow2f(em); a.t[t].vs[blk] = pow2f(ev); }
+    // next to a border: a sum within 2^-17 of a step, a block maximum within 2^-20 of a power of two, values that are not finite
+    // (or held at float32's largest), a code that stands for one
+    const bool hard = near < 0x10000u || (hm && ((hm + 1) & 0xfffffu) < 2) || (hv && ((hv + 1) & 0xfffffu) < 2) || hm >= 0x7ff00000u || hv >= 0x47efffffu
+                      || (((cvu & 0x7f7f7f7fu) + 0x01010101u) & cvu & 0x80808080u);
+    if (__any(hard)) { again |= 1u << u; continue; }
+    f32x4 pu = pp[u];
+#pragma unroll
+    for (int e = 0; e < 4; e++) pu[e] = adam_param(pu[e], mf[e], vf[e], c, a.eps);
+    *(unsigned*)(m + i) = om; *(unsigned*)(v + i) = ov;
+    store4(p + i, 4, pu);
+    if (lane == 0) { ms[blk] = pow2f(em); vs[blk] = pow2f(ev); }
   }
+  for (; again; again &= again - 1) adam8_block<T>(a, t, c, cl, key, i0, ((__ffs(again) - 1) * 4 + wave) * 256, left, lane);
 }
 // the float32 values of 8-bit states: p, g of an entry are the places of m's and v's values
 __global__ __launch_bounds__(256) void hoic_adamw_values_kernel(AdamArgs a) {
@@ -2115,7 +2194,7 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
   static_assert(ADAM8_CHUNK == ADAM32_CHUNK, "one chunk size for the launch below");
   hipStream_t st = (hipStream_t)stream;
   AdamArgs a;
-  a.b1 = (float)x->b1; a.c1 = (float)(1. - x->b1); a.b2 = (float)x->b2; a.c2 = (float)(1. - x->b2); a.eps = (float)x->eps; a.lrwd = (float)(x->lr * x->weight_decay);
+  a.b1 = (float)x->b1; a.c1 = (float)(1. - x->b1); a.b2 = (float)x->b2; a.c2 = (float)(1. - x->b2); a.eps = x->eps > 0. ? std::max((float)x->eps, 1.17549435e-38f) : 0.f; a.lrwd = (float)(x->lr * x->weight_decay);
   a.b1d = x->b1; a.c1d = 1. - x->b1; a.b2d = x->b2; a.c2d = 1. - x->b2; a.consts = x->d_consts;
   a.at = 0;
   long long total = 0;
