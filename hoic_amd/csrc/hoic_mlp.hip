@@ -26,6 +26,7 @@
 #include <stdint.h>
 #include <algorithm>
 #include <string>
+#include <type_traits>
 #include "../../include/hoic.h"
 #include "hoic_zfilter_core.h"
 
@@ -1498,16 +1499,6 @@ template <class T> __device__ __forceinline__ void store4(T* __restrict__ x, int
     if (left > 2) x[2] = (T)r.z;
   }
 }
-__device__ __forceinline__ f32x4 load4_any(const void* x, long long i, int left, int type) {
-  if (type == HOIC_F32) return load4((const float*)x + i, left);
-  if (type == HOIC_F16) return load4((const _Float16*)x + i, left);
-  return load4((const __bf16*)x + i, left);
-}
-__device__ __forceinline__ void store4_any(void* x, long long i, int left, int type, f32x4 r) {
-  if (type == HOIC_F32) store4((float*)x + i, left, r);
-  else if (type == HOIC_F16) store4((_Float16*)x + i, left, r);
-  else store4((__bf16*)x + i, left, r);
-}
 
 // ---------------------------------------------------------------------------------------------- clipped policy loss with a KL term
 // rows m, action dimensions j; mu, s = log sigma, action a, advantage A, old log-probability l0, reference policy (mu0, s0):
@@ -1523,15 +1514,56 @@ struct PolicyLossArgs {
   hoic_policy_loss_args a;
   int lpr_log2;
   const int* counts; int ncounts;        // partial counts of the valid rows (gradient with a mask)
-  double* part;                          // [blocks][dims + 3]
+  double* part; int nb;                  // [dims + 4][PL_BLOCKS]: the workgroups' sums, column by column; how many there are
 };
 #define PL_NT 256
+#define PL_BLOCKS 1024
+#define PL_COUNTS 256
 
+// e^x to 2e-13: 2^k (1 + r + ... + r^10 / 10!), |r| <= ln 2 / 2; the next term is r^11 / 11! < 2.2e-13.  (A relative 2e-13 of a row's terms
+// moves its ratio by 1e-11.)  A NaN stays one; infinities are for exp_row.
+__device__ __forceinline__ double exp_terms(double x) {
+  const double k = __builtin_rint(x * 1.4426950408889634074);
+  double r = fma(k, -0x1.62e42fee00000p-1, x);
+  r = fma(k, -0x1.a39ef35793c76p-33, r);
+  double p = fma(r, 1. / 3628800., 1. / 362880.);
+  p = fma(r, p, 1. / 40320.); p = fma(r, p, 1. / 5040.); p = fma(r, p, 1. / 720.); p = fma(r, p, 1. / 120.); p = fma(r, p, 1. / 24.);
+  p = fma(r, p, 1. / 6.); p = fma(r, p, 0.5); p = fma(r, p, 1.); p = fma(r, p, 1.);
+  return __builtin_amdgcn_ldexp(p, (int)k);
+}
+__device__ __forceinline__ double exp_row(double x) { return exp_terms(x < -800. ? -800. : x > 800. ? 800. : x); }      // (e^+-800: infinite, 0)
+// sum over the lpr lanes of a row: inside 16 lanes by DPP (exchange in pairs, in fours, mirrored eights, mirrored sixteens), above by shuffles
+template <int CTRL> __device__ __forceinline__ double dpp_add(double x) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, 0xf, 0xf, false), hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CTRL, 0xf, 0xf, false);
+  return x + __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double row_sum(double x, int lpr) {
+  if (lpr > 1) x = dpp_add<0xb1>(x);       // quad_perm 1 0 3 2
+  if (lpr > 2) x = dpp_add<0x4e>(x);       // quad_perm 2 3 0 1
+  if (lpr > 4) x = dpp_add<0x141>(x);      // row_half_mirror
+  if (lpr > 8) x = dpp_add<0x140>(x);      // row_mirror
+  if (lpr > 16) x += __shfl_xor(x, 16, 64);
+  if (lpr > 32) x += __shfl_xor(x, 32, 64);
+  return x;
+}
+__device__ __forceinline__ double wave_sum(double x) { return row_sum(x, 64); }
+
+// valid rows of 4096 bytes a workgroup step, 16 a lane
 __global__ __launch_bounds__(256) void hoic_count_valid_kernel(const unsigned char* __restrict__ valid, long long rows, long long per_block, int* __restrict__ counts) {
+  typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(1)));
   __shared__ int red[4];
   const long long r0 = (long long)blockIdx.x * per_block, r1 = r0 + per_block < rows ? r0 + per_block : rows;
   int c = 0;
-  for (long long r = r0 + threadIdx.x; r < r1; r += 256) c += valid[r] != 0;
+  for (long long r = r0 + threadIdx.x * 16; r < r1; r += 4096) {
+    if (r + 16 <= r1) {
+      const u4 x = *(const u4*)(valid + r);
+#pragma unroll
+      for (int e = 0; e < 4; e++) c += __popc((((x[e] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x[e]) & 0x80808080u);       // bytes that are not 0
+    } else {
+      for (long long i = r; i < r1; i++) c += valid[i] != 0;
+    }
+  }
 #pragma unroll
   for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
@@ -1546,142 +1578,201 @@ __device__ __forceinline__ void policy_loss_scalars(const hoic_policy_loss_args&
   a.out[1] = (float)surr; a.out[2] = (float)kl; a.out[3] = (float)(clipped / d); a.out[4] = (float)n; a.out[5] = 0.f;
   *(double*)(a.out + 6) = n;
 }
-
-template <class TM, class TA> __global__ __launch_bounds__(PL_NT) void hoic_policy_loss_kernel(PolicyLossArgs k) {
+__device__ __forceinline__ void store_log_std_grad(const hoic_policy_loss_args& a, int j, double x) {
+  if (a.t_std == HOIC_F32) ((float*)a.d_log_std)[j] = (float)x;
+  else if (a.t_std == HOIC_F16) ((_Float16*)a.d_log_std)[j] = (_Float16)(float)x;
+  else ((__bf16*)a.d_log_std)[j] = (__bf16)(float)x;
+}
+// SHARED: one row of log-deviations (and of the reference's) for all rows: their terms are made once a lane.  VEC: dims is a multiple of 4,
+// a lane's four dimensions are one load (else four).  Rows outside the batch read row 0's place and are dropped at the end: short
+// straight code matters more here than their traffic, a launch of a few rows waits for its instructions first of all.
+template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __launch_bounds__(PL_NT) void hoic_policy_loss_kernel(PolicyLossArgs k) {
   const hoic_policy_loss_args& a = k.a;
   __shared__ double red[PL_NT * 4];
-  __shared__ double tail[3][PL_NT / 64];
+  __shared__ double tail[4][PL_NT / 64];
   __shared__ int wcount[PL_NT / 64];
   const int lpr = 1 << k.lpr_log2, sub = threadIdx.x & (lpr - 1), j = sub * 4, left = a.dims - j;
   const int rpb = PL_NT >> k.lpr_log2, rg = threadIdx.x >> k.lpr_log2;
-  const bool grad = a.d_mean != nullptr, kl_on = a.ref_mean != nullptr, shared_std = a.ld_std == 0, sum_ls = grad && a.d_log_std && shared_std;
-  double n = (double)a.rows;
-  if (grad && a.valid) {
-    if (a.count) {
-      n = *a.count;
-    } else {
-      int c = 0;
-      for (int i = threadIdx.x; i < k.ncounts; i += PL_NT) c += k.counts[i];
+  const bool full = a.dims == 4 * lpr;
+  int off[4];
 #pragma unroll
-      for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
-      if ((threadIdx.x & 63) == 0) wcount[threadIdx.x >> 6] = c;
-      __syncthreads();
-      n = 0.;
-      for (int w = 0; w < PL_NT / 64; w++) n += (double)wcount[w];
+  for (int e = 0; e < 4; e++) off[e] = e < left ? j + e : 0;
+  auto load = [&](const auto* x, long long at) {
+    f32x4 r;
+    if (VEC) {
+      r = __builtin_convertvector(*(const typename vec4<std::decay_t<decltype(*x)>>::type*)(x + at + off[0]), f32x4);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) r[e] = (float)x[at + off[e]];
     }
+    if (!full) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) r[e] = e < left ? r[e] : 0.f;
+    }
+    return r;
+  };
+  auto load_std = [&](const void* x, long long at) { return a.t_std == HOIC_F32 ? load((const float*)x, at) : load((const TM*)x, at); };
+  double scale = 0., klw = 0.;
+  if (GRAD) {
+    double n = (double)a.rows;
+    if (a.valid) {
+      if (a.count) {
+        n = *a.count;
+      } else {
+        int c = 0;
+        for (int i = threadIdx.x; i < k.ncounts; i += PL_NT) c += k.counts[i];
+#pragma unroll
+        for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
+        if ((threadIdx.x & 63) == 0) wcount[threadIdx.x >> 6] = c;
+        __syncthreads();
+        n = (double)(wcount[0] + wcount[1] + wcount[2] + wcount[3]);
+      }
+    }
+    scale = a.weight * (a.upstream ? (double)*a.upstream : 1.) / (n > 0. ? n : 1.);
+    klw = a.kl_coef * scale;
   }
-  const double scale = grad ? a.weight * (a.upstream ? (double)*a.upstream : 1.) / (n > 0. ? n : 1.) : 0.;
-  const double lo = 1. - a.clip_lo, hi = 1. + a.clip_hi, klw = a.kl_coef * scale;
-  double iv[4], lc[4], kc[4], ke[4];            // 1 / sigma^2, -s - log(2 pi) / 2, the KL's part without the means, e^{2 (s0 - s)}
+  const double lo = 1. - a.clip_lo, hi = 1. + a.clip_hi;
+  // 1 / sigma^2 and 1 - e^{2 (s0 - s)} per dimension; the sums over the lane's dimensions of -s - log(2 pi) / 2 and of the KL's part without the means
+  double iv[4], ke[4], lc, kc;
   auto std_terms = [&](f32x4 s, f32x4 s0) {
+    lc = 0.; kc = 0.;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const double sd = (double)s[e], s0d = (double)s0[e];
-      iv[e] = e < left ? exp(-2. * sd) : 0.;
-      lc[e] = e < left ? -sd - 0.91893853320467274178 : 0.;
-      ke[e] = kl_on && e < left ? exp(2. * (s0d - sd)) : 0.;
-      kc[e] = kl_on && e < left ? sd - s0d + 0.5 * ke[e] - 0.5 : 0.;
+      const double sd = (double)s[e];
+      iv[e] = exp_terms(-2. * sd);
+      lc -= e < left ? sd + 0.91893853320467274178 : 0.;
+      ke[e] = 0.;
+      if (KL) {
+        const double dd = (double)s0[e] - sd, x = exp_terms(2. * dd);
+        ke[e] = 1. - x;
+        kc += e < left ? 0.5 * x - dd - 0.5 : 0.;
+      }
     }
   };
-  const bool once = shared_std && (!kl_on || a.ld_ref_std == 0);
-  if (once) std_terms(load4_any(a.log_std, j, left, a.t_std), kl_on ? load4_any(a.ref_log_std, j, left, a.t_std) : f32x4{0.f, 0.f, 0.f, 0.f});
-  double dls[4] = {0., 0., 0., 0.}, acc_s = 0., acc_k = 0., acc_c = 0., acc_n = 0.;
+  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+  if (SHARED) std_terms(load_std(a.log_std, 0), KL ? load_std(a.ref_log_std, 0) : zero4);
+  double dls[4] = {0., 0., 0., 0.}, acc_s = 0., acc_k = 0.;
+  int acc_c = 0, acc_n = 0;
+  const bool sum_ls = GRAD && a.d_log_std && a.ld_std == 0, row_ls = GRAD && a.d_log_std && a.ld_std != 0;
   const long long nchunks = (a.rows + rpb - 1) / rpb;
   for (long long c = blockIdx.x; c < nchunks; c += gridDim.x) {
     const long long row = c * rpb + rg;
-    const bool in = row < a.rows, ok = in && (!a.valid || a.valid[row]);
-    const int l = ok ? left : 0;
-    f32x4 mu = load4((const TM*)a.mean + (ok ? row * a.ld_mean + j : 0), l), x = load4((const TA*)a.act + (ok ? row * a.ld_act + j : 0), l);
-    f32x4 mu0 = kl_on ? load4((const TM*)a.ref_mean + (ok ? row * a.ld_ref_mean + j : 0), l) : f32x4{0.f, 0.f, 0.f, 0.f};
-    if (!once) std_terms(load4_any(a.log_std, ok ? row * a.ld_std + j : 0, l, a.t_std),
-                         kl_on ? load4_any(a.ref_log_std, ok ? row * a.ld_ref_std + j : 0, l, a.t_std) : f32x4{0.f, 0.f, 0.f, 0.f});
-    const double A = ok ? (double)a.adv[row] : 0., l0 = ok && a.fixed ? (double)a.fixed[row] : 0.;
+    const bool in = row < a.rows;
+    const long long at = in ? row : 0;
+    const bool ok = in && (!a.valid || a.valid[at]);
+    const f32x4 mu = load((const TM*)a.mean, at * a.ld_mean), x = a.t_act == HOIC_F32 ? load((const float*)a.act, at * a.ld_act) : load((const TM*)a.act, at * a.ld_act);
+    const f32x4 mu0 = KL ? load((const TM*)a.ref_mean, at * a.ld_ref_mean) : zero4;
+    if (!SHARED) std_terms(load_std(a.log_std, at * a.ld_std), KL ? load_std(a.ref_log_std, at * a.ld_ref_std) : zero4);
+    const double A = (double)a.adv[at], l0 = a.fixed ? (double)a.fixed[at] : 0.;
     double d[4], dk[4], lp = 0., kl = 0.;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       d[e] = (double)x[e] - (double)mu[e];
-      dk[e] = kl_on ? (double)mu[e] - (double)mu0[e] : 0.;
-      lp += lc[e] - 0.5 * d[e] * d[e] * iv[e];
-      kl += kc[e] + 0.5 * dk[e] * dk[e] * iv[e];
+      lp = fma(d[e] * d[e], iv[e], lp);
+      dk[e] = 0.;
+      if (KL) { dk[e] = (double)mu[e] - (double)mu0[e]; kl = fma(dk[e] * dk[e], iv[e], kl); }
     }
-    for (int o = lpr >> 1; o; o >>= 1) { lp += __shfl_xor(lp, o, 64); kl += __shfl_xor(kl, o, 64); }
-    const double r = a.fixed ? exp(lp - l0) : 1.;
+    lp = row_sum(fma(-0.5, lp, lc), lpr);
+    if (KL) kl = row_sum(fma(0.5, kl, kc), lpr);
+    const double r = a.fixed ? exp_row(lp - l0) : 1.;
     const double s1 = r * A, s2 = (r < lo ? lo : r > hi ? hi : r) * A;
     const bool pass = s1 < s2 || (r >= lo && r <= hi) || r != r;      // (a NaN is passed on)
     if (ok && sub == 0) {
       acc_s -= s1 < s2 || s1 != s1 ? s1 : s2;
       acc_k += kl;
-      acc_c += pass ? 0. : 1.;
-      acc_n += 1.;
+      acc_c += pass ? 0 : 1;
+      acc_n += 1;
     }
     if (a.log_probs && in && sub == 0) a.log_probs[row] = ok ? (float)lp : 0.f;
-    if (grad && in) {
-      const double dlp = ok && pass ? -scale * s1 : 0.;
+    if (GRAD) {
+      const double dlp = pass ? -scale * s1 : 0.;
       f32x4 g, gs;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const double gm = ok ? (dlp * d[e] + klw * dk[e]) * iv[e] : 0.;
-        const double gl = ok ? dlp * (d[e] * d[e] * iv[e] - 1.) + (kl_on ? klw * (1. - ke[e] - dk[e] * dk[e] * iv[e]) : 0.) : 0.;
-        g[e] = (float)gm; gs[e] = (float)gl;
-        if (sum_ls) dls[e] += gl;
+        const double q = d[e] * iv[e];
+        double gm = dlp * q, gl = dlp * fma(d[e], q, -1.);
+        if (KL) {
+          const double qk = dk[e] * iv[e];
+          gm = fma(klw, qk, gm); gl = fma(klw, fma(-dk[e], qk, ke[e]), gl);
+        }
+        g[e] = ok ? (float)gm : 0.f; gs[e] = ok ? (float)gl : 0.f;
+        dls[e] += ok ? gl : 0.;
       }
-      store4((TM*)a.d_mean + row * a.ld_dmean + j, left, g);
-      if (a.d_log_std && !shared_std) store4_any(a.d_log_std, row * a.dims + j, left, a.t_std, gs);
+      if (in) {
+        auto store = [&](auto* out, f32x4 v) {
+          typedef std::decay_t<decltype(*out)> T;
+          if (VEC) { if (left > 0) *(typename vec4<T>::type*)(out + j) = __builtin_convertvector(v, typename vec4<T>::type); }
+          else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) if (e < left) out[j + e] = (T)v[e];
+          }
+        };
+        store((TM*)a.d_mean + row * a.ld_dmean, g);
+        if (row_ls) { if (a.t_std == HOIC_F32) store((float*)a.d_log_std + row * a.dims, gs); else store((TM*)a.d_log_std + row * a.dims, gs); }
+      }
     }
   }
-  // the block's sums in fixed order: the gradient of a shared log-deviation over the block's row groups, then the scalars
-  const int ps = a.dims + 4;
-  double* part = k.part + (long long)blockIdx.x * ps;
+  // the workgroup's sums in fixed order: the gradient of a shared log-deviation over the row groups, then the scalars; a lone workgroup's are final
+  const bool lone = gridDim.x == 1;
   if (sum_ls) {
 #pragma unroll
     for (int e = 0; e < 4; e++) red[rg * (lpr * 4) + j + e] = dls[e];
   }
+  acc_s = wave_sum(acc_s); if (KL) acc_k = wave_sum(acc_k);
 #pragma unroll
-  for (int o = 32; o; o >>= 1) { acc_s += __shfl_xor(acc_s, o, 64); acc_k += __shfl_xor(acc_k, o, 64); acc_c += __shfl_xor(acc_c, o, 64); acc_n += __shfl_xor(acc_n, o, 64); }
-  if ((threadIdx.x & 63) == 0) { const int w = threadIdx.x >> 6; tail[0][w] = acc_s; tail[1][w] = acc_k; tail[2][w] = acc_c; wcount[w] = (int)acc_n; }
+  for (int o = 32; o; o >>= 1) { acc_c += __shfl_xor(acc_c, o, 64); acc_n += __shfl_xor(acc_n, o, 64); }
+  if ((threadIdx.x & 63) == 0) { const int w = threadIdx.x >> 6; tail[0][w] = acc_s; tail[1][w] = acc_k; tail[2][w] = (double)acc_c; tail[3][w] = (double)acc_n; }
   __syncthreads();
   if (sum_ls && threadIdx.x < a.dims) {
     double t = 0.;
     for (int q = 0; q < rpb; q++) t += red[q * (lpr * 4) + threadIdx.x];
-    part[threadIdx.x] = t;
+    if (lone) store_log_std_grad(a, threadIdx.x, t);
+    else k.part[(long long)threadIdx.x * PL_BLOCKS + blockIdx.x] = t;
   }
-  if (threadIdx.x == 0 && !a.count) {
-    double t[4] = {0., 0., 0., 0.};
-    for (int w = 0; w < PL_NT / 64; w++) { t[0] += tail[0][w]; t[1] += tail[1][w]; t[2] += tail[2][w]; t[3] += (double)wcount[w]; }
-    for (int q = 0; q < 4; q++) part[a.dims + q] = t[q];
+  if (a.count || threadIdx.x >= 4) return;
+  const double t = (tail[threadIdx.x][0] + tail[threadIdx.x][1]) + (tail[threadIdx.x][2] + tail[threadIdx.x][3]);
+  if (!lone) {
+    k.part[(long long)(a.dims + threadIdx.x) * PL_BLOCKS + blockIdx.x] = t;
+  } else {
+    const double kl = __shfl(t, 1, 64), cl = __shfl(t, 2, 64), n = __shfl(t, 3, 64);
+    if (threadIdx.x == 0) policy_loss_scalars(a, t, kl, cl, n);
   }
 }
 
-// sums of the blocks' parts: workgroup 0 the scalars, the others eight dimensions each (32 lanes a column, fixed order)
-__global__ __launch_bounds__(256) void hoic_policy_loss_finish_kernel(PolicyLossArgs k, int nb) {
+// sums of the workgroups' parts, a column a wavefront: workgroup 0 the scalars, the others four dimensions each
+__global__ __launch_bounds__(256) void hoic_policy_loss_finish_kernel(PolicyLossArgs k) {
   const hoic_policy_loss_args& a = k.a;
-  const int ps = a.dims + 4, col = threadIdx.x & 7, q = threadIdx.x >> 3;
-  const int j = blockIdx.x == 0 ? (col < 4 ? a.dims + col : -1) : ((int)blockIdx.x - 1) * 8 + col;
-  const bool on = blockIdx.x == 0 ? col < 4 && !a.count : j < a.dims;       // (with a.count the forward call wrote the scalars)
-  __shared__ double red[32][9];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, j = blockIdx.x == 0 ? a.dims + w : ((int)blockIdx.x - 1) * 4 + w;
+  const bool on = blockIdx.x == 0 ? !a.count : j < a.dims;            // (with a.count the forward call wrote the scalars)
+  __shared__ double red[4];
+  const double* col = k.part + (long long)j * PL_BLOCKS;
+  double x[PL_BLOCKS / 64];
+#pragma unroll
+  for (int i = 0; i < PL_BLOCKS / 64; i++) x[i] = on && i * 64 + lane < k.nb ? col[i * 64 + lane] : 0.;
   double t = 0.;
-  if (on) for (int b = q; b < nb; b += 32) t += k.part[(long long)b * ps + j];
-  red[q][col] = t;
-  __syncthreads();
-  if (threadIdx.x < 8) {
-    double s = 0.;
-    for (int i = 0; i < 32; i++) s += red[i][threadIdx.x];
-    red[0][threadIdx.x] = s;
-    if (blockIdx.x > 0 && on) {
-      if (a.t_std == HOIC_F32) ((float*)a.d_log_std)[j] = (float)s;
-      else if (a.t_std == HOIC_F16) ((_Float16*)a.d_log_std)[j] = (_Float16)(float)s;
-      else ((__bf16*)a.d_log_std)[j] = (__bf16)(float)s;
-    }
+#pragma unroll
+  for (int i = 0; i < PL_BLOCKS / 64; i++) t += x[i];
+  t = wave_sum(t);
+  if (lane == 0) {
+    if (blockIdx.x > 0 && on) store_log_std_grad(a, j, t);
+    red[w] = t;
   }
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0 && !a.count) policy_loss_scalars(a, red[0][0], red[0][1], red[0][2], red[0][3]);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && !a.count) policy_loss_scalars(a, red[0], red[1], red[2], red[3]);
 }
 
-#define PL_BLOCKS 512
-#define PL_COUNTS 256
 extern "C" int64_t hoic_policy_loss_scratch_bytes(int32_t dims) { return dims <= 0 ? 0 : (int64_t)PL_BLOCKS * (dims + 4) * 8 + PL_COUNTS * 4; }
-template <class TM, class TA> static void launch_policy_loss(const PolicyLossArgs& k, int nb, hipStream_t st) {
-  hipLaunchKernelGGL((hoic_policy_loss_kernel<TM, TA>), dim3(nb), dim3(PL_NT), 0, st, k);
+template <class TM, bool SHARED, bool KL, bool GRAD> static void launch_policy_loss(const PolicyLossArgs& k, hipStream_t st) {
+  if (k.a.dims % 4 == 0) hipLaunchKernelGGL((hoic_policy_loss_kernel<TM, SHARED, KL, GRAD, true>), dim3(k.nb), dim3(PL_NT), 0, st, k);
+  else hipLaunchKernelGGL((hoic_policy_loss_kernel<TM, SHARED, KL, GRAD, false>), dim3(k.nb), dim3(PL_NT), 0, st, k);
+}
+template <class TM, bool SHARED, bool KL> static void launch_policy_loss(const PolicyLossArgs& k, hipStream_t st) {
+  if (k.a.d_mean) launch_policy_loss<TM, SHARED, KL, true>(k, st); else launch_policy_loss<TM, SHARED, KL, false>(k, st);
+}
+template <class TM> static void launch_policy_loss(const PolicyLossArgs& k, hipStream_t st) {
+  const bool kl = k.a.ref_mean != nullptr, shared = k.a.ld_std == 0 && (!kl || k.a.ld_ref_std == 0);
+  if (shared) { if (kl) launch_policy_loss<TM, true, true>(k, st); else launch_policy_loss<TM, true, false>(k, st); }
+  else { if (kl) launch_policy_loss<TM, false, true>(k, st); else launch_policy_loss<TM, false, false>(k, st); }
 }
 extern "C" int32_t hoic_policy_loss(const hoic_policy_loss_args* p, void* stream) {
   if (!p) { hoic_set_error("hoic_policy_loss: no arguments"); return HOIC_ERR_ARG; }
@@ -1709,15 +1800,14 @@ extern "C" int32_t hoic_policy_loss(const hoic_policy_loss_args* p, void* stream
     k.ncounts = (int)((a.rows + per - 1) / per);
     hipLaunchKernelGGL(hoic_count_valid_kernel, dim3(k.ncounts), dim3(256), 0, st, a.valid, (long long)a.rows, per, counts);
   }
-  const int rpb = PL_NT >> k.lpr_log2;
-  const int nb = (int)std::max<long long>(1, std::min<long long>(PL_BLOCKS, (a.rows + rpb - 1) / rpb));
-  if (a.t_mean == HOIC_F32) launch_policy_loss<float, float>(k, nb, st);
-  else if (a.t_mean == HOIC_F16) { if (a.t_act == HOIC_F32) launch_policy_loss<_Float16, float>(k, nb, st); else launch_policy_loss<_Float16, _Float16>(k, nb, st); }
-  else { if (a.t_act == HOIC_F32) launch_policy_loss<__bf16, float>(k, nb, st); else launch_policy_loss<__bf16, __bf16>(k, nb, st); }
+  // workgroups of equally many steps (of PL_NT / lpr rows), at most PL_BLOCKS of them
+  const long long steps = std::max<long long>(1, (a.rows + (PL_NT >> k.lpr_log2) - 1) / (PL_NT >> k.lpr_log2)), each = (steps + PL_BLOCKS - 1) / PL_BLOCKS;
+  k.nb = (int)((steps + each - 1) / each);
+  if (a.t_mean == HOIC_F32) launch_policy_loss<float>(k, st);
+  else if (a.t_mean == HOIC_F16) launch_policy_loss<_Float16>(k, st);
+  else launch_policy_loss<__bf16>(k, st);
   const bool sum_ls = a.d_log_std && a.ld_std == 0;
-  if (!a.count || sum_ls) {
-    hipLaunchKernelGGL(hoic_policy_loss_finish_kernel, dim3(sum_ls ? 1 + (a.dims + 7) / 8 : 1), dim3(256), 0, st, k, nb);
-  }
+  if (k.nb > 1 && (!a.count || sum_ls)) hipLaunchKernelGGL(hoic_policy_loss_finish_kernel, dim3(sum_ls ? 1 + (a.dims + 3) / 4 : 1), dim3(256), 0, st, k);
   MCHK(hipGetLastError());
   return HOIC_OK;
 }
