@@ -1586,9 +1586,9 @@ __device__ __forceinline__ void store_log_std_grad(const hoic_policy_loss_args& 
 // SHARED: one row of log-deviations (and of the reference's) for all rows: their terms are made once a lane.  VEC: dims is a multiple of 4,
 // a lane's four dimensions are one load (else four).  Rows outside the batch read row 0's place and are dropped at the end: short
 // straight code matters more here than their traffic, a launch of a few rows waits for its instructions first of all.
-template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __launch_bounds__(PL_NT) void hoic_policy_loss_kernel(PolicyLossArgs k) {
+template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __launch_bounds__(PL_NT, 4) void hoic_policy_loss_kernel(PolicyLossArgs k) {
   const hoic_policy_loss_args& a = k.a;
-  __shared__ double red[PL_NT * 4];
+  __shared__ double red[PL_NT * 4];          // the dimensions' terms first, the row groups' sums in the end
   __shared__ double tail[4][PL_NT / 64];
   __shared__ int wcount[PL_NT / 64];
   const int lpr = 1 << k.lpr_log2, sub = threadIdx.x & (lpr - 1), j = sub * 4, left = a.dims - j;
@@ -1632,27 +1632,34 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
     klw = a.kl_coef * scale;
   }
   const double lo = 1. - a.clip_lo, hi = 1. + a.clip_hi;
-  // 1 / sigma^2 and 1 - e^{2 (s0 - s)} per dimension; the sums over the lane's dimensions of -s - log(2 pi) / 2 and of the KL's part without the means
-  double iv[4], ke[4], lc, kc;
-  auto std_terms = [&](f32x4 s, f32x4 s0) {
-    lc = 0.; kc = 0.;
+  // per dimension 1 / sigma^2, 1 - e^{2 (s0 - s)}, -s - log(2 pi) / 2 and the KL's part without the means; of the last two the sum over the lane's
+  double iv[4], ke[4], lc = 0., kc = 0.;
+  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+  auto dim_terms = [&](float s, float s0, double& v, double& e, double& l, double& kp) {
+    const double sd = (double)s;
+    v = exp_terms(-2. * sd);
+    l = -sd - 0.91893853320467274178;
+    e = kp = 0.;
+    if (KL) { const double dd = (double)s0 - sd, x = exp_terms(2. * dd); e = 1. - x; kp = 0.5 * x - dd - 0.5; }
+  };
+  if (SHARED) {                              // once a dimension in the workgroup, handed round in LDS
+    double* tab = red;
+    if (threadIdx.x < a.dims) {
+      auto one = [&](const void* x) { return a.t_std == HOIC_F32 ? ((const float*)x)[threadIdx.x] : (float)((const TM*)x)[threadIdx.x]; };
+      dim_terms(one(a.log_std), KL ? one(a.ref_log_std) : 0.f, tab[threadIdx.x], tab[PL_NT + threadIdx.x], tab[2 * PL_NT + threadIdx.x], tab[3 * PL_NT + threadIdx.x]);
+    }
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const double sd = (double)s[e];
-      iv[e] = exp_terms(-2. * sd);
-      lc -= e < left ? sd + 0.91893853320467274178 : 0.;
-      ke[e] = 0.;
-      if (KL) {
-        const double dd = (double)s0[e] - sd, x = exp_terms(2. * dd);
-        ke[e] = 1. - x;
-        kc += e < left ? 0.5 * x - dd - 0.5 : 0.;
-      }
+      const bool on = e < left;
+      iv[e] = on ? tab[off[e]] : 0.; ke[e] = KL && on ? tab[PL_NT + off[e]] : 0.;
+      lc += on ? tab[2 * PL_NT + off[e]] : 0.; kc += KL && on ? tab[3 * PL_NT + off[e]] : 0.;
     }
-  };
-  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
-  if (SHARED) std_terms(load_std(a.log_std, 0), KL ? load_std(a.ref_log_std, 0) : zero4);
-  double dls[4] = {0., 0., 0., 0.}, acc_s = 0., acc_k = 0.;
-  int acc_c = 0, acc_n = 0;
+    __syncthreads();
+  }
+  // a shared log-deviation's gradient: sum (dlp d^2 / sigma^2 - klw dk^2 / sigma^2) - sum dlp + klw (1 - e^{2 (s0 - s)}) rows
+  double dls[4] = {0., 0., 0., 0.}, acc_l = 0., acc_s = 0., acc_k = 0.;
+  int rows_in = 0, acc_c = 0, acc_n = 0;      // (acc_c, acc_n: of the wavefront)
   const bool sum_ls = GRAD && a.d_log_std && a.ld_std == 0, row_ls = GRAD && a.d_log_std && a.ld_std != 0;
   const long long nchunks = (a.rows + rpb - 1) / rpb;
   for (long long c = blockIdx.x; c < nchunks; c += gridDim.x) {
@@ -1660,44 +1667,60 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
     const bool in = row < a.rows;
     const long long at = in ? row : 0;
     const bool ok = in && (!a.valid || a.valid[at]);
-    const f32x4 mu = load((const TM*)a.mean, at * a.ld_mean), x = a.t_act == HOIC_F32 ? load((const float*)a.act, at * a.ld_act) : load((const TM*)a.act, at * a.ld_act);
-    const f32x4 mu0 = KL ? load((const TM*)a.ref_mean, at * a.ld_ref_mean) : zero4;
-    if (!SHARED) std_terms(load_std(a.log_std, at * a.ld_std), KL ? load_std(a.ref_log_std, at * a.ld_ref_std) : zero4);
-    const double A = (double)a.adv[at], l0 = a.fixed ? (double)a.fixed[at] : 0.;
-    double d[4], dk[4], lp = 0., kl = 0.;
+    f32x4 mu = load((const TM*)a.mean, at * a.ld_mean), x = a.t_act == HOIC_F32 ? load((const float*)a.act, at * a.ld_act) : load((const TM*)a.act, at * a.ld_act);
+    f32x4 mu0 = KL ? load((const TM*)a.ref_mean, at * a.ld_ref_mean) : zero4;
+    if (!SHARED) {
+      const f32x4 s = load_std(a.log_std, at * a.ld_std), s0 = KL ? load_std(a.ref_log_std, at * a.ld_ref_std) : zero4;
+      lc = kc = 0.;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        double l, kp;
+        dim_terms(s[e], s0[e], iv[e], ke[e], l, kp);
+        lc += e < left ? l : 0.; kc += e < left ? kp : 0.;
+        if (!KL) ke[e] = 0.;
+      }
+    }
+    double A = (double)a.adv[at], l0 = a.fixed ? (double)a.fixed[at] : 0.;
+    if (!ok) { mu = x = mu0 = zero4; A = l0 = 0.; }
+    double d[4], dk[4], q[4], qk[4], lp = 0., kl = 0.;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       d[e] = (double)x[e] - (double)mu[e];
-      lp = fma(d[e] * d[e], iv[e], lp);
-      dk[e] = 0.;
-      if (KL) { dk[e] = (double)mu[e] - (double)mu0[e]; kl = fma(dk[e] * dk[e], iv[e], kl); }
+      q[e] = d[e] * iv[e];
+      lp = fma(d[e], q[e], lp);
+      if (KL) { dk[e] = (double)mu[e] - (double)mu0[e]; qk[e] = dk[e] * iv[e]; kl = fma(dk[e], qk[e], kl); }
     }
     lp = row_sum(fma(-0.5, lp, lc), lpr);
     if (KL) kl = row_sum(fma(0.5, kl, kc), lpr);
     const double r = a.fixed ? exp_row(lp - l0) : 1.;
     const double s1 = r * A, s2 = (r < lo ? lo : r > hi ? hi : r) * A;
     const bool pass = s1 < s2 || (r >= lo && r <= hi) || r != r;      // (a NaN is passed on)
-    if (ok && sub == 0) {
+    const bool first = ok && sub == 0;
+    if (first) {
       acc_s -= s1 < s2 || s1 != s1 ? s1 : s2;
-      acc_k += kl;
-      acc_c += pass ? 0 : 1;
-      acc_n += 1;
+      if (KL) acc_k += kl;
     }
+    acc_c += __popcll(__ballot(first && !pass)); acc_n += __popcll(__ballot(first));
     if (a.log_probs && in && sub == 0) a.log_probs[row] = ok ? (float)lp : 0.f;
     if (GRAD) {
-      const double dlp = pass ? -scale * s1 : 0.;
+      const double dlp = ok && pass ? -scale * s1 : 0.;
+      const double kw = ok ? klw : 0.;
       f32x4 g, gs;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const double q = d[e] * iv[e];
-        double gm = dlp * q, gl = dlp * fma(d[e], q, -1.);
-        if (KL) {
-          const double qk = dk[e] * iv[e];
-          gm = fma(klw, qk, gm); gl = fma(klw, fma(-dk[e], qk, ke[e]), gl);
+        const double gm = dlp * q[e], gk = KL ? kw * qk[e] : 0.;
+        if (SHARED) {
+          dls[e] = fma(d[e], gm, dls[e]);
+          if (KL) dls[e] = fma(-dk[e], gk, dls[e]);
+        } else {
+          double gl = fma(d[e], gm, -dlp);
+          if (KL) gl += fma(kw, ke[e], -dk[e] * gk);
+          gs[e] = (float)gl;
+          dls[e] += gl;
         }
-        g[e] = ok ? (float)gm : 0.f; gs[e] = ok ? (float)gl : 0.f;
-        dls[e] += ok ? gl : 0.;
+        g[e] = (float)(gm + gk);
       }
+      if (SHARED) { acc_l += dlp; rows_in += ok ? 1 : 0; }
       if (in) {
         auto store = [&](auto* out, f32x4 v) {
           typedef std::decay_t<decltype(*out)> T;
@@ -1716,11 +1739,9 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
   const bool lone = gridDim.x == 1;
   if (sum_ls) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) red[rg * (lpr * 4) + j + e] = dls[e];
+    for (int e = 0; e < 4; e++) red[rg * (lpr * 4) + j + e] = SHARED ? dls[e] - acc_l + klw * (ke[e] * rows_in) : dls[e];
   }
   acc_s = wave_sum(acc_s); if (KL) acc_k = wave_sum(acc_k);
-#pragma unroll
-  for (int o = 32; o; o >>= 1) { acc_c += __shfl_xor(acc_c, o, 64); acc_n += __shfl_xor(acc_n, o, 64); }
   if ((threadIdx.x & 63) == 0) { const int w = threadIdx.x >> 6; tail[0][w] = acc_s; tail[1][w] = acc_k; tail[2][w] = (double)acc_c; tail[3][w] = (double)acc_n; }
   __syncthreads();
   if (sum_ls && threadIdx.x < a.dims) {
