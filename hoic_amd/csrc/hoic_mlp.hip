@@ -1574,9 +1574,9 @@ __global__ __launch_bounds__(256) void hoic_count_valid_kernel(const unsigned ch
 __device__ __forceinline__ void policy_loss_scalars(const hoic_policy_loss_args& a, double surr, double kl, double clipped, double n) {
   const double d = n > 0. ? n : 1.;
   surr /= d; kl /= d;
-  a.out[0] = (float)(surr + a.kl_coef * kl);
-  a.out[1] = (float)surr; a.out[2] = (float)kl; a.out[3] = (float)(clipped / d); a.out[4] = (float)n; a.out[5] = 0.f;
-  *(double*)(a.out + 6) = n;
+  *a.loss = (float)(surr + a.kl_coef * kl);
+  a.info[0] = (float)surr; a.info[1] = (float)kl; a.info[2] = (float)(clipped / d); a.info[3] = (float)n;
+  if (a.n_out) *a.n_out = n;
 }
 __device__ __forceinline__ void store_log_std_grad(const hoic_policy_loss_args& a, int j, double x) {
   if (a.t_std == HOIC_F32) ((float*)a.d_log_std)[j] = (float)x;
@@ -1803,7 +1803,7 @@ extern "C" int32_t hoic_policy_loss(const hoic_policy_loss_args* p, void* stream
       || (a.t_std != a.t_mean && a.t_std != HOIC_F32)) {
     hoic_set_error("hoic_policy_loss: 1 .. 256 dimensions; actions and log_std in float32 or in the mean's type"); return HOIC_ERR_ARG;
   }
-  if (!a.scratch || (!a.count && !a.out) || !a.log_std || (a.rows > 0 && (!a.mean || !a.act || !a.adv)) || (!a.ref_mean) != (!a.ref_log_std) || (a.d_log_std && !a.d_mean)
+  if (!a.scratch || (!a.count && (!a.loss || !a.info)) || !a.log_std || (a.rows > 0 && (!a.mean || !a.act || !a.adv)) || (!a.ref_mean) != (!a.ref_log_std) || (a.d_log_std && !a.d_mean)
       || (a.count && !a.d_mean)) {
     hoic_set_error("hoic_policy_loss: missing tensors"); return HOIC_ERR_ARG;
   }

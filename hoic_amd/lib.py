@@ -40,7 +40,7 @@ class RewardParams(C.Structure):
 
 
 # hoic_policy_loss_args and hoic_adamw_args (include/hoic.h) as struct formats: one pack() is the whole argument block
-POLICY_LOSS_ARGS = struct.Struct("@q4i5P6q5P4d5P")
+POLICY_LOSS_ARGS = struct.Struct("@q4i5P6q5P4d7P")
 ADAMW_ARGS = struct.Struct("@2i5d4Pdq2I")
 
 
@@ -174,6 +174,33 @@ def cu_masked_stream(device, first_cu, n_cus):
     if rc != 0 or not h.value:
         raise HoicError(f"hipExtStreamCreateWithCUMask failed ({rc})")
     return torch.cuda.ExternalStream(h.value, device=dev)
+
+
+class Launch:
+    """``with Launch(device) as stream``: the device current (switched only when another one is), its current stream's handle.  Every
+    entry point launches on the stream that it is given and carries no device ordinal."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, dev):
+        self.index = dev.index
+
+    def __enter__(self):
+        global _tc
+        if _tc is None:
+            import torch
+            _tc = torch._C
+        self.before = _tc._cuda_getDevice()
+        if self.before != self.index:
+            _tc._cuda_setDevice(self.index)
+        return _tc._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            _tc._cuda_setDevice(self.before)
+
+
+_tc = None
 
 
 def build_id() -> str:

@@ -44,26 +44,6 @@ def _check(t, what):
         raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
 
 
-class _Launch:
-    """``with _Launch(device) as stream``: the device current (switched only when another one is), its current stream's handle.  Every
-    entry point launches on the stream that it is given and carries no device ordinal."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, dev):
-        self.index = dev.index
-
-    def __enter__(self):
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.index:
-            torch._C._cuda_setDevice(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch._C._cuda_setDevice(self.before)
-
-
 def _norm_list(grads):
     """The arguments of the hoic_grad_norm family for CUDA tensors of one device: ((pointers, sizes, types, count), parts, tensors held)"""
     dev, n = grads[0].device, len(grads)
@@ -98,7 +78,7 @@ def grad_norm(tensors):
         if parts == 0:
             return norm.zero_()
         buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
-        with _Launch(dev) as st:
+        with lib.Launch(dev) as st:
             lib._chk(lib.load().hoic_grad_norm(*args, buf.data_ptr(), norm.data_ptr(), st), "hoic_grad_norm")
     return norm
 
@@ -122,7 +102,7 @@ def clip_grad_norm_(parameters, max_norm):
     if parts == 0:
         return norm.zero_()
     buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
-    with _Launch(dev) as st:
+    with lib.Launch(dev) as st:
         lib._chk(lib.load().hoic_clip_grads(*args, b, buf.data_ptr(), norm.data_ptr(), st), "hoic_clip_grads")
     torch.autograd.graph.increment_version(grads)
     return norm
@@ -271,7 +251,7 @@ class AdamW(torch.optim.Optimizer):
             if parts:
                 buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
                 buf_ptr, norm_ptr = buf.data_ptr(), norm.data_ptr()
-                with _Launch(dev) as st:
+                with lib.Launch(dev) as st:
                     lib._chk(L.hoic_grad_norm_partial(*args, buf_ptr, st), "hoic_grad_norm_partial")
             else:
                 norm.zero_()
@@ -295,7 +275,7 @@ class AdamW(torch.optim.Optimizer):
             consts = torch.empty(4 * len(todo), dtype=torch.float32, device=dev) if capturable else None
             a = lib.ADAMW_ARGS.pack(TYPES[dtype], bits, lr, b1, b2, group["eps"], group["weight_decay"], lr_ptr,
                                     0 if consts is None else consts.data_ptr(), buf_ptr, norm_ptr, bound or 0.0, parts, group["seed"], 0)
-            with _Launch(dev) as st:
+            with lib.Launch(dev) as st:
                 lib._chk(L.hoic_adamw((C.c_int64 * len(flat))(*flat), len(todo), a, st), "hoic_adamw")
         torch.autograd.graph.increment_version(params)
         return loss
@@ -319,7 +299,7 @@ class AdamW(torch.optim.Optimizer):
                 ms.append(m)
                 vs.append(v)
         for dev, flat in work.items():
-            with _Launch(dev) as st:
+            with lib.Launch(dev) as st:
                 lib._chk(lib.load().hoic_adamw_values((C.c_int64 * len(flat))(*flat), len(flat) // 10, st), "hoic_adamw_values")
         return ms, vs
 

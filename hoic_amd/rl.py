@@ -15,6 +15,8 @@ import numpy as np
 import torch
 import torch.nn as nn
 
+from . import lib
+
 
 class MLP(nn.Module):
     def __init__(self, input_dim, hidden_dims=(128, 128), activation="tanh"):
@@ -125,7 +127,6 @@ def estimate_advantages(rewards, masks, values, gamma, tau, next_values=None, di
             prev_v = values[t]
         returns = values + adv
     if valid is None and dist_group is None and adv.is_cuda and adv.dtype == torch.float32 and adv.is_contiguous() and adv.numel() >= 2:
-        from . import lib
         L = lib.load()
         if hasattr(L, "hoic_normalize_advantages"):      # two launches (float64 sums in a fixed order) instead of ~15 tensor kernels
             import ctypes as C
@@ -151,7 +152,6 @@ def estimate_advantages(rewards, masks, values, gamma, tau, next_values=None, di
 
 
 def _gae_device(rewards, masks, values, gamma, tau, next_values):
-    from . import lib
     import ctypes as C
     L = lib.load()
     f = lambda x: x.to(torch.float32).contiguous()
@@ -196,36 +196,43 @@ class PolicyLossGrad(NamedTuple):
 _LOSS_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}         # enum hoic_type
 
 
-def _loss_rows(t, name, M, N, dev, types, shared=False):
+def _loss_rows(t, name, size, at, types, shared=False):
     """[M, N] (``shared``: or one row for all) of the right type and place, with unit stride along the dimensions"""
+    if t.dtype in types and t.get_device() == at and t.is_contiguous() and (t.shape == size or (shared and t.shape == (1, size[1]))):
+        return t
+    M, N = size
     if shared and t.dim() == 1:
         t = t[None]
     if t.dim() != 2 or t.shape[1] != N or (t.shape[0] != M and not (shared and t.shape[0] == 1)):
         raise ValueError(f"{name}: {tuple(t.shape)} for means of {(M, N)}")
-    if t.dtype not in types or t.device != dev:
-        raise ValueError(f"{name}: {t.dtype} on {t.device}; wanted {' or '.join(str(x) for x in types)} on {dev}")
-    if t.is_contiguous():
-        return t
+    if t.dtype not in types or t.get_device() != at:
+        raise ValueError(f"{name}: {t.dtype} on {t.device}; wanted {' or '.join(str(x) for x in types)} where the means are")
     if shared and t.shape[0] > 1 and t.stride(0) == 0:
         return t.contiguous()                      # a row expanded over the batch: its gradient has a value per row
     return t if t.stride(1) == 1 or N == 1 else t.contiguous()
 
 
-def _loss_flat(t, name, M, dev, types):
-    if t.numel() != M or t.dtype not in types or t.device != dev:
-        raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device} for {M} rows on {dev}")
+def _loss_flat(t, name, M, at, types):
+    if t.numel() != M or t.dtype not in types or t.get_device() != at:
+        raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device} for {M} rows")
     return t if t.is_contiguous() else t.reshape(-1).contiguous()
+
+
+_TYPES_OF = {torch.float32: ((torch.float32,), (torch.float32,), (torch.float32,)), torch.float64: ((torch.float64,), (torch.float64,), (torch.float64,)),
+             torch.float16: ((torch.float16,), (torch.float16, torch.float32), (torch.float32,)),
+             torch.bfloat16: ((torch.bfloat16,), (torch.bfloat16, torch.float32), (torch.float32,))}       # a mean's own, actions' and log_std's, vectors'
+_FLAGS = (torch.bool, torch.uint8)
 
 
 def _loss_inputs(mean, log_std, actions, advantages, fixed, clip_epsilon, ref_mean, ref_log_std, kl_coef, valid):
     """Checks of the policy loss's arguments; row tensors come back with unit stride along the dimensions, vectors contiguous."""
-    if mean.dim() != 2 or mean.shape[1] < 1:
-        raise ValueError(f"mean must be [rows, dimensions], not {tuple(mean.shape)}")
-    M, N = mean.shape
-    dev, dtype = mean.device, mean.dtype
-    if not dtype.is_floating_point:
-        raise ValueError(f"mean: a floating type, not {dtype}")
-    f32 = torch.float32 if dtype is not torch.float64 else dtype
+    size, at = mean.shape, mean.get_device()
+    if len(size) != 2 or size[1] < 1:
+        raise ValueError(f"mean must be [rows, dimensions], not {tuple(size)}")
+    types = _TYPES_OF.get(mean.dtype)
+    if types is None:
+        raise ValueError(f"mean: a floating type, not {mean.dtype}")
+    own, wide, vector = types
     if (ref_mean is None) is not (ref_log_std is None):
         raise ValueError("the reference policy is ref_mean and ref_log_std together")
     if ref_mean is None and kl_coef:
@@ -233,39 +240,41 @@ def _loss_inputs(mean, log_std, actions, advantages, fixed, clip_epsilon, ref_me
     lo, hi = clip_epsilon if isinstance(clip_epsilon, (tuple, list)) else (clip_epsilon, clip_epsilon)
     if not (0.0 <= lo < math.inf and 0.0 <= hi < math.inf and math.isfinite(kl_coef)):
         raise ValueError(f"clip_epsilon {clip_epsilon} (>= 0) or kl_coef {kl_coef}")
-    wide = (dtype, f32)
-    mean, actions = _loss_rows(mean, "mean", M, N, dev, wide), _loss_rows(actions, "actions", M, N, dev, wide)
-    log_std = _loss_rows(log_std, "log_std", M, N, dev, wide, True)
-    advantages = _loss_flat(advantages, "advantages", M, dev, (f32,))
+    M = size[0]
+    mean, actions, log_std = _loss_rows(mean, "mean", size, at, own), _loss_rows(actions, "actions", size, at, wide), _loss_rows(log_std, "log_std", size, at, wide, True)
+    advantages = _loss_flat(advantages, "advantages", M, at, vector)
     if fixed is not None:
-        fixed = _loss_flat(fixed, "fixed_log_probs", M, dev, (f32,))
+        fixed = _loss_flat(fixed, "fixed_log_probs", M, at, vector)
     if ref_mean is not None:
-        ref_mean = _loss_rows(ref_mean, "ref_mean", M, N, dev, (dtype,))
-        ref_log_std = _loss_rows(ref_log_std, "ref_log_std", M, N, dev, (log_std.dtype,), True)
+        ref_mean = _loss_rows(ref_mean, "ref_mean", size, at, own)
+        ref_log_std = _loss_rows(ref_log_std, "ref_log_std", size, at, (log_std.dtype,), True)
     if valid is not None:
-        valid = _loss_flat(valid, "valid", M, dev, (torch.bool, torch.uint8))
+        valid = _loss_flat(valid, "valid", M, at, _FLAGS)
     return mean, log_std, actions, advantages, fixed, (float(lo), float(hi)), ref_mean, ref_log_std, valid
 
 
 def _policy_loss_launch(x, kl_coef, weight, grad, upstream=None, count=None):
-    """hoic_policy_loss on checked inputs -> (out [8] or None, d_mean, d_log_std [1 or M, N], log_probs)"""
-    from . import lib
-    from .optim import _Launch
+    """hoic_policy_loss on checked inputs -> (loss, info, n as float64 [1], d_mean, d_log_std [1 or M, N], log_probs).  ``count``: the n of
+    an earlier call, for the gradient alone (loss, info and n are then None)."""
     mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid = x
     M, N = mean.shape
     if N > 256:
         raise ValueError(f"the policy loss's kernel takes up to 256 action dimensions, not {N}")
-    L, dev, f32, empty = lib.load(), mean.device, torch.float32, torch.empty
-    out = empty(8, dtype=f32, device=dev) if count is None else None
-    d_mean = empty((M, N), dtype=mean.dtype, device=dev) if grad else None
-    d_log_std = empty(log_std.shape, dtype=log_std.dtype, device=dev) if grad else None
-    log_probs = empty((M, 1), dtype=f32, device=dev) if fixed is None and count is None else None
+    L, dev = lib.load(), mean.device
+    loss = info = n = log_probs = None
+    if count is None:
+        loss, info = advantages.new_empty(()), advantages.new_empty(4)
+        if not grad:
+            n = advantages.new_empty(1, dtype=torch.float64)
+        if fixed is None:
+            log_probs = advantages.new_empty((M, 1))
+    d_mean, d_log_std = (torch.empty_like(mean, memory_format=torch.contiguous_format), torch.empty_like(log_std, memory_format=torch.contiguous_format)) if grad else (None, None)
     if M == 0:
-        for t in (out, d_log_std):
+        for t in (loss, info, n, d_log_std):
             if t is not None:
                 t.zero_()
-        return out, d_mean, d_log_std, log_probs
-    scratch = empty(L.hoic_policy_loss_scratch_bytes(N), dtype=torch.uint8, device=dev)
+        return loss, info, n, d_mean, d_log_std, log_probs
+    scratch = torch.empty(L.hoic_policy_loss_scratch_bytes(N), dtype=torch.uint8, device=dev)
     ptr = lambda t: 0 if t is None else t.data_ptr()
     ld = lambda t: 0 if t is None or t.shape[0] == 1 else t.stride(0)          # (one row is a shared one: stride 0)
     args = lib.POLICY_LOSS_ARGS.pack(
@@ -273,12 +282,12 @@ def _policy_loss_launch(x, kl_coef, weight, grad, upstream=None, count=None):
         mean.data_ptr(), actions.data_ptr(), log_std.data_ptr(), ptr(ref_mean), ptr(ref_log_std),
         mean.stride(0), actions.stride(0), ld(log_std), 0 if ref_mean is None else ref_mean.stride(0), ld(ref_log_std), N,
         advantages.data_ptr(), ptr(fixed), ptr(valid), ptr(upstream), ptr(count), clip[0], clip[1], kl_coef, weight,
-        ptr(d_mean), ptr(d_log_std), ptr(log_probs), ptr(out), scratch.data_ptr())
-    with _Launch(dev) as st:
+        ptr(d_mean), ptr(d_log_std), ptr(log_probs), ptr(loss), ptr(info), ptr(n), scratch.data_ptr())
+    with lib.Launch(dev) as st:
         rc = L.hoic_policy_loss(args, st)
     if rc != 0:
         raise lib.HoicError(f"hoic_policy_loss failed ({rc}): {L.hoic_last_error().decode()}")
-    return out, d_mean, d_log_std, log_probs
+    return loss, info, n, d_mean, d_log_std, log_probs
 
 
 class _ClippedPolicyLoss(torch.autograd.Function):
@@ -288,10 +297,9 @@ class _ClippedPolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, kl_coef, clip, mean, log_std, *rest):
         actions, advantages, fixed, ref_mean, ref_log_std, valid = rest
-        out, _, _, log_probs = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0, False)
+        loss, info, ctx.count, _, _, log_probs = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0, False)
         ctx.save_for_backward(mean, log_std, *rest)
-        ctx.consts, ctx.count = (kl_coef, clip), out[6:].view(torch.float64)
-        loss, info = out[0], out[1:5]
+        ctx.consts = (kl_coef, clip)
         ctx.mark_non_differentiable(*((info,) if log_probs is None else (info, log_probs)))
         return loss, info, log_probs
 
@@ -300,7 +308,7 @@ class _ClippedPolicyLoss(torch.autograd.Function):
     def backward(ctx, g, *_):
         mean, log_std, actions, advantages, fixed, ref_mean, ref_log_std, valid = ctx.saved_tensors
         kl_coef, clip = ctx.consts
-        _, d_mean, d_log_std, _ = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0,
+        *_, d_mean, d_log_std, _ = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0,
                                                       True, upstream=g.float().contiguous(), count=ctx.count)
         return (None, None, d_mean, d_log_std) + (None,) * 6
 
@@ -373,8 +381,8 @@ def clipped_policy_loss_grad(mean, log_std, actions, advantages, fixed_log_probs
             d_mean, d_log_std = torch.autograd.grad(loss * weight, (mu, s))
         return PolicyLossGrad(loss.detach(), info, d_mean, d_log_std, log_probs)
     x = _loss_inputs(mean, log_std, *args)
-    out, d_mean, d_log_std, log_probs = _policy_loss_launch(x, float(kl_coef), float(weight), True)
-    return PolicyLossGrad(out[0], out[1:5], d_mean, d_log_std if log_std.dim() == 2 else d_log_std[0], log_probs)
+    loss, info, _, d_mean, d_log_std, log_probs = _policy_loss_launch(x, float(kl_coef), float(weight), True)
+    return PolicyLossGrad(loss, info, d_mean, d_log_std if log_std.dim() == 2 else d_log_std[0], log_probs)
 
 
 # ----------------------------------------------------------------------------- observation filter

@@ -357,8 +357,8 @@ enum hoic_type { HOIC_F32 = 0, HOIC_F16 = 1, HOIC_BF16 = 2 };
  *   d_mean  NULL: value only;  else weight * upstream * dL/dmean (t_mean; upstream: device scalar, NULL = 1)
  *   d_log_std  (with d_mean) t_std: [dims] summed over the rows when ld_std is 0, else [rows][dims] contiguous
  *   log_probs [rows]: l (0 outside `valid`) or NULL
- *   out [8] float32: L (unweighted), mean S, mean K, share of rows without gradient (clipped), n, 0, and n as a double in out[6..7]
- *   count  device double: the n of an earlier call's out + 6 (gradient alone: the scalars are not computed, out is not written)
+ *   loss: L (unweighted);  info [4]: mean S, mean K, share of rows without gradient (clipped), n;  n_out: n as a double, or NULL
+ *   count  device double: the n of an earlier call (gradient alone: the scalars are not computed, loss, info, n_out not written)
  *   scratch  hoic_policy_loss_scratch_bytes(dims) bytes, aligned to 8 */
 typedef struct hoic_policy_loss_args {
   int64_t rows;
@@ -371,7 +371,8 @@ typedef struct hoic_policy_loss_args {
   const double* count;
   double clip_lo, clip_hi, kl_coef, weight;
   void *d_mean, *d_log_std;
-  float *log_probs, *out;
+  float *log_probs, *loss, *info;
+  double* n_out;
   void* scratch;
 } hoic_policy_loss_args;
 int64_t hoic_policy_loss_scratch_bytes(int32_t dims);

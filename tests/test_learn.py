@@ -328,10 +328,10 @@ def test_policy_loss_entry_point_refuses_on_the_host():
     L = lib.load()
     assert L.hoic_policy_loss(None, None) == -1
     names = ("rows dims t_mean t_act t_std mean act log_std ref_mean ref_log_std ld_mean ld_act ld_std ld_ref_mean ld_ref_std ld_dmean adv fixed valid upstream count "
-             "clip_lo clip_hi kl_coef weight d_mean d_log_std log_probs out scratch").split()
+             "clip_lo clip_hi kl_coef weight d_mean d_log_std log_probs loss info n_out scratch").split()
     at = 64
-    good = dict.fromkeys(names, 0) | dict(rows=4, dims=4, mean=at, act=at, log_std=at, adv=at, out=at, scratch=at)
-    for change in (dict(dims=0), dict(dims=257), dict(rows=-1), dict(t_mean=3), dict(t_mean=2, t_act=1), dict(t_std=1), dict(mean=0), dict(scratch=0), dict(out=0),
+    good = dict.fromkeys(names, 0) | dict(rows=4, dims=4, mean=at, act=at, log_std=at, adv=at, loss=at, info=at, scratch=at)
+    for change in (dict(dims=0), dict(dims=257), dict(rows=-1), dict(t_mean=3), dict(t_mean=2, t_act=1), dict(t_std=1), dict(mean=0), dict(scratch=0), dict(loss=0), dict(info=0),
                    dict(ref_mean=at), dict(ref_log_std=at), dict(d_log_std=at), dict(count=at)):
         assert L.hoic_policy_loss(lib.POLICY_LOSS_ARGS.pack(*(good | change).values()), None) == -1, change
     assert L.hoic_policy_loss_scratch_bytes(0) == 0
