@@ -1867,13 +1867,52 @@ __device__ __forceinline__ double2 join_norm(const Joint& j) {
 struct NormEntry { const void* g; long long n; int first; };
 #define NORM_MAX 120
 struct NormArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; double* part; };
-template <class T> __device__ __forceinline__ double sumsq(const T* g, long long i0, long long i1) {
-  double s = 0.;
-  for (long long i = i0 + threadIdx.x * 4; i < i1; i += 1024) {
-    const long long l = i1 - i;
-    const f32x4 x = load4(g + i, l < 4 ? (int)l : 4);
+// Eight loads of 16 bytes a lane, all in flight before the first is used: 8192 elements of 32 bits a workgroup's step, 16384 of 16
+#define NORM_STEP 16384          // elements in whole steps of either kind
+typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef __bf16 b8u __attribute__((ext_vector_type(8), aligned(2)));
+template <class T> struct wide { typedef typename vec4<T>::type type; enum { n = 4 }; };
+template <> struct wide<_Float16> { typedef h8u type; enum { n = 8 }; };
+template <> struct wide<__bf16> { typedef b8u type; enum { n = 8 }; };
+template <class T> struct WideStep {
+  static constexpr int N = wide<T>::n, SPAN = 256 * N;          // elements of a load, of a workgroup's row of loads
+  typename wide<T>::type x[8];
+  // the lane's elements from i on, of which those below i1 exist (the rest read as 0)
+  __device__ __forceinline__ void load(const T* g, long long i, long long i1) {
+    if (i - threadIdx.x * N + 8 * SPAN <= i1) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) s = fma((double)x[e], (double)x[e], s);
+      for (int u = 0; u < 8; u++) x[u] = *(const typename wide<T>::type*)(g + i + u * SPAN);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const long long at = i + u * SPAN;
+        if (at + N <= i1) { x[u] = *(const typename wide<T>::type*)(g + at); continue; }
+#pragma unroll
+        for (int e = 0; e < N; e++) x[u][e] = at + e < i1 ? g[at + e] : (T)0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* g, long long i, long long i1) const {
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const long long at = i + u * SPAN;
+      if (at + N <= i1) { *(typename wide<T>::type*)(g + at) = x[u]; continue; }
+#pragma unroll
+      for (int e = 0; e < N; e++) if (at + e < i1) g[at + e] = x[u][e];
+    }
+  }
+};
+template <class T> __device__ __forceinline__ double sumsq(const T* g, long long i0, long long i1) {
+  typedef WideStep<T> W;
+  double s = 0.;
+  W w;
+  for (long long i = i0 + threadIdx.x * W::N; i - threadIdx.x * W::N < i1; i += 8 * W::SPAN) {
+    w.load(g, i, i1);
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+#pragma unroll
+      for (int e = 0; e < W::N; e++) { const double x = (double)(float)w.x[u][e]; s = fma(x, x, s); }
+    }
   }
   return s;
 }
@@ -1895,30 +1934,40 @@ __global__ __launch_bounds__(256) void hoic_norm_finish_kernel(Joint j, double* 
 }
 // g *= factor where it is not 1
 struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; Joint clip; };
-template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, float c) {
-  for (long long i = i0 + threadIdx.x * 4; i < i1; i += 1024) {
-    const int l = i1 - i < 4 ? (int)(i1 - i) : 4;
-    f32x4 x = load4(g + i, l);
+template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, const Joint& clip) {
+  typedef WideStep<T> W;
+  W w;
+  long long i = i0 + threadIdx.x * W::N;
+  w.load(g, i, i1);                            // (on their way while the norm is joined)
+  const double f = join_norm(clip).y;
+  if (f == 1.) return;
+  const float c = (float)f;
+  while (true) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) x[e] *= c;
-    store4(g + i, l, x);
+    for (int u = 0; u < 8; u++) {
+#pragma unroll
+      for (int e = 0; e < W::N; e++) w.x[u][e] = (T)((float)w.x[u][e] * c);
+    }
+    w.store(g, i, i1);
+    i += 8 * W::SPAN;
+    if (i - threadIdx.x * W::N >= i1) break;
+    w.load(g, i, i1);
   }
 }
 __global__ __launch_bounds__(256) void hoic_scale_kernel(ScaleArgs a) {
-  const double c = join_norm(a.clip).y;
-  if (c == 1.) return;
   const int t = list_find(a.t, a.nt, blockIdx.x);
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * a.chunk, i1 = i0 + a.chunk < a.t[t].n ? i0 + a.chunk : a.t[t].n;
-  if (a.type == HOIC_F32) scale_list((float*)a.t[t].g, i0, i1, (float)c);
-  else if (a.type == HOIC_F16) scale_list((_Float16*)a.t[t].g, i0, i1, (float)c);
-  else scale_list((__bf16*)a.t[t].g, i0, i1, (float)c);
+  if (a.type == HOIC_F32) scale_list((float*)a.t[t].g, i0, i1, a.clip);
+  else if (a.type == HOIC_F16) scale_list((_Float16*)a.t[t].g, i0, i1, a.clip);
+  else scale_list((__bf16*)a.t[t].g, i0, i1, a.clip);
 }
-// elements a workgroup: at least 8192, at most ~2048 workgroups (= parts) a list beyond one per tensor
+// elements a workgroup: whole steps, or one of 8192 in lists too short to fill the chip otherwise; at most ~1024 workgroups (= parts) a list
+// beyond one per tensor
 static long long norm_chunk(const int64_t* n, int32_t nt) {
   long long tot = 0;
   for (int i = 0; i < nt; i++) tot += n[i];
-  const long long c = (tot + 2047) / 2048;
-  return std::max<long long>(8192, (c + 1023) / 1024 * 1024);
+  const long long c = (tot + 1023) / 1024;
+  return c <= 8192 ? 8192 : (c + NORM_STEP - 1) / NORM_STEP * NORM_STEP;
 }
 #define JOIN_PARTS 2048          // up to so many parts are joined by the workgroups that use them
 static int32_t norm_check(const char* who, const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt) {
@@ -2060,6 +2109,18 @@ __device__ __forceinline__ unsigned wave_max(unsigned x) {
 #define JOIN_BLOCKS 4096         // a launch of more workgroups is given the joined factor
 template <class T> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
+  T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; float* m = (float*)a.t[t].m; float* v = (float*)a.t[t].v;
+  const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM32_CHUNK, left = a.t[t].n - i0;
+  constexpr int U = ADAM32_CHUNK / 1024;
+  f32x4 pp[U], gg[U], mm[U], vv[U];
+  auto count = [&](int u) { const long long o = left - u * 1024 - threadIdx.x * 4; return o < 4 ? (int)o : 4; };      // elements of the lane's four that exist
+  const bool whole = left >= ADAM32_CHUNK;
+#pragma unroll
+  for (int u = 0; u < U; u++) {            // on their way while the norm is joined
+    const long long i = i0 + u * 1024 + threadIdx.x * 4;
+    const int l = whole ? 4 : count(u);
+    gg[u] = load4(g + i, l); mm[u] = load4(m + i, l); vv[u] = load4(v + i, l); pp[u] = load4(p + i, l);
+  }
   float cl = 1.f;
   if (a.clip.parts) {
     const double2 f = join_norm(a.clip);
@@ -2067,23 +2128,18 @@ template <class T> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(Ad
     cl = (float)f.y;
   }
   const AdamConsts c = adam_consts(a, t);
-  T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; float* m = (float*)a.t[t].m; float* v = (float*)a.t[t].v;
-  const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM32_CHUNK, left = a.t[t].n - i0;
 #pragma unroll
-  for (int u = 0; u < ADAM32_CHUNK / 1024; u++) {
-    const long long o = u * 1024 + threadIdx.x * 4;
-    if (o >= left) break;
-    const int l = left - o < 4 ? (int)(left - o) : 4;
-    const long long i = i0 + o;
-    f32x4 pp = load4(p + i, l), gg = load4(g + i, l), mm = load4(m + i, l), vv = load4(v + i, l);
+  for (int u = 0; u < U; u++) {
+    const long long i = i0 + u * 1024 + threadIdx.x * 4;
+    const int l = whole ? 4 : count(u);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float x = gg[e] * cl;
-      mm[e] = fmaf(a.b1, mm[e], a.c1 * x);
-      vv[e] = fmaf(a.b2, vv[e], a.c2 * x * x);
-      pp[e] = adam_param(pp[e], mm[e], vv[e], c, a.eps);
+      const float x = gg[u][e] * cl;
+      mm[u][e] = fmaf(a.b1, mm[u][e], a.c1 * x);
+      vv[u][e] = fmaf(a.b2, vv[u][e], a.c2 * x * x);
+      pp[u][e] = adam_param(pp[u][e], mm[u][e], vv[u][e], c, a.eps);
     }
-    store4(m + i, l, mm); store4(v + i, l, vv); store4(p + i, l, pp);
+    store4(m + i, l, mm[u]); store4(v + i, l, vv[u]); store4(p + i, l, pp[u]);
   }
 }
 __device__ __forceinline__ unsigned hi32(double x) { return (unsigned)(__builtin_bit_cast(unsigned long long, x) >> 32); }
@@ -2183,17 +2239,9 @@ __device__ __forceinline__ unsigned code8_quick(double a, double r, int low, uns
 }
 template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
-  double cl = 1.;
-  if (a.clip.parts) {
-    const double2 f = join_norm(a.clip);
-    if (!(f.x < INFINITY)) return;
-    cl = f.y;
-  }
-  const AdamConsts c = adam_consts(a, t);
   T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; unsigned char* m = (unsigned char*)a.t[t].m; unsigned char* v = (unsigned char*)a.t[t].v;
   float* ms = a.t[t].ms; float* vs = a.t[t].vs;
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM8_CHUNK, left = a.t[t].n - i0;
-  const unsigned key = mix32(c.key + (unsigned)(i0 >> 32));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   constexpr int U = ADAM8_CHUNK / 1024;
   unsigned again = 0;               // blocks left to adam8_block, a tensor's last, partial one among them
@@ -2209,6 +2257,14 @@ template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(Ada
     cm[u] = *(const unsigned*)(m + i); cv[u] = *(const unsigned*)(v + i);
     km[u] = ms[(i0 + ob) >> 8]; kv[u] = vs[(i0 + ob) >> 8];
   }
+  double cl = 1.;
+  if (a.clip.parts) {
+    const double2 f = join_norm(a.clip);
+    if (!(f.x < INFINITY)) return;
+    cl = f.y;
+  }
+  const AdamConsts c = adam_consts(a, t);
+  const unsigned key = mix32(c.key + (unsigned)(i0 >> 32));
 #pragma unroll
   for (int u = 0; u < U; u++) {
     const long long ob = (u * 4 + wave) * 256, i = i0 + ob + lane * 4, blk = (i0 + ob) >> 8;

@@ -283,24 +283,30 @@ class AdamW(torch.optim.Optimizer):
     def state_values(self):
         """([m, ...], [v, ...]): both moments of every parameter in float32 (8-bit states: the values that their codes stand for, made
         anew by one launch per 48 tensors; 32-bit ones: the states themselves); zeros where a parameter has no state yet."""
+        bits, groups = self.defaults["state_bits"], self.param_groups
+        states = [(p, self.state.get(p)) for group in groups for p in group["params"]]
+        if bits == 32 and all(s for _, s in states):
+            return [s["exp_avg"] for _, s in states], [s["exp_avg_sq"] for _, s in states]
+        new = lambda p: torch.empty_like(p, dtype=torch.float32, requires_grad=False)
         ms, vs, work = [], [], {}
-        bits = self.defaults["state_bits"]
-        for group in self.param_groups:
-            for p in group["params"]:
-                s = self.state.get(p)
-                if not s:
-                    m, v = torch.zeros_like(p, dtype=torch.float32, requires_grad=False), torch.zeros_like(p, dtype=torch.float32, requires_grad=False)
-                elif bits == 32:
-                    m, v = s["exp_avg"], s["exp_avg_sq"]
-                else:
-                    m, v = torch.empty_like(p, dtype=torch.float32, requires_grad=False), torch.empty_like(p, dtype=torch.float32, requires_grad=False)
-                    work.setdefault(p.device, []).extend((m.data_ptr(), v.data_ptr(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(),
-                                                          s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr(), p.numel(), 1, 0, 0))
-                ms.append(m)
-                vs.append(v)
-        for dev, flat in work.items():
+        first = states[0][0]
+        if bits == 8 and all(s and p.device == first.device and p.is_contiguous() for p, s in states):
+            # one buffer a moment, cut into the parameters' shapes (an allocation a parameter costs more than the launch)
+            params, n = [p for p, _ in states], sum(p.numel() for p, _ in states)
+            ms, vs = (list(torch._C._nn.unflatten_dense_tensors(torch.empty(n, dtype=torch.float32, device=first.device), params)) for _ in range(2))
+        for i, (p, s) in enumerate(states):
+            if len(ms) <= i:
+                ms.append(s["exp_avg"] if s and bits == 32 else new(p) if s else new(p).zero_())
+                vs.append(s["exp_avg_sq"] if s and bits == 32 else new(p) if s else new(p).zero_())
+            if s and bits == 8:
+                rows = work.get(p.device)
+                if rows is None:
+                    rows = work[p.device] = []
+                rows += (ms[i].data_ptr(), vs[i].data_ptr(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), s["exp_avg_scale"].data_ptr(),
+                         s["exp_avg_sq_scale"].data_ptr(), p.numel(), 1, 0, 0)
+        for dev, rows in work.items():
             with lib.Launch(dev) as st:
-                lib._chk(lib.load().hoic_adamw_values((C.c_int64 * len(flat))(*flat), len(flat) // 10, st), "hoic_adamw_values")
+                lib._chk(lib.load().hoic_adamw_values((C.c_int64 * len(rows))(*rows), len(rows) // 10, st), "hoic_adamw_values")
         return ms, vs
 
 
