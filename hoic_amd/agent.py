@@ -40,7 +40,7 @@ from .config import Config
 from .env import BatchedHandObjMimic
 from . import lib
 from .lib import NV as lib_NV
-from .rl import MLP, BatchZFilter, PolicyGaussian, RunningStat, Value, ZFilter, estimate_advantages, ppo_loss
+from .rl import MLP, BatchZFilter, PolicyGaussian, RunningStat, Value, ZFilter, clipped_policy_loss, estimate_advantages, ppo_loss
 
 
 class RefUnpickler(pickle.Unpickler):
@@ -154,10 +154,10 @@ class PPOLearner:
         # update_streams (f16x3 update on one rank): 3 = every GEMM on one stream, each chain's small kernels on a stream of its own
         # (default), 2 = the value chain on a side stream, 1 = one stream
         self.update_streams = int(update_streams)
-        fused = {"fused": True} if (torch.device(device).type == "cuda" and fused_adam) else {}
-        self.optimizer_policy = torch.optim.Adam(self.policy_net.parameters(), lr=cfg.policy_lr, weight_decay=cfg.policy_weightdecay, **fused)
-        self.optimizer_value = torch.optim.Adam(self.value_net.parameters(), lr=cfg.value_lr, weight_decay=cfg.value_weightdecay, **fused)
+        self.optimizer_policy = self._make_optimizer(getattr(cfg, "policy_optimizer", "Adam"), self.policy_net, cfg.policy_lr, cfg.policy_weightdecay, fused_adam, 0)
+        self.optimizer_value = self._make_optimizer(getattr(cfg, "value_optimizer", "Adam"), self.value_net, cfg.value_lr, cfg.value_weightdecay, fused_adam, 1)
         self.gamma, self.tau, self.clip_epsilon = cfg.gamma, cfg.tau, cfg.clip_epsilon
+        self.kl_coef = float(getattr(cfg, "kl_coef", 0.0))
         self.opt_num_epochs = cfg.num_optim_epoch
         self._losses = None
         self.aux_stream = None                 # a stream of the caller's that is idle during an update (update_streams=3: the policy chain's small kernels)
@@ -171,6 +171,20 @@ class PPOLearner:
         # the f16-range check of an update in two halves (mlp._post_overflow): with defer_checks the host does not wait for
         # the update it has just enqueued -- the counters are read before the NEXT update is enqueued (or by finish_update)
         self.defer_checks = False
+
+    def _make_optimizer(self, name, net, lr, weight_decay, fused_adam, ordinal):
+        """cfg.policy_optimizer / value_optimizer: "AdamW" and "AdamW8bit" = hoic_amd.optim.AdamW with moments in 32 or 8 bits (decoupled
+        weight decay; the same rounding on every rank: the seed is the config's), anything else the reference's Adam"""
+        cuda = self.device.type == "cuda"
+        if name in ("AdamW", "AdamW8bit") and cuda and self.dtype == torch.float32:
+            from .optim import AdamW
+            return AdamW(net.parameters(), lr=lr, weight_decay=weight_decay, state_bits=8 if name == "AdamW8bit" else 32, seed=2 * int(self.cfg.seed) + ordinal)
+        if name == "AdamW8bit":
+            raise lib.HoicError("AdamW8bit: 8-bit moments exist on the GPU only, for float32 networks")
+        if name == "AdamW":
+            return torch.optim.AdamW(net.parameters(), lr=lr, weight_decay=weight_decay)
+        fused = {"fused": True} if (cuda and fused_adam) else {}
+        return torch.optim.Adam(net.parameters(), lr=lr, weight_decay=weight_decay, **fused)
 
     # ------------------------------------------------------------------ update (agent_pg.py:39-55, agent_ppo.py:16-64)
     def _allreduce_start(self, params):
@@ -295,13 +309,23 @@ class PPOLearner:
             (loss * weight if weight != 1.0 else loss).backward()
             return loss.detach(), h.grad
 
+        old = {}                # the policy at the start of the update (kl_coef): its means and log_std
+
         def policy_step_head(h, fixed_log_probs):
             if M.heads_fusable(h, self.policy_net.action_mean):
+                if self.kl_coef:
+                    return M.ppo_kl_head_step(h, self.policy_net, actions, advantages, fixed_log_probs, self.clip_epsilon, self.kl_coef, old, weight)
                 return M.ppo_head_step(h, self.policy_net, actions, advantages, fixed_log_probs, self.clip_epsilon, weight)
             if fixed_log_probs is None:
                 with torch.no_grad():
                     fixed_log_probs = self.policy_net.get_log_prob(None, actions, hidden=h.detach())
-            loss = ppo_loss(self.policy_net, None, actions, advantages, fixed_log_probs, self.clip_epsilon, hidden=h)
+                    if self.kl_coef:
+                        old["mean"], old["log_std"] = M.head_linear(h.detach(), self.policy_net.action_mean), self.policy_net.action_log_std.detach().clone()
+            if self.kl_coef:
+                loss = clipped_policy_loss(M.head_linear(h, self.policy_net.action_mean), self.policy_net.action_log_std, actions, advantages, fixed_log_probs,
+                                           self.clip_epsilon, ref_mean=old["mean"], ref_log_std=old["log_std"], kl_coef=self.kl_coef).loss
+            else:
+                loss = ppo_loss(self.policy_net, None, actions, advantages, fixed_log_probs, self.clip_epsilon, hidden=h)
             (loss * weight if weight != 1.0 else loss).backward()
             return loss.detach(), h.grad, fixed_log_probs
 
@@ -513,16 +537,24 @@ class PPOLearner:
             states = PackedInput(states)
         if not f16x3:
             with torch.no_grad(), self._autocast():
-                fixed_log_probs = self.policy_net.get_log_prob(states, actions).float()
+                if self.kl_coef:
+                    old_mean, old_log_std = self.policy_net(states)[0], self.policy_net.action_log_std.detach().clone()
+                    fixed_log_probs = clipped_policy_loss(old_mean, old_log_std, actions, advantages, None, self.clip_epsilon).log_probs
+                else:
+                    fixed_log_probs = self.policy_net.get_log_prob(states, actions).float()
 
         def policy_step(pending):
             self._allreduce_finish(pending)
             # policy_grad_clip=[(parameters() generator, 40)] clips only on the first optimizer step of the run
             # (agent_handmimic.py:67); strict_reference=False clips every step
-            if not (self.strict_reference and self._policy_clip_used):
-                torch.nn.utils.clip_grad_norm_(pparams, 40)
-                self._policy_clip_used = True
-            self.optimizer_policy.step()
+            clip = not (self.strict_reference and self._policy_clip_used)
+            self._policy_clip_used = True
+            if hasattr(self.optimizer_policy, "grad_norm"):       # hoic_amd.optim.AdamW clips inside its step
+                self.optimizer_policy.step(max_norm=40 if clip else None)
+            else:
+                if clip:
+                    torch.nn.utils.clip_grad_norm_(pparams, 40)
+                self.optimizer_policy.step()
             if self._engines is not None:
                 self._engines[1].weights_changed()
 
@@ -542,7 +574,11 @@ class PPOLearner:
             if p_waiting:
                 policy_step(p_pending); p_waiting = False
             with self._autocast():
-                surr = ppo_loss(self.policy_net, states, actions, advantages, fixed_log_probs, self.clip_epsilon)
+                if self.kl_coef:
+                    surr = clipped_policy_loss(self.policy_net(states)[0], self.policy_net.action_log_std, actions, advantages, fixed_log_probs,
+                                               self.clip_epsilon, ref_mean=old_mean, ref_log_std=old_log_std, kl_coef=self.kl_coef).loss
+                else:
+                    surr = ppo_loss(self.policy_net, states, actions, advantages, fixed_log_probs, self.clip_epsilon)
             self.optimizer_policy.zero_grad(set_to_none=True)
             (surr * weight if weight != 1.0 else surr).backward()
             p_pending, p_waiting = self._allreduce_start(pparams), True

@@ -82,6 +82,8 @@ class Config:
         self.value_htype = g("value_htype", "relu"); self.value_hsize = g("value_hsize", [300, 200])
         self.value_optimizer = g("value_optimizer", "Adam"); self.value_lr = g("value_lr", 3e-4)
         self.value_momentum = g("value_momentum", 0.0); self.value_weightdecay = g("value_weightdecay", 0.0)
+        # kl_coef: weight of KL(policy at the start of the update || policy) in the policy loss (PPO's penalty form; 0 = the reference's loss)
+        self.kl_coef = float(g("kl_coef", 0.0))
         self.clip_epsilon = g("clip_epsilon", 0.2); self.log_std = g("log_std", -2.3); self.fix_std = g("fix_std", False)
         self.num_optim_epoch = g("num_optim_epoch", 10); self.min_batch_size = g("min_batch_size", 50000)
         self.mini_batch_size = g("mini_batch_size", self.min_batch_size)

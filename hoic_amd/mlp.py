@@ -716,6 +716,26 @@ def ppo_head_step(hidden, policy, actions, advantages, fixed_log_probs, clip_eps
     return sums[32], dh, (new_fixed if new_fixed is not None else fixed_log_probs.view(M_, 1))
 
 
+def ppo_kl_head_step(hidden, policy, actions, advantages, fixed_log_probs, clip_epsilon, kl_coef, old, weight=1.0):
+    """``ppo_head_step`` with ``kl_coef`` KL(old policy || policy) in the loss (hoic_policy_loss instead of hoic_mlp_ppo_loss).  ``old``: a
+    dict of the caller's, filled in epoch 0 (``fixed_log_probs`` None) with that epoch's means and log-deviations and read in the later
+    ones.  Sets the same ``.grad``s and returns the same three values; the loss includes the KL term."""
+    from .rl import clipped_policy_loss_grad
+    lin, dev = policy.action_mean, hidden.device
+    hidden = hidden.detach()
+    with torch.cuda.device(dev), torch.no_grad():
+        mean, log_std = action_head(hidden, lin.weight, lin.bias), policy.action_log_std.detach()
+        if fixed_log_probs is None:
+            old["mean"], old["log_std"] = mean, log_std.clone()
+        o = clipped_policy_loss_grad(mean, log_std, actions, advantages, fixed_log_probs, clip_epsilon, ref_mean=old["mean"], ref_log_std=old["log_std"],
+                                     kl_coef=kl_coef, weight=weight)
+        dh, dW, db = _head_backward(hidden, lin.weight, o.d_mean)
+        lin.weight.grad, lin.bias.grad = dW, db
+        if policy.action_log_std.requires_grad:
+            policy.action_log_std.grad = o.d_log_std
+    return o.loss, dh, (o.log_probs if fixed_log_probs is None else fixed_log_probs)
+
+
 def value_head_step(hidden, value_net, returns, weight=1.0):
     """One value epoch's head, loss and their backward pass without autograd (agent_pg.py:18-25): value head, mean squared error
     with its gradient (hoic_mlp_value_loss), head backward.  Sets ``.grad`` of value_head.weight / .bias; returns

@@ -47,6 +47,9 @@ def build_parser():
     p.add_argument("--update_dtype", default="f16x3", choices=["f16x3", "f32", "bf16"],
                    help="GEMMs of the PPO update: f16x3 = float32 operands as float16 pairs on the matrix cores (float32-class accuracy, "
                         "hidden sizes must be multiples of 256), f32 = PyTorch float32, bf16 = autocast")
+    p.add_argument("--optimizer", default=None, choices=["Adam", "AdamW", "AdamW8bit"],
+                   help="override cfg.policy_optimizer and cfg.value_optimizer: AdamW / AdamW8bit = hoic_amd.optim.AdamW with moments in 32 / 8 bits")
+    p.add_argument("--kl_coef", type=float, default=None, help="override cfg.kl_coef: weight of KL(sampling policy || policy) in the policy loss")
     return p
 
 
@@ -70,7 +73,11 @@ def main(argv=None):
         dist.init_process_group("nccl", device_id=torch.device("cuda", local_rank))
 
     cfg = Config(cfg_id=args.cfg, base_dir=args.base_dir, create_dirs=not (args.render or args.epoch > 0))
+    kl_coef = cfg.kl_coef if args.kl_coef is None else args.kl_coef
     cfg.update(args)                                    # the reference copies the argparse attributes onto cfg (:37)
+    cfg.kl_coef = kl_coef
+    if args.optimizer is not None:
+        cfg.policy_optimizer = cfg.value_optimizer = args.optimizer
     if args.num_epoch is not None:
         cfg.num_epoch = args.num_epoch
     if rank == 0:

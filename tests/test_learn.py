@@ -883,3 +883,116 @@ def test_rounding_bits_are_uniform():
     s = lambda x: (x >> 16) / 65536.0 - 0.5
     for a, b in ((f(h)[1:], f(h)[:-1]), (f(h), s(h)), (f(h), f(k)), (s(h), s(k)), (f(h), f(l)), (s(h), f(l)), (f(h)[256:], f(h)[:-256])):
         assert abs(float((a * b).mean()) * 12) < 6 * 2.0 ** -9
+
+
+# ================================================================================================ together: the learner's update
+def learner_config(hsize, **kw):
+    from hoic_amd.config import Config, release_cfg_dict
+    return Config("box_future5_light_add_geom", cfg_dict={**release_cfg_dict("box"), "policy_hsize": hsize, "value_hsize": hsize, "fix_std": False, **kw})
+
+
+def learner_batch(T, N, D, A, dtype, dev, seed=5):
+    from types import SimpleNamespace
+    g = torch.Generator().manual_seed(seed)
+    mk = lambda *sh: torch.randn(*sh, generator=g)
+    b = dict(states=torch.clamp(mk(T, N, D), -5, 5), actions=mk(T, N, A) * 0.1, rewards=torch.rand(T, N, generator=g), masks=(torch.rand(T, N, generator=g) > 0.05).float(),
+             next_values=torch.zeros(N))
+    return SimpleNamespace(valid=None, **{k: v.to(dev, dtype) for k, v in b.items()})
+
+
+def test_learner_kl_update_is_the_formula():
+    """PPOLearner on the CPU in float64 with kl_coef: five epochs against a loop written out here, to rounding"""
+    from hoic_amd.agent import PPOLearner
+    cfg = learner_config([24, 16], kl_coef=0.7, policy_lr=1e-2)
+    torch.manual_seed(3)
+    L = PPOLearner(cfg, 20, 5, "cpu", torch.float64)
+    assert L.kl_coef == 0.7 and type(L.optimizer_policy) is torch.optim.Adam
+    net = copy.deepcopy(L.policy_net)
+    b = learner_batch(4, 50, 20, 5, torch.float64, "cpu")
+    adv = torch.randn(200, 1, dtype=torch.float64, generator=torch.Generator().manual_seed(1))
+    states, actions = b.states.reshape(200, 20), b.actions.reshape(200, 5)
+    L.optimize(states, actions, adv, torch.zeros(200, 1, dtype=torch.float64))
+    opt = torch.optim.Adam(net.parameters(), lr=1e-2)
+    logp = lambda mu, s: (-(actions - mu) ** 2 / (2 * torch.exp(2 * s)) - s - 0.5 * math.log(2 * math.pi)).sum(1, keepdim=True)
+    mu0, s0 = (t.detach().clone() for t in net(states))
+    for ep in range(5):
+        mu, s = net(states)
+        r = torch.exp(logp(mu, s) - logp(mu0, s0))
+        kl = (s - s0 + (torch.exp(2 * s0) + (mu - mu0) ** 2) / (2 * torch.exp(2 * s)) - 0.5).sum(1, keepdim=True)
+        loss = (-torch.min(r * adv, torch.clamp(r, 0.8, 1.2) * adv) + 0.7 * kl).mean()
+        opt.zero_grad(); loss.backward()
+        if ep == 0:
+            torch.nn.utils.clip_grad_norm_(net.parameters(), 40)
+        opt.step()
+    for p, q in zip(L.policy_net.parameters(), net.parameters()):
+        assert float((p - q).abs().max()) < 1e-10             # five Adam steps of lr 1e-2: rounding of 1e-16 grows by 1 / (eps-like small gradients), 1e6 allowed
+    assert abs(L.last_losses[1] - float(loss)) < 1e-12
+
+
+def test_learner_optimizers_follow_the_config():
+    from hoic_amd.agent import PPOLearner
+    L = PPOLearner(learner_config([8], policy_optimizer="AdamW", value_optimizer="Adam", policy_weightdecay=0.1), 6, 2, "cpu")
+    assert type(L.optimizer_policy) is torch.optim.AdamW and type(L.optimizer_value) is torch.optim.Adam and L.optimizer_policy.param_groups[0]["weight_decay"] == 0.1
+    with pytest.raises(lib.HoicError):
+        PPOLearner(learner_config([8], policy_optimizer="AdamW8bit"), 6, 2, "cpu")
+
+
+@gpu
+@pytest.mark.parametrize("update_dtype,streams", [("f16x3", 3), ("f16x3", 1), ("f32", 3), ("bf16", 3)])
+def test_learner_update_with_kl_adamw_and_clipping(update_dtype, streams):
+    """loss with KL -> gradients -> norm and clipping -> AdamW in a learner's update (five epochs, both networks), against the same update
+    in float64 with torch's AdamW: as close as the float32 library path is (Adam divides rounding noise by its own size: any two
+    float32 computations differ there); with 8-bit moments within a quarter of the way moved (a code is 1/8 of its value
+    at most: 20 % of a step); the same bits in two runs."""
+    from hoic_amd.agent import PPOLearner
+    dev = torch.device("cuda")
+
+    def run(ud, optimizer, dtype=torch.float32):
+        torch.manual_seed(0)
+        cfg = learner_config([512, 256, 256], kl_coef=0.5, policy_optimizer=optimizer, value_optimizer=optimizer, policy_weightdecay=0.01, value_weightdecay=0.01)
+        # (float64 networks need the optimiser of float64 parameters: made before the first step)
+        L = PPOLearner(cfg, 617, 32, dev, update_dtype=ud, strict_reference=False, update_streams=streams)
+        if dtype == torch.float64 or optimizer == "torch":
+            for n, lr in (("policy", cfg.policy_lr), ("value", cfg.value_lr)):
+                getattr(L, n + "_net").to(dtype)
+                setattr(L, "optimizer_" + n, torch.optim.AdamW(getattr(L, n + "_net").parameters(), lr=lr, weight_decay=0.01))
+        start = {n: [p.detach().double().clone() for p in getattr(L, n + "_net").parameters()] for n in ("policy", "value")}
+        L.update_params(learner_batch(16, 256, 617, 32, dtype, dev))
+        return {n: [p.detach().double() for p in getattr(L, n + "_net").parameters()] for n in ("policy", "value")}, start, L
+
+    dist = lambda a, b: math.sqrt(sum(float(((x - y) ** 2).sum()) for x, y in zip(a, b)))
+    ref, start, L64 = run("f32", "torch", torch.float64)
+    lib32 = run("f32", "torch")[0]
+    got, _, L = run(update_dtype, "AdamW")
+    again = run(update_dtype, "AdamW")[0]
+    low, _, L8 = run(update_dtype, "AdamW8bit")
+    assert type(L.optimizer_policy) is optim.AdamW and L8.optimizer_policy.defaults["state_bits"] == 8
+    assert float(L.optimizer_policy.grad_norm) > 0 and all(L.optimizer_policy.state[p]["step"] == 5 for p in L.policy_net.parameters())
+    for n in ("policy", "value"):
+        moved = dist(ref[n], start[n])
+        assert moved > 0
+        if update_dtype != "bf16":
+            assert dist(got[n], ref[n]) <= 1.5 * dist(lib32[n], ref[n]) + 1e-3 * moved, n
+            assert dist(low[n], ref[n]) <= 0.25 * moved, n
+            assert all(torch.equal(x, y) for x, y in zip(got[n], again[n]))
+        else:                    # bfloat16 products: 2^-8 of a gradient and sign changes of small ones; the update's direction stays
+            assert dist(got[n], ref[n]) <= 0.5 * moved, n
+    if update_dtype != "bf16":
+        assert abs(L.last_losses[1] - L64.last_losses[1]) < 1e-4 * abs(L64.last_losses[1]) + 1e-6
+
+
+@gpu
+def test_learner_kl_holds_the_policy_back():
+    """the KL term's gradient reaches the networks: a large kl_coef leaves the policy nearer to where it was"""
+    from hoic_amd.agent import PPOLearner
+    moved = []
+    for kl in (0.0, 100.0):
+        torch.manual_seed(0)
+        L = PPOLearner(learner_config([512, 256, 256], kl_coef=kl, policy_lr=1e-3), 617, 32, torch.device("cuda"), update_dtype="f16x3")
+        b = learner_batch(16, 256, 617, 32, torch.float32, "cuda")
+        with torch.no_grad():
+            before = L.policy_net(b.states.reshape(-1, 617))[0]
+        L.update_params(b)
+        with torch.no_grad():
+            moved.append(float((L.policy_net(b.states.reshape(-1, 617))[0] - before).pow(2).mean()))
+    assert moved[1] < moved[0]
