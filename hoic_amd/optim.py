@@ -44,16 +44,29 @@ def _check(t, what):
         raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
 
 
-def _norm_list(grads):
-    """The arguments of the hoic_grad_norm family for CUDA tensors of one device: ((pointers, sizes, types, count), parts, tensors held)"""
-    dev, n = grads[0].device, len(grads)
-    for g in grads:
-        if g.device != dev:
-            raise ValueError(f"one norm over gradients on several devices ({dev}, {g.device})")
-    grads = [g if _dense(g) else g.contiguous() for g in grads]
-    sizes = (C.c_int64 * n)(*[g.numel() for g in grads])
-    args = ((C.c_void_p * n)(*[g.data_ptr() for g in grads]), sizes, bytes([TYPES[g.dtype] for g in grads]), n)
-    return args, lib.load().hoic_grad_norm_parts(sizes, n), grads
+def _list_args(ptrs, sizes, types):
+    """(pointers, sizes, types, count) of the hoic_grad_norm family, and the number of partial sums"""
+    n = len(ptrs)
+    sizes = (C.c_int64 * n)(*sizes)
+    return ((C.c_void_p * n)(*ptrs), sizes, bytes(types), n), lib.load().hoic_grad_norm_parts(sizes, n)
+
+
+def _tensor_list(tensors, what):
+    """_list_args of dense CUDA tensors of one device"""
+    ptrs, sizes, types, at = [], [], [], None
+    for t in tensors:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in TYPES and t.layout is torch.strided):
+            _check(t, what)
+        if t.get_device() != at:
+            if at is not None:
+                raise ValueError(f"{what}: one norm over tensors on several devices (cuda:{at}, {t.device})")
+            at = t.get_device()
+        if not t.is_contiguous() and not _dense(t):
+            raise ValueError(f"{what}: a tensor whose elements do not fill their memory (an expanded or cut view)")
+        ptrs.append(t.data_ptr())
+        sizes.append(t.numel())
+        types.append(TYPES[t.dtype])
+    return _list_args(ptrs, sizes, types)
 
 
 def _bound(max_norm):
@@ -67,19 +80,20 @@ def grad_norm(tensors):
     """sqrt(sum of squares) over a list of tensors (float32 / float16 / bfloat16, any mix, one device) as a float32 scalar on the
     device; 64-bit sums in a fixed order: the same bits in every run."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    for t in tensors:
-        _check(t, "grad_norm")
     if not tensors:
         return torch.zeros(())
-    with torch.no_grad():
-        args, parts, held = _norm_list(tensors)
-        dev = held[0].device
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        if parts == 0:
-            return norm.zero_()
-        buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
-        with lib.Launch(dev) as st:
-            lib._chk(lib.load().hoic_grad_norm(*args, buf.data_ptr(), norm.data_ptr(), st), "hoic_grad_norm")
+    for i, t in enumerate(tensors):
+        _check(t, "grad_norm")
+        if not _dense(t):
+            tensors[i] = t.detach().contiguous()
+    args, parts = _tensor_list(tensors, "grad_norm")
+    dev = tensors[0].device
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    if parts == 0:
+        return norm.zero_()
+    buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
+    with lib.Launch(dev) as st:
+        lib._chk(lib.load().hoic_grad_norm(*args, buf.data_ptr(), norm.data_ptr(), st), "hoic_grad_norm")
     return norm
 
 
@@ -89,21 +103,17 @@ def clip_grad_norm_(parameters, max_norm):
     that is not finite gives the factor that the formula gives (0 or NaN)."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [g for g in [p.grad for p in parameters] if g is not None]
-    b = _bound(max_norm)
-    for g in grads:
-        _check(g, "clip_grad_norm_")
-        if not _dense(g):
-            raise ValueError("clip_grad_norm_: a gradient whose elements do not fill their memory cannot be scaled in place")
+    bound = _bound(max_norm)
     if not grads:
         return torch.zeros(())
-    args, parts, _ = _norm_list(grads)
+    args, parts = _tensor_list(grads, "clip_grad_norm_")
     dev = grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=dev)
     if parts == 0:
         return norm.zero_()
     buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
     with lib.Launch(dev) as st:
-        lib._chk(lib.load().hoic_clip_grads(*args, b, buf.data_ptr(), norm.data_ptr(), st), "hoic_clip_grads")
+        lib._chk(lib.load().hoic_clip_grads(*args, bound, buf.data_ptr(), norm.data_ptr(), st), "hoic_clip_grads")
     torch.autograd.graph.increment_version(grads)
     return norm
 
@@ -208,8 +218,11 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         bound = None if max_norm is None else _bound(max_norm)
         bits, capturable = self.defaults["state_bits"], self.defaults["capturable"]
+        capturing, state = torch.cuda.is_current_stream_capturing(), self.state
         # rows of the list (hoic_adamw_tensor) per device, group and type
-        ordinal, work, grads, params, fresh = -1, {}, [], [], []
+        ordinal, work, key, rows = -1, {}, None, None
+        params, held, touched, g_ptrs, g_sizes, g_types = [], [], [], [], [], []
+        t = d_step = m_scale = v_scale = 0
         for gi, group in enumerate(self.param_groups):
             for p in group["params"]:
                 ordinal += 1
@@ -220,34 +233,47 @@ class AdamW(torch.optim.Optimizer):
                 if g.dtype is not dtype or g.layout is not torch.strided:
                     raise ValueError(f"AdamW: a {g.dtype} gradient (dense ones only) of a {dtype} parameter")
                 if not (p.is_contiguous() and g.is_contiguous()) and _strides(g) != _strides(p):
-                    g = torch.empty_like(p).copy_(g.detach())          # the parameter's order of elements
+                    g = torch.empty_like(p, requires_grad=False).copy_(g.detach())          # the parameter's order of elements
+                    held.append(g)
+                s = state[p]
+                if not s or capturing:
+                    if capturing and not capturable:
+                        raise lib.HoicError("AdamW: a captured step needs capturable=True (its step count would stand still)")
+                    if capturing and not s:
+                        raise lib.HoicError("AdamW: take one eager step before a capture (the states would be made anew at every replay)")
+                    if not s:
+                        s.update(self._make_state(p))
+                if (p.get_device(), gi, dtype) != key:
+                    key = (p.get_device(), gi, dtype)
+                    rows = work.get(key)
+                    if rows is None:
+                        rows = work[key] = []
+                if capturable:
+                    d_step = s["step"].data_ptr()
+                else:
+                    t = s["step"] + 1
+                if bits == 8:
+                    m_scale, v_scale = s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr()
+                ptr, n = g.data_ptr(), p.numel()
+                rows += (p.data_ptr(), ptr, s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), m_scale, v_scale, n, t, d_step, ordinal)
                 params.append(p)
-                grads.append(g)
-                s = self.state[p]
-                if not s:
-                    fresh.append(p)
-                todo = work.get((p.device, gi, dtype))
-                if todo is None:
-                    todo = work[(p.device, gi, dtype)] = []
-                todo.append((p, g, s, ordinal))
+                touched.append(s)
+                g_ptrs.append(ptr)
+                g_sizes.append(n)
+                g_types.append(TYPES[dtype])
         self.grad_norm = None
         if not work:
             if bound is not None:
                 self.grad_norm = torch.zeros(())
             return loss
-        if torch.cuda.is_current_stream_capturing():
-            if not capturable:
-                raise lib.HoicError("AdamW: a captured step needs capturable=True (its step count would stand still)")
-            if fresh:
-                raise lib.HoicError("AdamW: take one eager step before a capture (the states would be made anew at every replay)")
-        for p in fresh:
-            self.state[p].update(self._make_state(p))
         L = lib.load()
         buf_ptr = norm_ptr = parts = 0
         if bound is not None:
-            args, parts, held = _norm_list(grads)
-            dev = held[0].device
+            if len({k[0] for k in work}) > 1:
+                raise ValueError("AdamW: one norm over gradients on several devices")
+            dev = params[0].device
             self.grad_norm = norm = torch.empty((), dtype=torch.float32, device=dev)
+            args, parts = _list_args(g_ptrs, g_sizes, g_types)
             if parts:
                 buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
                 buf_ptr, norm_ptr = buf.data_ptr(), norm.data_ptr()
@@ -255,28 +281,22 @@ class AdamW(torch.optim.Optimizer):
                     lib._chk(L.hoic_grad_norm_partial(*args, buf_ptr, st), "hoic_grad_norm_partial")
             else:
                 norm.zero_()
-        for (dev, gi, dtype), todo in work.items():
-            group = self.param_groups[gi]
+        if not capturable:
+            for s in touched:
+                s["step"] += 1
+        for (at, gi, dtype), rows in work.items():
+            group, dev, n = self.param_groups[gi], torch.device("cuda", at), len(rows) // 10
             lr, (b1, b2) = group["lr"], group["betas"]
             lr_ptr = 0
             if isinstance(lr, torch.Tensor):
                 if not capturable or lr.device != dev or lr.dtype != torch.float32 or lr.numel() != 1:
                     raise ValueError("lr: a float, or with capturable=True a float32 tensor of one element on the parameters' device")
                 lr, lr_ptr = 0.0, lr.data_ptr()
-            flat, t, d_step, ms, vs = [], 0, 0, 0, 0
-            for p, g, s, o in todo:
-                if capturable:
-                    d_step = s["step"].data_ptr()
-                else:
-                    s["step"] = t = s["step"] + 1
-                if bits == 8:
-                    ms, vs = s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr()
-                flat += (p.data_ptr(), g.data_ptr(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), ms, vs, p.numel(), t, d_step, o)
-            consts = torch.empty(4 * len(todo), dtype=torch.float32, device=dev) if capturable else None
+            consts = torch.empty(4 * n, dtype=torch.float32, device=dev) if capturable else None
             a = lib.ADAMW_ARGS.pack(TYPES[dtype], bits, lr, b1, b2, group["eps"], group["weight_decay"], lr_ptr,
                                     0 if consts is None else consts.data_ptr(), buf_ptr, norm_ptr, bound or 0.0, parts, group["seed"], 0)
             with lib.Launch(dev) as st:
-                lib._chk(L.hoic_adamw((C.c_int64 * len(flat))(*flat), len(todo), a, st), "hoic_adamw")
+                lib._chk(L.hoic_adamw((C.c_int64 * len(rows))(*rows), n, a, st), "hoic_adamw")
         torch.autograd.graph.increment_version(params)
         return loss
 

@@ -996,3 +996,22 @@ def test_learner_kl_holds_the_policy_back():
         with torch.no_grad():
             moved.append(float((L.policy_net(b.states.reshape(-1, 617))[0] - before).pow(2).mean()))
     assert moved[1] < moved[0]
+
+
+@gpu
+def test_train_script_with_the_new_options(tmp_path):
+    """scripts/train_hand_mimic.py --optimizer / --kl_coef: two iterations each way, checkpoint"""
+    import importlib.util
+    import os
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("train_hand_mimic", os.path.join(ROOT, "scripts", "train_hand_mimic.py"))
+    mod = importlib.util.module_from_spec(spec); spec.loader.exec_module(mod)
+    base = ["--cfg", "box_future5_light_add_geom", "--num_threads", "16", "--no_log", "--num_epoch", "2", "--base_dir", str(tmp_path)]
+    for more, bits in ((["--n_envs", "128", "--optimizer", "AdamW8bit", "--kl_coef", "0.2"], 8), (["--sample_mode", "episodes", "--optimizer", "AdamW"], 32)):
+        agent = mod.main(base + more)
+        assert type(agent.optimizer_policy) is optim.AdamW and agent.optimizer_value.defaults["state_bits"] == bits
+        assert agent.learner.kl_coef == (0.2 if bits == 8 else 0.0) and agent.epoch == 1
+        assert all(bool(torch.isfinite(p).all()) for p in agent.policy_net.parameters())
+        assert agent.optimizer_policy.param_groups[0]["lr"] == float(agent.cfg.adp_policy_lr)
+        agent.save_checkpoint(1)
+        agent.env.close()
