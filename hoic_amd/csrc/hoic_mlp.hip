@@ -1625,7 +1625,7 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
         for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
         if ((threadIdx.x & 63) == 0) wcount[threadIdx.x >> 6] = c;
         __syncthreads();
-        n = (double)(wcount[0] + wcount[1] + wcount[2] + wcount[3]);
+        n = ((double)wcount[0] + (double)wcount[1]) + ((double)wcount[2] + (double)wcount[3]);
       }
     }
     scale = a.weight * (a.upstream ? (double)*a.upstream : 1.) / (n > 0. ? n : 1.);
@@ -2353,9 +2353,9 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
   }
   for (int i = 0; i < nt; i++) {
     const hoic_adamw_tensor& e = t[i];
-    if (e.n < 0 || (e.n > 0 && (!e.p || !e.g || !e.m || !e.v || (x->state_bits == 8 && (!e.m_scale || !e.v_scale)))) || (x->d_consts ? !e.d_step : e.step < 1)
+    if (e.n < 0 || (e.n > 0 && (!e.p || !e.g || !e.m || !e.v || (x->state_bits == 8 && (!e.m_scale || !e.v_scale || ((uintptr_t)e.m | (uintptr_t)e.v) & 3)))) || (x->d_consts ? !e.d_step : e.step < 1)
         || (e.n + ADAM32_CHUNK - 1) / ADAM32_CHUNK > 0x7fffffff / ADAM_MAX) {
-      hoic_set_error("hoic_adamw: a tensor without memory, state or step count, or too large"); return HOIC_ERR_ARG;
+      hoic_set_error("hoic_adamw: a tensor without memory, state (8-bit: aligned to 4 bytes) or step count, or too large"); return HOIC_ERR_ARG;
     }
   }
   static_assert(ADAM8_CHUNK == ADAM32_CHUNK, "one chunk size for the launch below");
@@ -2409,7 +2409,7 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
 extern "C" int32_t hoic_adamw_values(const hoic_adamw_tensor* t, int32_t nt, void* stream) {
   if (nt < 0 || (nt > 0 && !t)) { hoic_set_error("hoic_adamw_values: bad list"); return HOIC_ERR_ARG; }
   for (int i = 0; i < nt; i++)
-    if (t[i].n < 0 || (t[i].n > 0 && (!t[i].p || !t[i].g || !t[i].m || !t[i].v || !t[i].m_scale || !t[i].v_scale)) || (t[i].n + ADAM8_CHUNK - 1) / ADAM8_CHUNK > 0x7fffffff / ADAM_MAX) {
+    if (t[i].n < 0 || (t[i].n > 0 && (!t[i].p || !t[i].g || !t[i].m || !t[i].v || !t[i].m_scale || !t[i].v_scale || ((uintptr_t)t[i].m | (uintptr_t)t[i].v) & 3)) || (t[i].n + ADAM8_CHUNK - 1) / ADAM8_CHUNK > 0x7fffffff / ADAM_MAX) {
       hoic_set_error("hoic_adamw_values: a tensor without memory, or too large"); return HOIC_ERR_ARG;
     }
   AdamArgs a;

@@ -107,6 +107,8 @@ def clip_grad_norm_(parameters, max_norm):
     if not grads:
         return torch.zeros(())
     args, parts = _tensor_list(grads, "clip_grad_norm_")
+    if len({p for p, n in zip(args[0], args[1]) if n}) < sum(1 for n in args[1] if n):
+        raise ValueError("clip_grad_norm_: two gradients in the same memory (each would be scaled twice)")
     dev = grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=dev)
     if parts == 0:
@@ -157,8 +159,12 @@ class AdamW(torch.optim.Optimizer):
         for key in ("state_bits", "capturable"):
             if group.get(key, self.defaults[key]) != self.defaults[key]:
                 raise ValueError(f"{key} is one for all groups")
+        memory = {p.data_ptr() for g in self.param_groups for p in g["params"]}
         for p in ps:
             _check(p, "AdamW")
+            if p.numel() and p.data_ptr() in memory:
+                raise ValueError("AdamW: two parameters in the same memory")
+            memory.add(p.data_ptr())
             if not _dense(p):
                 raise ValueError("AdamW: a parameter whose elements do not fill their memory (an expanded or cut view)")
         super().add_param_group(group)

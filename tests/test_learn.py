@@ -173,6 +173,17 @@ def test_policy_loss_strides_and_expanded_rows():
     x = {**base, **{k: base[k].t().contiguous().t() for k in ("mean", "actions", "log_std", "ref_mean", "ref_log_std")}}
     for a, b in zip(check_loss(x)[:4], want[:4]):
         assert torch.equal(a, b)
+    # four dimensions a load at every alignment of a type, a mask that starts anywhere
+    for dt, at in ((torch.float32, 1), (torch.bfloat16, 1), (torch.float16, 3)):
+        b = loss_case(150, 8, mask=0.3, per_row=True, seed=21, device="cuda")
+        for k in ("mean", "actions", "ref_mean"):
+            b[k] = b[k].to(dt)
+        cut = lambda t: torch.nn.functional.pad(t, (at, 2))[:, at:at + t.shape[1]]
+        shift = lambda t: torch.cat([t[:at], t])[at:]
+        y = {**b, **{k: cut(b[k]) for k in ("mean", "actions", "log_std", "ref_mean", "ref_log_std")}, "valid": shift(b["valid"]), "advantages": shift(b["advantages"])}
+        assert y["mean"].data_ptr() % 16 and y["valid"].data_ptr() % 4
+        for a, c in zip(rl.clipped_policy_loss_grad(**y, kl_coef=0.3)[:4], rl.clipped_policy_loss_grad(**b, kl_coef=0.3)[:4]):
+            assert torch.equal(a, c)
     one = {**base, "mean": base["mean"][:1].expand(200, 9), "log_std": base["log_std"][:1].expand(200, 9)}
     check_loss(one)
 
@@ -388,6 +399,22 @@ def test_grad_norm_of_mixed_types_strides_and_values():
     assert math.isinf(float(n)) and math.isinf(float(m)) and torch.equal(torch.isnan(p.grad), torch.isnan(q.grad)) and float(p.grad[0]) == float(q.grad[0]) == 0
     assert float(optim.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3, device="cuda"))], 1.0)) == 0      # no gradient anywhere
     assert float(optim.grad_norm([torch.zeros(0, device="cuda")])) == 0
+    flat = torch.randn(1000, device="cuda")
+    twice = [torch.nn.Parameter(torch.zeros(500, device="cuda")) for _ in range(2)]
+    for p in twice:
+        p.grad = flat[3:503]
+    with pytest.raises(ValueError, match="same memory"):
+        optim.clip_grad_norm_(twice, 1.0)
+    with pytest.raises(ValueError, match="fill their memory"):
+        twice[0].grad = flat[::2]
+        optim.clip_grad_norm_(twice[:1], 1.0)
+    # views of one buffer at odd offsets, as a network's gradients in a bucket
+    want = float(flat[1:].double().norm())
+    for p, (i, j) in zip(twice, ((1, 501), (501, 1000))):
+        p.data = torch.zeros(j - i, device="cuda"); p.grad = flat[i:j]
+    first = flat.clone()
+    assert abs(float(optim.clip_grad_norm_(twice, 0.5 * want)) - want) <= (U32 + 1e-12) * want
+    assert float(flat[0]) == float(first[0]) and bool(((flat[1:] - 0.5 * first[1:]).abs() <= (4 * U32 + 1e-6 / want) * first[1:].abs()).all())
 
 
 def test_norm_refusals():
@@ -868,6 +895,56 @@ def test_adamw_refuses_what_it_cannot_hold():
     assert not opt.state[p]
     with pytest.raises(ValueError):
         opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(3, device="cuda"))], state_bits=8))
+    with pytest.raises(ValueError, match="same memory"):
+        optim.AdamW([torch.nn.Parameter(p.data), torch.nn.Parameter(p.data)])
+    with pytest.raises(ValueError, match="same memory"):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(p.data)]))
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_hooks_closure_scheduler_and_profiler(bits):
+    """what a torch optimiser offers around its step keeps working"""
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = optim.AdamW([p], lr=1e-2, state_bits=bits)
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, 0.5)
+    seen = []
+    opt.register_step_pre_hook(lambda o, a, k: seen.append("pre")); opt.register_step_post_hook(lambda o, a, k: seen.append("post"))
+    def closure():
+        opt.zero_grad()
+        loss = (p ** 2).sum()
+        loss.backward()
+        return loss
+    assert float(opt.step(closure, max_norm=1.0).detach()) == 300.0 and seen == ["pre", "post"] and float(opt.grad_norm) > 0
+    sched.step()
+    assert opt.param_groups[0]["lr"] == 5e-3
+    with torch.autograd.profiler.profile():
+        opt.step(closure)
+    assert seen == ["pre", "post"] * 2 and opt.grad_norm is None and opt.state[p]["step"] == 2
+    opt.zero_grad(set_to_none=True)
+    before = p.detach().clone()
+    opt.step(max_norm=1.0)                                       # nothing to do
+    assert torch.equal(before, p.detach()) and float(opt.grad_norm) == 0 and opt.state[p]["step"] == 2
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_unaligned_views_and_a_side_stream(bits):
+    """parameters and gradients that are views at odd offsets of one buffer, stepped on another stream: the same bits as aligned copies"""
+    for dt in (torch.float32, torch.bfloat16):
+        flat, grad = tensor_list([20000], dt, 1)[0], tensor_list([20000], dt, 2)[0]
+        cuts = [(1, 4098), (4099, 9000), (9001, 9002), (9003, 19999)]
+        ps = [torch.nn.Parameter(flat[i:j]) for i, j in cuts]; qs = [torch.nn.Parameter(flat[i:j].clone()) for i, j in cuts]
+        for p, q, (i, j) in zip(ps, qs, cuts):
+            p.grad, q.grad = grad[i:j], grad[i:j].clone()
+        edges = flat[[0, 4098, 9000, 9002, 19999]].clone()
+        a, b = optim.AdamW(ps, **HYP, state_bits=bits), optim.AdamW(qs, **HYP, state_bits=bits)
+        st = torch.cuda.Stream(); st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            a.step(max_norm=1.0); a.step()
+        torch.cuda.current_stream().wait_stream(st)
+        b.step(max_norm=1.0); b.step()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and torch.equal(flat[[0, 4098, 9000, 9002, 19999]], edges)
 
 
 def test_rounding_bits_are_uniform():
