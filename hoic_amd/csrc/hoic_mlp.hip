@@ -2105,7 +2105,7 @@ __device__ __forceinline__ unsigned wave_max(unsigned x) {
 #undef DPP_MAX
   return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
-#define ADAM32_CHUNK 4096
+#define ADAM32_CHUNK 2048
 #define JOIN_BLOCKS 4096         // a launch of more workgroups is given the joined factor
 template <class T> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
@@ -2185,7 +2185,7 @@ __device__ __forceinline__ unsigned code8(double a, double r, int up, int low, u
   q = y > 0. && (Y_DOWN >> (ey + 14)) & 1 ? nudge(q, -1) : q;
   return (unsigned)(q + u) + (unsigned)(ey - low) * 8u;
 }
-#define ADAM8_CHUNK 4096
+#define ADAM8_CHUNK 2048
 // One block of 256 elements from element i0 + ob on in the tensor form's arithmetic (a wavefront): blocks in which a value lies next to a
 // border or is not finite.
 template <class T> __device__ __forceinline__ void adam8_block(const AdamArgs& a, int t, const AdamConsts& c, double cl, unsigned key, long long i0, long long ob, long long left,

@@ -359,7 +359,10 @@ def clipped_policy_loss(mean, log_std, actions, advantages, fixed_log_probs=None
     float32; ``valid`` [M] bool: rows outside it take no part, whatever they hold.  ``fixed_log_probs`` None: the old policy
     is this one (ratio 1), the log-probabilities come back for the later epochs.  ``clip_epsilon``: eps, or (lower, upper).
     On the GPU one pass over the batch for the value and one for the gradient (hoic_policy_loss), per-row arithmetic and sums in
-    64 bits in a fixed order; CPU and float64 tensors take the tensor form.  Returns a ``PolicyLoss``."""
+    64 bits in a fixed order; CPU and float64 tensors take the tensor form.  Returns a ``PolicyLoss``.
+
+    Under graph capture take ``clipped_policy_loss_grad``, or ``torch.autograd.grad`` on tensors made for the captured graph: a captured
+    ``backward()`` into leaves that an eager graph elsewhere still holds ends the process inside the autograd engine."""
     x = _loss_inputs(mean, log_std, actions, advantages, fixed_log_probs, clip_epsilon, ref_mean, ref_log_std, kl_coef, valid)
     if not _on_kernel(mean):
         return _policy_loss_tensors(x, kl_coef)

@@ -292,6 +292,30 @@ def test_policy_loss_on_a_side_stream_and_in_a_graph():
         torch.cuda.synchronize()
         e = rl.clipped_policy_loss_grad(**{**x, "mean": mu.detach()}, kl_coef=0.3, weight=2.0)
         assert torch.equal(p.loss, e.loss) and torch.equal(gm, e.d_mean) and torch.equal(gs, e.d_log_std) and torch.equal(p.info, e.info), rep
+    # the one-pass form with its count of the valid rows, beside the norm and the clipping of what it made
+    grads = [torch.nn.Parameter(torch.zeros_like(x["mean"])), torch.nn.Parameter(torch.zeros_like(x["log_std"]))]
+    for p_ in grads:
+        p_.grad = torch.zeros_like(p_)
+    second = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(second):
+        o = rl.clipped_policy_loss_grad(**{**x, "mean": mu.detach()}, kl_coef=0.3, weight=100.0)
+        grads[0].grad.copy_(o.d_mean); grads[1].grad.copy_(o.d_log_std)
+        norm = optim.clip_grad_norm_(grads, 0.5)
+        after = optim.grad_norm([p_.grad for p_ in grads])
+    for rep in range(4):
+        x["valid"].copy_(torch.rand(3000, device="cuda") < 0.2 * (rep + 1))
+        x["mean"].nan_to_num_(0.0); x["actions"].nan_to_num_(0.0, 0.0, 0.0); x["advantages"].nan_to_num_(0.0, 0.0, 0.0); x["fixed_log_probs"].nan_to_num_(-10.0)
+        with torch.no_grad():
+            mu.copy_(x["mean"]).add_(0.01 * rep)
+        second.replay(); graph.replay()                   # (two graphs of the same operators, one after the other)
+        torch.cuda.synchronize()
+        e = rl.clipped_policy_loss_grad(**{**x, "mean": mu.detach()}, kl_coef=0.3, weight=100.0)
+        assert torch.equal(o.loss, e.loss) and torch.equal(o.info, e.info) and torch.equal(o.d_mean, e.d_mean) and torch.equal(o.d_log_std, e.d_log_std), rep
+        total = float(optim.grad_norm([e.d_mean, e.d_log_std]))
+        # (rows that were padding are valid now, their reference means at float32's lowest value: where the norm is not finite, what was
+        #  scaled by 0 is NaN in the infinite places)
+        assert float(norm) == total and total > 0.5, rep
+        assert abs(float(after) - 0.5) <= 0.5 * (1e-6 / 0.5 + 8 * U32) if math.isfinite(total) else math.isnan(float(after)), rep
 
 
 @gpu
