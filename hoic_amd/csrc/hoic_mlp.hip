@@ -1933,13 +1933,14 @@ __global__ __launch_bounds__(256) void hoic_norm_finish_kernel(Joint j, double* 
   if (threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
 }
 // g *= factor where it is not 1
-struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; Joint clip; };
-template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, const Joint& clip) {
+struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; Joint clip; const float* factor; };      // factor: in the place of the clipping one
+template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, const Joint& clip, const float* factor) {
   typedef WideStep<T> W;
   W w;
+  if (factor && *factor == 1.f) return;
   long long i = i0 + threadIdx.x * W::N;
   w.load(g, i, i1);                            // (on their way while the norm is joined)
-  const double f = join_norm(clip).y;
+  const double f = factor ? (double)*factor : join_norm(clip).y;
   if (f == 1.) return;
   const float c = (float)f;
   while (true) {
@@ -1957,9 +1958,9 @@ template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0
 __global__ __launch_bounds__(256) void hoic_scale_kernel(ScaleArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * a.chunk, i1 = i0 + a.chunk < a.t[t].n ? i0 + a.chunk : a.t[t].n;
-  if (a.type == HOIC_F32) scale_list((float*)a.t[t].g, i0, i1, a.clip);
-  else if (a.type == HOIC_F16) scale_list((_Float16*)a.t[t].g, i0, i1, a.clip);
-  else scale_list((__bf16*)a.t[t].g, i0, i1, a.clip);
+  if (a.type == HOIC_F32) scale_list((float*)a.t[t].g, i0, i1, a.clip, a.factor);
+  else if (a.type == HOIC_F16) scale_list((_Float16*)a.t[t].g, i0, i1, a.clip, a.factor);
+  else scale_list((__bf16*)a.t[t].g, i0, i1, a.clip, a.factor);
 }
 // elements a workgroup: whole steps, or one of 8192 in lists too short to fill the chip otherwise; at most ~1024 workgroups (= parts) a list
 // beyond one per tensor
@@ -2039,9 +2040,23 @@ extern "C" int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8
   hipStream_t st = (hipStream_t)stream;
   norm_partial((const void* const*)g, n, type, nt, d_buf + 2, st);
   ScaleArgs a;
+  a.factor = nullptr;
   a.clip = norm_join(d_buf, np, bound, d_norm, false, st);
   norm_launches(a, (const void* const*)g, n, type, nt, [&](long long blocks) {
     hipLaunchKernelGGL(hoic_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  });
+  MCHK(hipGetLastError());
+  return HOIC_OK;
+}
+
+extern "C" int32_t hoic_scale_list(void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, const float* d_factor, void* stream) {
+  const int32_t rc = norm_check("hoic_scale_list", (const void* const*)g, n, type, nt);
+  if (rc != HOIC_OK) return rc;
+  if (!d_factor || hoic_grad_norm_parts(n, nt) > 0x7fffffff) { hoic_set_error("hoic_scale_list: no factor, or too large a list"); return HOIC_ERR_ARG; }
+  ScaleArgs a;
+  a.factor = d_factor; a.clip = Joint{nullptr, 0, 0., nullptr};
+  norm_launches(a, (const void* const*)g, n, type, nt, [&](long long blocks) {
+    hipLaunchKernelGGL(hoic_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
   });
   MCHK(hipGetLastError());
   return HOIC_OK;

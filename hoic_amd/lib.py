@@ -53,7 +53,7 @@ EXPORTS = ["hoic_create", "hoic_destroy", "hoic_num_envs", "hoic_obs_dim", "hoic
            "hoic_mlp_colsum_packed", "hoic_mlp_amax_colsum", "hoic_mlp_colpart_finish", "hoic_mlp_update_exps_rel", "hoic_mlp_pack_tiled", "hoic_mlp_forward_tiled",
            "hoic_set_async_reward", "hoic_sync_rewards", "hoic_set_cu_reserve", "hoic_mlp_head", "hoic_mlp_head_backward", "hoic_mlp_ppo_loss",
            "hoic_mlp_value_loss", "hoic_policy_loss", "hoic_policy_loss_scratch_bytes", "hoic_grad_norm_parts", "hoic_grad_norm",
-           "hoic_grad_norm_partial", "hoic_clip_grads", "hoic_adamw", "hoic_adamw_values"]
+           "hoic_grad_norm_partial", "hoic_scale_list", "hoic_clip_grads", "hoic_adamw", "hoic_adamw_values"]
 
 
 def build(force: bool = False) -> str:
@@ -131,6 +131,7 @@ def load():
         L.hoic_grad_norm_parts.restype = C.c_int64
         L.hoic_grad_norm.argtypes = [vp, vp, vp, i32, vp, vp, vp]
         L.hoic_grad_norm_partial.argtypes = [vp, vp, vp, i32, vp, vp]
+        L.hoic_scale_list.argtypes = [vp, vp, vp, i32, vp, vp]
         L.hoic_clip_grads.argtypes = [vp, vp, vp, i32, C.c_double, vp, vp, vp]
         L.hoic_adamw.argtypes = [vp, i32, vp, vp]       # the list: n x 10 int64 (hoic_adamw_tensor is 80 bytes of 8-byte fields)
         L.hoic_adamw_values.argtypes = [vp, i32, vp]

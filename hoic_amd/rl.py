@@ -253,7 +253,7 @@ def _loss_inputs(mean, log_std, actions, advantages, fixed, clip_epsilon, ref_me
     return mean, log_std, actions, advantages, fixed, (float(lo), float(hi)), ref_mean, ref_log_std, valid
 
 
-def _policy_loss_launch(x, kl_coef, weight, grad, upstream=None, count=None):
+def _policy_loss_launch(x, kl_coef, weight, grad, upstream=None, count=None, want_count=False):
     """hoic_policy_loss on checked inputs -> (loss, info, n as float64 [1], d_mean, d_log_std [1 or M, N], log_probs).  ``count``: the n of
     an earlier call, for the gradient alone (loss, info and n are then None)."""
     mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid = x
@@ -264,7 +264,7 @@ def _policy_loss_launch(x, kl_coef, weight, grad, upstream=None, count=None):
     loss = info = n = log_probs = None
     if count is None:
         loss, info = advantages.new_empty(()), advantages.new_empty(4)
-        if not grad:
+        if want_count:
             n = advantages.new_empty(1, dtype=torch.float64)
         if fixed is None:
             log_probs = advantages.new_empty((M, 1))
@@ -291,15 +291,19 @@ def _policy_loss_launch(x, kl_coef, weight, grad, upstream=None, count=None):
 
 
 class _ClippedPolicyLoss(torch.autograd.Function):
-    """Value in the forward call; the backward call makes the gradients from the same inputs, scaled by the incoming one on the
-    device (a gradient made in the forward call would have to be written, read and written again)."""
+    """float32 means: one pass over the batch makes value and gradients; the backward call multiplies them by the incoming gradient where
+    that is not 1 (on the device; nothing is read or written for ``loss.backward()``).  16-bit means, and a second backward call: the
+    gradients are made by a pass of their own, scaled before their one rounding (a float16 gradient of a mean over thousands of
+    rows would underflow unscaled)."""
 
     @staticmethod
     def forward(ctx, kl_coef, clip, mean, log_std, *rest):
         actions, advantages, fixed, ref_mean, ref_log_std, valid = rest
-        loss, info, ctx.count, _, _, log_probs = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0, False)
+        x = (mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid)
+        grad = (ctx.needs_input_grad[2] or ctx.needs_input_grad[3]) and mean.dtype == torch.float32
+        loss, info, ctx.count, d_mean, d_log_std, log_probs = _policy_loss_launch(x, kl_coef, 1.0, grad, want_count=True)
         ctx.save_for_backward(mean, log_std, *rest)
-        ctx.consts = (kl_coef, clip)
+        ctx.consts, ctx.grads = (kl_coef, clip), (d_mean, d_log_std) if grad else None
         ctx.mark_non_differentiable(*((info,) if log_probs is None else (info, log_probs)))
         return loss, info, log_probs
 
@@ -307,9 +311,21 @@ class _ClippedPolicyLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, *_):
         mean, log_std, actions, advantages, fixed, ref_mean, ref_log_std, valid = ctx.saved_tensors
-        kl_coef, clip = ctx.consts
-        *_, d_mean, d_log_std, _ = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0,
-                                                      True, upstream=g.float().contiguous(), count=ctx.count)
+        g = g.float().contiguous()
+        if ctx.grads is not None:
+            (d_mean, d_log_std), ctx.grads = ctx.grads, None
+            if mean.shape[0]:
+                L = lib.load()
+                import ctypes as C
+                with lib.Launch(mean.device) as st:
+                    rc = L.hoic_scale_list((C.c_void_p * 2)(d_mean.data_ptr(), d_log_std.data_ptr()), (C.c_int64 * 2)(d_mean.numel(), d_log_std.numel()), bytes(2), 2,
+                                           g.data_ptr(), st)
+                if rc != 0:
+                    raise lib.HoicError(f"hoic_scale_list failed ({rc}): {L.hoic_last_error().decode()}")
+        else:
+            kl_coef, clip = ctx.consts
+            *_, d_mean, d_log_std, _ = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0,
+                                                           True, upstream=g, count=ctx.count)
         return (None, None, d_mean, d_log_std) + (None,) * 6
 
 
@@ -358,8 +374,8 @@ def clipped_policy_loss(mean, log_std, actions, advantages, fixed_log_probs=None
     gradient is summed) or [M, N], float32 or the mean's type, ref_log_std alike; advantages, fixed_log_probs [M] or [M, 1]
     float32; ``valid`` [M] bool: rows outside it take no part, whatever they hold.  ``fixed_log_probs`` None: the old policy
     is this one (ratio 1), the log-probabilities come back for the later epochs.  ``clip_epsilon``: eps, or (lower, upper).
-    On the GPU one pass over the batch for the value and one for the gradient (hoic_policy_loss), per-row arithmetic and sums in
-    64 bits in a fixed order; CPU and float64 tensors take the tensor form.  Returns a ``PolicyLoss``.
+    On the GPU one pass over the batch for value and gradient of float32 means, one each for 16-bit ones (hoic_policy_loss); per-row
+    arithmetic and sums in 64 bits in a fixed order; CPU and float64 tensors take the tensor form.  Returns a ``PolicyLoss``.
 
     Under graph capture take ``clipped_policy_loss_grad``, or ``torch.autograd.grad`` on tensors made for the captured graph: a captured
     ``backward()`` into leaves that an eager graph elsewhere still holds ends the process inside the autograd engine."""

@@ -382,10 +382,12 @@ int32_t hoic_policy_loss(const hoic_policy_loss_args* a, void* stream);
  * order.  d_buf: hoic_grad_norm_parts(n, nt) + 2 doubles of scratch; d_norm: the norm in float32.
  * hoic_grad_norm: the norm; d_buf[0..1] = {norm, 1} afterwards.
  * hoic_grad_norm_partial: the parts alone, for hoic_adamw (d_norm_buf, norm_parts) to join.
+ * hoic_scale_list: g *= *d_factor (device float; 1 touches nothing).
  * hoic_clip_grads: g *= min(1, bound / (norm + 1e-6)) in place (a factor of 1 touches nothing). */
 int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt);
 int32_t hoic_grad_norm(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* d_buf, float* d_norm, void* stream);
 int32_t hoic_grad_norm_partial(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* d_buf, void* stream);
+int32_t hoic_scale_list(void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, const float* d_factor, void* stream);
 int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double bound, double* d_buf, float* d_norm, void* stream);
 /* hoic_adamw: one AdamW step over nt tensors of one type (in the place of the optimiser step of agent_ppo.py:46-56 / agent_pg.py:18-25;
  * list in HOST memory).  m' = b1 m + (1 - b1) c g, v' = b2 v + (1 - b2) (c g)^2, p' = p - (lr wd p + lr / (1 - b1^t) m' / (sqrt(v' / (1 - b2^t))

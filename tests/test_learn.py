@@ -251,6 +251,35 @@ def test_policy_loss_gradient_against_differences():
 
 
 @gpu
+@pytest.mark.parametrize("mean", ["f32", "bf16"])
+def test_policy_loss_backward_twice_and_in_part(mean):
+    """a graph kept for a second backward call, gradients taken over by the leaves and changed there, one input without gradient"""
+    x = loss_case(300, 8, mean, mask=0.3, seed=30, device="cuda")
+    ref = loss_reference(x, kl_coef=0.3)
+    mu, s = x["mean"].detach().requires_grad_(), x["log_std"].detach().requires_grad_()
+    p = rl.clipped_policy_loss(**{**x, "mean": mu, "log_std": s}, kl_coef=0.3)
+    p.loss.backward(retain_graph=True)
+    close(mu.grad, ref["d_mean"], "first"); close(s.grad, ref["d_log_std"], "first", 1e-12 * float(ref["terms"]))
+    mu.grad.zero_(); s.grad.fill_(7.0)
+    g = torch.autograd.grad(p.loss, (mu, s), grad_outputs=torch.tensor(4.0, device="cuda"), retain_graph=True)
+    for a, k in zip(g, ("d_mean", "d_log_std")):
+        close(a, 4 * ref[k], "second", 1e-11 * float(ref["terms"]))
+    (2.0 * p.loss + 1.0).backward()
+    close(mu.grad, 2 * ref["d_mean"], "third")
+    for only in ("mean", "log_std"):
+        leaf = x[only].detach().requires_grad_()
+        rl.clipped_policy_loss(**{**x, only: leaf}, kl_coef=0.3).loss.backward()
+        close(leaf.grad, ref["d_" + only], only, 1e-12 * float(ref["terms"]))
+    with torch.no_grad():
+        assert not rl.clipped_policy_loss(**{**x, "mean": mu}, kl_coef=0.3).loss.requires_grad
+    q = rl.clipped_policy_loss(**{**x, "mean": mu}, kl_coef=0.3)
+    with torch.no_grad():
+        mu.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        q.loss.backward()
+
+
+@gpu
 def test_policy_loss_matches_the_existing_losses():
     """kl_coef 0: rl.ppo_loss on the CPU in float64, and the fused head step's loss kernel's gradient, on the learner's own shapes"""
     x = loss_case(1000, 32, ref=False, seed=18, device="cuda")
@@ -463,6 +492,7 @@ def test_norm_refusals():
     for n, norm, bound in ((one, None, 1.0), (none, 8, 1.0), (one, 8, -1.0), (one, 8, math.nan)):
         assert L.hoic_clip_grads(some, n, b"\0", 1, bound, 8, norm, None) == -1
     assert L.hoic_grad_norm(some, none, b"\0", 1, 8, 8, None) == -1
+    assert L.hoic_scale_list(some, one, b"\0", 1, None, None) == -1 and L.hoic_scale_list(null, one, b"\0", 1, 8, None) == -1
 
 
 # ================================================================================================ AdamW
