@@ -8,6 +8,7 @@ and the PPO-clip loss (uhc/khrylib/rl/agents/agent_ppo.py:58-64).
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 from typing import NamedTuple
 
@@ -129,7 +130,6 @@ def estimate_advantages(rewards, masks, values, gamma, tau, next_values=None, di
     if valid is None and dist_group is None and adv.is_cuda and adv.dtype == torch.float32 and adv.is_contiguous() and adv.numel() >= 2:
         L = lib.load()
         if hasattr(L, "hoic_normalize_advantages"):      # two launches (float64 sums in a fixed order) instead of ~15 tensor kernels
-            import ctypes as C
             scratch = torch.empty(512, dtype=torch.float64, device=adv.device)
             with torch.cuda.device(adv.device):
                 rc = L.hoic_normalize_advantages(adv.numel(), C.c_void_p(adv.data_ptr()), C.c_void_p(scratch.data_ptr()),
@@ -152,7 +152,6 @@ def estimate_advantages(rewards, masks, values, gamma, tau, next_values=None, di
 
 
 def _gae_device(rewards, masks, values, gamma, tau, next_values):
-    import ctypes as C
     L = lib.load()
     f = lambda x: x.to(torch.float32).contiguous()
     rewards, masks, values = f(rewards), f(masks), f(values)
@@ -301,7 +300,7 @@ class _ClippedPolicyLoss(torch.autograd.Function):
         actions, advantages, fixed, ref_mean, ref_log_std, valid = rest
         x = (mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid)
         grad = (ctx.needs_input_grad[2] or ctx.needs_input_grad[3]) and mean.dtype == torch.float32
-        loss, info, ctx.count, d_mean, d_log_std, log_probs = _policy_loss_launch(x, kl_coef, 1.0, grad, want_count=True)
+        loss, info, ctx.count, d_mean, d_log_std, log_probs = _policy_loss_launch(x, kl_coef, 1.0, grad, want_count=not grad)
         ctx.save_for_backward(mean, log_std, *rest)
         ctx.consts, ctx.grads = (kl_coef, clip), (d_mean, d_log_std) if grad else None
         ctx.mark_non_differentiable(*((info,) if log_probs is None else (info, log_probs)))
@@ -316,7 +315,6 @@ class _ClippedPolicyLoss(torch.autograd.Function):
             (d_mean, d_log_std), ctx.grads = ctx.grads, None
             if mean.shape[0]:
                 L = lib.load()
-                import ctypes as C
                 with lib.Launch(mean.device) as st:
                     rc = L.hoic_scale_list((C.c_void_p * 2)(d_mean.data_ptr(), d_log_std.data_ptr()), (C.c_int64 * 2)(d_mean.numel(), d_log_std.numel()), bytes(2), 2,
                                            g.data_ptr(), st)
@@ -383,7 +381,7 @@ def clipped_policy_loss(mean, log_std, actions, advantages, fixed_log_probs=None
     if not _on_kernel(mean):
         return _policy_loss_tensors(x, kl_coef)
     mean2, log_std2, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid = x
-    const = [None if t is None else t.detach() for t in (actions, advantages, fixed, ref_mean, ref_log_std, valid)]
+    const = [t.detach() if t is not None and t.requires_grad else t for t in (actions, advantages, fixed, ref_mean, ref_log_std, valid)]
     return PolicyLoss(*_ClippedPolicyLoss.apply(float(kl_coef), clip, mean2, log_std2, *const))
 
 
@@ -510,7 +508,6 @@ class BatchZFilter:
         if self._st.is_cuda and 0 < len(forks) <= 8 and all(f._st.is_cuda and f.dim == self.dim for f in forks):
             # one launch (hoic_zfilter_absorb) instead of ~35 float64 tensor operations per fork: bit-identical statistics
             from . import lib
-            import ctypes as C
             L = lib.load()
             if hasattr(L, "hoic_zfilter_absorb"):
                 if self._alt is None:
@@ -550,7 +547,6 @@ class BatchZFilter:
         hoic_amd.mlp.TiledForward engine whose operand the normalised rows are), hoic_zfilter_tiled: the second launch also writes
         the engine's operand and refreshes its delayed exponents (bit-identical states and filter; two launches instead of four)."""
         from . import lib
-        import ctypes as C
         L = lib.load()
         x = x.contiguous()
         n = x.shape[0]
