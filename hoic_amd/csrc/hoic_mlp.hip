@@ -1478,11 +1478,14 @@ template <> struct vec4<float> { typedef f4u type; };
 template <> struct vec4<_Float16> { typedef h4u type; };
 template <> struct vec4<__bf16> { typedef b4u type; };
 
+// NT: around the caches, for lists that would only push one another out of them (STREAM_BYTES below)
+template <bool NT, class V> __device__ __forceinline__ V load_as(const V* x) { return NT ? __builtin_nontemporal_load(x) : *x; }
+template <bool NT, class V> __device__ __forceinline__ void store_as(V* x, V v) { if (NT) __builtin_nontemporal_store(v, x); else *x = v; }
 // four elements from x on, of which the first `left` exist (the rest read as 0)
-template <class T> __device__ __forceinline__ f32x4 load4(const T* __restrict__ x, int left) {
+template <bool NT = false, class T> __device__ __forceinline__ f32x4 load4(const T* __restrict__ x, int left) {
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
   if (left >= 4) {
-    r = __builtin_convertvector(*(const typename vec4<T>::type*)x, f32x4);
+    r = __builtin_convertvector(load_as<NT>((const typename vec4<T>::type*)x), f32x4);
   } else {
     if (left > 0) r.x = (float)x[0];
     if (left > 1) r.y = (float)x[1];
@@ -1490,9 +1493,9 @@ template <class T> __device__ __forceinline__ f32x4 load4(const T* __restrict__ 
   }
   return r;
 }
-template <class T> __device__ __forceinline__ void store4(T* __restrict__ x, int left, f32x4 r) {
+template <bool NT = false, class T> __device__ __forceinline__ void store4(T* __restrict__ x, int left, f32x4 r) {
   if (left >= 4) {
-    *(typename vec4<T>::type*)x = __builtin_convertvector(r, typename vec4<T>::type);
+    store_as<NT>((typename vec4<T>::type*)x, __builtin_convertvector(r, typename vec4<T>::type));
   } else {
     if (left > 0) x[0] = (T)r.x;
     if (left > 1) x[1] = (T)r.y;
@@ -1878,10 +1881,10 @@ template <class T> struct WideStep {
   static constexpr int N = wide<T>::n, SPAN = 256 * N;          // elements of a load, of a workgroup's row of loads
   typename wide<T>::type x[8];
   // the lane's elements from i on, of which those below i1 exist (the rest read as 0)
-  __device__ __forceinline__ void load(const T* g, long long i, long long i1) {
+  template <bool NT> __device__ __forceinline__ void load(const T* g, long long i, long long i1) {
     if (i - threadIdx.x * N + 8 * SPAN <= i1) {
 #pragma unroll
-      for (int u = 0; u < 8; u++) x[u] = *(const typename wide<T>::type*)(g + i + u * SPAN);
+      for (int u = 0; u < 8; u++) x[u] = load_as<NT>((const typename wide<T>::type*)(g + i + u * SPAN));
     } else {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
@@ -1902,12 +1905,12 @@ template <class T> struct WideStep {
     }
   }
 };
-template <class T> __device__ __forceinline__ double sumsq(const T* g, long long i0, long long i1) {
+template <bool NT, class T> __device__ __forceinline__ double sumsq(const T* g, long long i0, long long i1) {
   typedef WideStep<T> W;
   double s = 0.;
   W w;
   for (long long i = i0 + threadIdx.x * W::N; i - threadIdx.x * W::N < i1; i += 8 * W::SPAN) {
-    w.load(g, i, i1);
+    w.template load<NT>(g, i, i1);
 #pragma unroll
     for (int u = 0; u < 8; u++) {
 #pragma unroll
@@ -1916,11 +1919,11 @@ template <class T> __device__ __forceinline__ double sumsq(const T* g, long long
   }
   return s;
 }
-__global__ __launch_bounds__(256) void hoic_sumsq_kernel(NormArgs a) {
+template <bool NT> __global__ __launch_bounds__(256) void hoic_sumsq_kernel(NormArgs a) {
   __shared__ double red[4];
   const int t = list_find(a.t, a.nt, blockIdx.x);
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * a.chunk, i1 = i0 + a.chunk < a.t[t].n ? i0 + a.chunk : a.t[t].n;
-  double s = a.type == HOIC_F32 ? sumsq((const float*)a.t[t].g, i0, i1) : a.type == HOIC_F16 ? sumsq((const _Float16*)a.t[t].g, i0, i1) : sumsq((const __bf16*)a.t[t].g, i0, i1);
+  double s = a.type == HOIC_F32 ? sumsq<NT>((const float*)a.t[t].g, i0, i1) : a.type == HOIC_F16 ? sumsq<NT>((const _Float16*)a.t[t].g, i0, i1) : sumsq<NT>((const __bf16*)a.t[t].g, i0, i1);
 #pragma unroll
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -1934,12 +1937,12 @@ __global__ __launch_bounds__(256) void hoic_norm_finish_kernel(Joint j, double* 
 }
 // g *= factor where it is not 1
 struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; Joint clip; const float* factor; };      // factor: in the place of the clipping one
-template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, const Joint& clip, const float* factor) {
+template <bool NT, class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, const Joint& clip, const float* factor) {
   typedef WideStep<T> W;
   W w;
   if (factor && *factor == 1.f) return;
   long long i = i0 + threadIdx.x * W::N;
-  w.load(g, i, i1);                            // (on their way while the norm is joined)
+  w.template load<NT>(g, i, i1);               // (on their way while the norm is joined)
   const double f = factor ? (double)*factor : join_norm(clip).y;
   if (f == 1.) return;
   const float c = (float)f;
@@ -1952,15 +1955,15 @@ template <class T> __device__ __forceinline__ void scale_list(T* g, long long i0
     w.store(g, i, i1);
     i += 8 * W::SPAN;
     if (i - threadIdx.x * W::N >= i1) break;
-    w.load(g, i, i1);
+    w.template load<NT>(g, i, i1);
   }
 }
-__global__ __launch_bounds__(256) void hoic_scale_kernel(ScaleArgs a) {
+template <bool NT> __global__ __launch_bounds__(256) void hoic_scale_kernel(ScaleArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * a.chunk, i1 = i0 + a.chunk < a.t[t].n ? i0 + a.chunk : a.t[t].n;
-  if (a.type == HOIC_F32) scale_list((float*)a.t[t].g, i0, i1, a.clip, a.factor);
-  else if (a.type == HOIC_F16) scale_list((_Float16*)a.t[t].g, i0, i1, a.clip, a.factor);
-  else scale_list((__bf16*)a.t[t].g, i0, i1, a.clip, a.factor);
+  if (a.type == HOIC_F32) scale_list<NT>((float*)a.t[t].g, i0, i1, a.clip, a.factor);
+  else if (a.type == HOIC_F16) scale_list<NT>((_Float16*)a.t[t].g, i0, i1, a.clip, a.factor);
+  else scale_list<NT>((__bf16*)a.t[t].g, i0, i1, a.clip, a.factor);
 }
 // elements a workgroup: whole steps, or one of 8192 in lists too short to fill the chip otherwise; at most ~1024 workgroups (= parts) a list
 // beyond one per tensor
@@ -1984,6 +1987,15 @@ extern "C" int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt) {
   for (int i = 0; i < nt; i++) p += (n[i] + chunk - 1) / chunk;
   return p;
 }
+// Lists of more bytes than the last-level cache holds go around the caches.  Measured on both sides of 256 MB: AdamW with 32-bit states
+// 69 (through the caches) against 78 us at 256 MB, 128 against 115 at 384, 705 against 654 at 2 GB; with 8-bit ones 77 / 76, 121 / 110,
+// 653 / 589; the norm 43 / 42, 73 / 62, 357 / 309.  (Clipping loads so and stores through the caches: 172 us for 537 MB, 212 with both.)
+#define STREAM_BYTES (256ll << 20)
+static long long list_bytes(const int64_t* n, const uint8_t* type, int32_t nt) {
+  long long b = 0;
+  for (int i = 0; i < nt; i++) b += n[i] * (type[i] == HOIC_F32 ? 4 : 2);
+  return b;
+}
 // launches over a list, type by type: f(entries so far, blocks) for every NORM_MAX of them
 template <class A, class F> static void norm_launches(A& a, const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, F launch) {
   a.chunk = norm_chunk(n, nt);
@@ -2002,9 +2014,18 @@ template <class A, class F> static void norm_launches(A& a, const void* const* g
 static void norm_partial(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* part, hipStream_t st) {
   NormArgs a;
   a.part = part;
+  const bool stream = list_bytes(n, type, nt) > STREAM_BYTES;
   norm_launches(a, g, n, type, nt, [&](long long blocks) {
-    hipLaunchKernelGGL(hoic_sumsq_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (stream) hipLaunchKernelGGL(hoic_sumsq_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(hoic_sumsq_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, st, a);
     a.part += blocks;
+  });
+}
+static void scale_launches(ScaleArgs& a, void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, hipStream_t st) {
+  const bool stream = list_bytes(n, type, nt) > STREAM_BYTES;
+  norm_launches(a, (const void* const*)g, n, type, nt, [&](long long blocks) {
+    if (stream) hipLaunchKernelGGL(hoic_scale_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(hoic_scale_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, st, a);
   });
 }
 // d_buf = {norm, factor, parts ...}; what a launch that uses the factor is given: the parts, or {norm, factor} after a join
@@ -2042,9 +2063,7 @@ extern "C" int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8
   ScaleArgs a;
   a.factor = nullptr;
   a.clip = norm_join(d_buf, np, bound, d_norm, false, st);
-  norm_launches(a, (const void* const*)g, n, type, nt, [&](long long blocks) {
-    hipLaunchKernelGGL(hoic_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
-  });
+  scale_launches(a, g, n, type, nt, st);
   MCHK(hipGetLastError());
   return HOIC_OK;
 }
@@ -2055,9 +2074,7 @@ extern "C" int32_t hoic_scale_list(void* const* g, const int64_t* n, const uint8
   if (!d_factor || hoic_grad_norm_parts(n, nt) > 0x7fffffff) { hoic_set_error("hoic_scale_list: no factor, or too large a list"); return HOIC_ERR_ARG; }
   ScaleArgs a;
   a.factor = d_factor; a.clip = Joint{nullptr, 0, 0., nullptr};
-  norm_launches(a, (const void* const*)g, n, type, nt, [&](long long blocks) {
-    hipLaunchKernelGGL(hoic_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
-  });
+  scale_launches(a, g, n, type, nt, (hipStream_t)stream);
   MCHK(hipGetLastError());
   return HOIC_OK;
 }
@@ -2122,7 +2139,7 @@ __device__ __forceinline__ unsigned wave_max(unsigned x) {
 }
 #define ADAM32_CHUNK 2048
 #define JOIN_BLOCKS 4096         // a launch of more workgroups is given the joined factor
-template <class T> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(AdamArgs a) {
+template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; float* m = (float*)a.t[t].m; float* v = (float*)a.t[t].v;
   const long long i0 = (long long)(blockIdx.x - a.t[t].first) * ADAM32_CHUNK, left = a.t[t].n - i0;
@@ -2134,7 +2151,7 @@ template <class T> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(Ad
   for (int u = 0; u < U; u++) {            // on their way while the norm is joined
     const long long i = i0 + u * 1024 + threadIdx.x * 4;
     const int l = whole ? 4 : count(u);
-    gg[u] = load4(g + i, l); mm[u] = load4(m + i, l); vv[u] = load4(v + i, l); pp[u] = load4(p + i, l);
+    gg[u] = load4<NT>(g + i, l); mm[u] = load4<NT>(m + i, l); vv[u] = load4<NT>(v + i, l); pp[u] = load4<NT>(p + i, l);
   }
   float cl = 1.f;
   if (a.clip.parts) {
@@ -2154,7 +2171,7 @@ template <class T> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(Ad
       vv[u][e] = fmaf(a.b2, vv[u][e], a.c2 * x * x);
       pp[u][e] = adam_param(pp[u][e], mm[u][e], vv[u][e], c, a.eps);
     }
-    store4(m + i, l, mm[u]); store4(v + i, l, vv[u]); store4(p + i, l, pp[u]);
+    store4<NT>(m + i, l, mm[u]); store4<NT>(v + i, l, vv[u]); store4<NT>(p + i, l, pp[u]);
   }
 }
 __device__ __forceinline__ unsigned hi32(double x) { return (unsigned)(__builtin_bit_cast(unsigned long long, x) >> 32); }
@@ -2252,7 +2269,7 @@ __device__ __forceinline__ unsigned code8_quick(double a, double r, int low, uns
   near = min(near, (t << 15) + 0x8000u);
   return (t >> 17) - (sub ? (unsigned)(1023 + low) * 8u : (unsigned)(1022 + low) * 8u);
 }
-template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(AdamArgs a) {
+template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; unsigned char* m = (unsigned char*)a.t[t].m; unsigned char* v = (unsigned char*)a.t[t].v;
   float* ms = a.t[t].ms; float* vs = a.t[t].vs;
@@ -2268,8 +2285,8 @@ template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(Ada
   for (int u = 0; u < U; u++) {
     const long long ob = (u * 4 + wave) * 256, i = i0 + ob + lane * 4;
     if (ob + 256 > left) continue;
-    pp[u] = load4(p + i, 4); gg[u] = load4(g + i, 4);
-    cm[u] = *(const unsigned*)(m + i); cv[u] = *(const unsigned*)(v + i);
+    pp[u] = load4<NT>(p + i, 4); gg[u] = load4<NT>(g + i, 4);
+    cm[u] = load_as<NT>((const unsigned*)(m + i)); cv[u] = load_as<NT>((const unsigned*)(v + i));
     km[u] = ms[(i0 + ob) >> 8]; kv[u] = vs[(i0 + ob) >> 8];
   }
   double cl = 1.;
@@ -2319,8 +2336,8 @@ template <class T> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(Ada
     f32x4 pu = pp[u];
 #pragma unroll
     for (int e = 0; e < 4; e++) pu[e] = adam_param(pu[e], mf[e], vf[e], c, a.eps);
-    *(unsigned*)(m + i) = om; *(unsigned*)(v + i) = ov;
-    store4(p + i, 4, pu);
+    store_as<NT>((unsigned*)(m + i), om); store_as<NT>((unsigned*)(v + i), ov);
+    store4<NT>(p + i, 4, pu);
     if (lane == 0) { ms[blk] = pow2f(em); vs[blk] = pow2f(ev); }
   }
   for (; again; again &= again - 1) adam8_block<T>(a, t, c, cl, key, i0, ((__ffs(again) - 1) * 4 + wave) * 256, left, lane);
@@ -2379,8 +2396,11 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
   a.b1 = (float)x->b1; a.c1 = (float)(1. - x->b1); a.b2 = (float)x->b2; a.c2 = (float)(1. - x->b2); a.eps = x->eps > 0. ? std::max((float)x->eps, 1.17549435e-38f) : 0.f; a.lrwd = (float)(x->lr * x->weight_decay);
   a.b1d = x->b1; a.c1d = 1. - x->b1; a.b2d = x->b2; a.c2d = 1. - x->b2; a.consts = x->d_consts;
   a.at = 0;
-  long long total = 0;
-  for (int i = 0; i < nt; i++) total += (t[i].n + ADAM32_CHUNK - 1) / ADAM32_CHUNK;
+  long long total = 0, bytes = 0;
+  for (int i = 0; i < nt; i++) {
+    total += (t[i].n + ADAM32_CHUNK - 1) / ADAM32_CHUNK;
+    bytes += t[i].n * ((x->type == HOIC_F32 ? 8 : 4) + x->state_bits / 4);          // p, g, m, v
+  }
   a.clip = Joint{nullptr, 0, 0., nullptr};
   if (x->d_norm_buf) a.clip = norm_join(x->d_norm_buf, x->norm_parts, x->bound, x->d_norm, total > JOIN_BLOCKS, st);
   for (int i = 0; i < nt;) {
@@ -2405,16 +2425,14 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
       cnt.nt = a.nt; cnt.at = a.at; cnt.lr = x->lr; cnt.d_lr = x->d_lr; cnt.b1 = x->b1; cnt.b2 = x->b2; cnt.wd = x->weight_decay; cnt.seed = x->seed; cnt.consts = x->d_consts;
       hipLaunchKernelGGL(hoic_adamw_count_kernel, dim3(1), dim3(64), 0, st, cnt);
     }
-    const dim3 grid((unsigned)blocks), block(256);
-    if (x->state_bits == 32) {
-      if (x->type == HOIC_F32) hipLaunchKernelGGL(hoic_adamw32_kernel<float>, grid, block, 0, st, a);
-      else if (x->type == HOIC_F16) hipLaunchKernelGGL(hoic_adamw32_kernel<_Float16>, grid, block, 0, st, a);
-      else hipLaunchKernelGGL(hoic_adamw32_kernel<__bf16>, grid, block, 0, st, a);
-    } else {
-      if (x->type == HOIC_F32) hipLaunchKernelGGL(hoic_adamw8_kernel<float>, grid, block, 0, st, a);
-      else if (x->type == HOIC_F16) hipLaunchKernelGGL(hoic_adamw8_kernel<_Float16>, grid, block, 0, st, a);
-      else hipLaunchKernelGGL(hoic_adamw8_kernel<__bf16>, grid, block, 0, st, a);
-    }
+    const bool around = bytes > STREAM_BYTES;
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, a); };
+    auto typed = [&](auto zero) {
+      typedef decltype(zero) T;
+      if (x->state_bits == 32) { if (around) launch(hoic_adamw32_kernel<T, true>); else launch(hoic_adamw32_kernel<T, false>); }
+      else { if (around) launch(hoic_adamw8_kernel<T, true>); else launch(hoic_adamw8_kernel<T, false>); }
+    };
+    if (x->type == HOIC_F32) typed(0.f); else if (x->type == HOIC_F16) typed((_Float16)0); else typed((__bf16)0.f);
     a.at += a.nt;
     a.clip.norm = nullptr;       // (written by the first launch)
   }
