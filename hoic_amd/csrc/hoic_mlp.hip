@@ -1586,7 +1586,7 @@ __device__ __forceinline__ void store_log_std_grad(const hoic_policy_loss_args& 
   else if (a.t_std == HOIC_F16) ((_Float16*)a.d_log_std)[j] = (_Float16)(float)x;
   else ((__bf16*)a.d_log_std)[j] = (__bf16)(float)x;
 }
-// SHARED: one row of log-deviations (and of the reference's) for all rows: their terms are made once a lane.  VEC: dims is a multiple of 4,
+// SHARED: one row of log-deviations (and of the reference's) for all rows: their terms are made once a dimension.  VEC: dims is a multiple of 4,
 // a lane's four dimensions are one load (else four).  Rows outside the batch read row 0's place and are dropped at the end: short
 // straight code matters more here than their traffic, a launch of a few rows waits for its instructions first of all.
 template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __launch_bounds__(PL_NT, 4) void hoic_policy_loss_kernel(PolicyLossArgs k) {
@@ -1673,7 +1673,8 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
     f32x4 mu = load((const TM*)a.mean, at * a.ld_mean), x = a.t_act == HOIC_F32 ? load((const float*)a.act, at * a.ld_act) : load((const TM*)a.act, at * a.ld_act);
     f32x4 mu0 = KL ? load((const TM*)a.ref_mean, at * a.ld_ref_mean) : zero4;
     if (!SHARED) {
-      const f32x4 s = load_std(a.log_std, at * a.ld_std), s0 = KL ? load_std(a.ref_log_std, at * a.ld_ref_std) : zero4;
+      f32x4 s = load_std(a.log_std, at * a.ld_std), s0 = KL ? load_std(a.ref_log_std, at * a.ld_ref_std) : zero4;
+      if (!ok) s = s0 = zero4;               // (they may be no numbers, which no product with 0 takes out)
       lc = kc = 0.;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
@@ -1733,7 +1734,7 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
             for (int e = 0; e < 4; e++) if (e < left) out[j + e] = (T)v[e];
           }
         };
-        store((TM*)a.d_mean + row * a.ld_dmean, g);
+        store((TM*)a.d_mean + row * a.ld_dmean, SHARED && !ok ? zero4 : g);      // (0 also beside a shared deviation that is no number)
         if (row_ls) { if (a.t_std == HOIC_F32) store((float*)a.d_log_std + row * a.dims, gs); else store((TM*)a.d_log_std + row * a.dims, gs); }
       }
     }
@@ -1742,7 +1743,7 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
   const bool lone = gridDim.x == 1;
   if (sum_ls) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) red[rg * (lpr * 4) + j + e] = SHARED ? dls[e] - acc_l + klw * (ke[e] * rows_in) : dls[e];
+    for (int e = 0; e < 4; e++) red[rg * (lpr * 4) + j + e] = !SHARED ? dls[e] : rows_in ? dls[e] - acc_l + klw * (ke[e] * rows_in) : 0.;
   }
   acc_s = wave_sum(acc_s); if (KL) acc_k = wave_sum(acc_k);
   if ((threadIdx.x & 63) == 0) { const int w = threadIdx.x >> 6; tail[0][w] = acc_s; tail[1][w] = acc_k; tail[2][w] = (double)acc_c; tail[3][w] = (double)acc_n; }

@@ -160,6 +160,32 @@ def test_policy_loss_clips_and_references_of_other_shapes():
 
 
 @gpu
+@pytest.mark.parametrize("mean", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["both", "log_std", "ref_log_std"])
+def test_policy_loss_deviations_of_masked_rows_are_not_used(kind, mean):
+    """rows outside the batch (the first and the last among them) hold log-deviations that are no numbers, the policy's, the reference's or
+    both (a shared one of the policy's with the reference's per row, too): their gradients are 0 and nobody else's see them"""
+    for M, N in ((2, 3), (33, 4), (70, 32), (19, 100)):
+        x = loss_case(M, N, mean=mean, per_row=kind != "ref_log_std", ref_row=kind != "log_std", mask=0.4, seed=M)
+        bad = ~x["valid"]
+        bad[0] = bad[-1] = True                                                           # (of two rows none is left)
+        x["valid"] = ~bad
+        for value in (float("nan"), float("inf"), float("-inf")):
+            for name in ("log_std", "ref_log_std"):
+                if kind in ("both", name):
+                    x[name][bad] = value
+            o = check_loss({k: None if v is None else v.cuda() for k, v in x.items()})
+            assert not bool(o.d_mean.cpu()[bad].any())
+        # a shared deviation that is no number reaches the rows of the batch only, and none if there are none
+        y = dict(x, log_std=torch.full((1, N), float("nan")), ref_log_std=torch.full((1, N), float("inf")))
+        y = {k: v.cuda() for k, v in y.items()}
+        o = rl.clipped_policy_loss_grad(**y, kl_coef=0.3)
+        assert not bool(o.d_mean.cpu()[bad].any()) and (bool(bad.all()) or bool(torch.isnan(o.d_log_std).all()))
+        o = rl.clipped_policy_loss_grad(**dict(y, valid=torch.zeros(M, dtype=torch.bool, device="cuda")), kl_coef=0.3)
+        assert float(o.loss) == 0.0 and not bool(o.d_mean.any()) and not bool(o.d_log_std.any())
+
+
+@gpu
 def test_policy_loss_strides_and_expanded_rows():
     """row strides that are no multiple of the dimensions, columns that are not adjacent, one row expanded over the batch"""
     base = loss_case(200, 9, per_row=True, seed=11, device="cuda")
