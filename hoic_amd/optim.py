@@ -172,6 +172,8 @@ class AdamW(torch.optim.Optimizer):
     def _make_state(self, p, step=0):
         bits, s = self.defaults["state_bits"], {}
         s["step"] = torch.full((), step, dtype=torch.int32, device=p.device) if self.defaults["capturable"] else step
+        if not p.is_contiguous():
+            s["order"] = _strides(p)
         for key in ("exp_avg", "exp_avg_sq"):
             if bits == 32:
                 s[key] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
@@ -180,9 +182,22 @@ class AdamW(torch.optim.Optimizer):
                 s[key + "_scale"] = torch.full(((p.numel() + BLOCK - 1) // BLOCK,), _EMPTY_SCALE, dtype=torch.float32, device=p.device)
         return s
 
+    def _new_order(self, p, s, capturing):
+        """moments of a parameter that lies in another order in memory than when they were made"""
+        if self.defaults["state_bits"] == 8:
+            raise ValueError("AdamW: 8-bit moments lie in blocks in the parameter's order in memory, which has changed since they were made")
+        if capturing:
+            raise lib.HoicError("AdamW: a parameter's order in memory has changed: take one eager step before a capture")
+        for key in ("exp_avg", "exp_avg_sq"):
+            s[key] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(s[key].reshape(p.shape))
+        s.pop("order", None)
+        if not p.is_contiguous():
+            s["order"] = _strides(p)
+
     def load_state_dict(self, state_dict):
         """Also takes the state of a ``torch.optim.Adam`` / ``AdamW`` over the same parameters (``state_bits=32``).  The moments are
-        copied, and keep their own types whatever the parameters' are."""
+        copied, and keep their own types whatever the parameters' are.  (8-bit ones need parameters in the order in memory that they
+        were made for.)"""
         old = [p for g in state_dict["param_groups"] for p in g["params"]]
         new = [p for g in self.param_groups for p in g["params"]]
         want = {"exp_avg", "exp_avg_sq"} if self.defaults["state_bits"] == 32 else {"exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale"}
@@ -193,9 +208,11 @@ class AdamW(torch.optim.Optimizer):
             s = state_dict["state"].get(k)
             if s is None:
                 continue
-            if set(s) - {"step"} != want:
+            if set(s) - {"step", "order"} != want:
                 raise ValueError(f"a state of {sorted(s)}: this optimiser holds {sorted(want)} (state_bits={self.defaults['state_bits']})")
             mine = self._make_state(p, int(s["step"]))
+            if self.defaults["state_bits"] == 8 and list(s.get("order", ())) != list(mine.get("order", ())):
+                raise ValueError("8-bit moments of a parameter that lay in another order in memory")
             for key in want:
                 if s[key].numel() != mine[key].numel() or (mine[key].dtype == torch.uint8) != (s[key].dtype == torch.uint8):
                     raise ValueError(f"{key}: {tuple(s[key].shape)} {s[key].dtype} for a parameter of {p.numel()} elements")
@@ -235,10 +252,12 @@ class AdamW(torch.optim.Optimizer):
                 g = p.grad
                 if g is None:
                     continue
-                dtype = p.dtype
-                if g.dtype is not dtype or g.layout is not torch.strided:
-                    raise ValueError(f"AdamW: a {g.dtype} gradient (dense ones only) of a {dtype} parameter")
-                if not (p.is_contiguous() and g.is_contiguous()) and _strides(g) != _strides(p):
+                dtype, at, n, contiguous = p.dtype, p.get_device(), p.numel(), p.is_contiguous()
+                if g.dtype is not dtype or g.layout is not torch.strided or g.numel() != n or g.get_device() != at:
+                    raise ValueError(f"AdamW: a gradient {tuple(g.shape)} {g.dtype} on {g.device} (dense ones only) of a parameter {tuple(p.shape)} {dtype} on {p.device}")
+                if not (contiguous and g.is_contiguous()) and _strides(g) != _strides(p):
+                    if not _dense(p) or g.shape != p.shape:
+                        raise ValueError(f"AdamW: a parameter {tuple(p.shape)} whose elements do not fill their memory, or a gradient of another shape, {tuple(g.shape)}")
                     g = torch.empty_like(p, requires_grad=False).copy_(g.detach())          # the parameter's order of elements
                     held.append(g)
                 s = state[p]
@@ -249,8 +268,16 @@ class AdamW(torch.optim.Optimizer):
                         raise lib.HoicError("AdamW: take one eager step before a capture (the states would be made anew at every replay)")
                     if not s:
                         s.update(self._make_state(p))
-                if (p.get_device(), gi, dtype) != key:
-                    key = (p.get_device(), gi, dtype)
+                m = s["exp_avg"]
+                if m.numel() != n or m.get_device() != at:
+                    raise ValueError(f"AdamW: moments of {m.numel()} elements on {m.device} for a parameter of {n} on {p.device}")
+                if not contiguous or "order" in s:
+                    if s.get("order") != (None if contiguous else _strides(p)):
+                        self._new_order(p, s, capturing)
+                        m = s["exp_avg"]
+                if (at, gi, dtype) != key:
+                    _check(p, "AdamW")
+                    key = (at, gi, dtype)
                     rows = work.get(key)
                     if rows is None:
                         rows = work[key] = []
@@ -260,8 +287,8 @@ class AdamW(torch.optim.Optimizer):
                     t = s["step"] + 1
                 if bits == 8:
                     m_scale, v_scale = s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr()
-                ptr, n = g.data_ptr(), p.numel()
-                rows += (p.data_ptr(), ptr, s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), m_scale, v_scale, n, t, d_step, ordinal)
+                ptr = g.data_ptr()
+                rows += (p.data_ptr(), ptr, m.data_ptr(), s["exp_avg_sq"].data_ptr(), m_scale, v_scale, n, t, d_step, ordinal)
                 params.append(p)
                 touched.append(s)
                 g_ptrs.append(ptr)
@@ -311,6 +338,8 @@ class AdamW(torch.optim.Optimizer):
         anew by one launch per 48 tensors; 32-bit ones: the states themselves); zeros where a parameter has no state yet."""
         bits, groups = self.defaults["state_bits"], self.param_groups
         states = [(p, self.state.get(p)) for group in groups for p in group["params"]]
+        if not states:
+            return [], []
         if bits == 32 and all(s for _, s in states):
             return [s["exp_avg"] for _, s in states], [s["exp_avg_sq"] for _, s in states]
         new = lambda p: torch.empty_like(p, dtype=torch.float32, requires_grad=False)
@@ -325,6 +354,8 @@ class AdamW(torch.optim.Optimizer):
                 ms.append(s["exp_avg"] if s and bits == 32 else new(p) if s else new(p).zero_())
                 vs.append(s["exp_avg_sq"] if s and bits == 32 else new(p) if s else new(p).zero_())
             if s and bits == 8:
+                if s["exp_avg"].numel() != p.numel() or s["exp_avg"].device != p.device or s.get("order") != (None if p.is_contiguous() else _strides(p)):
+                    raise ValueError("AdamW: 8-bit moments of a parameter whose size, device or order in memory has changed since")
                 rows = work.get(p.device)
                 if rows is None:
                     rows = work[p.device] = []

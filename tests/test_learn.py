@@ -815,6 +815,67 @@ def test_adamw_layouts_groups_and_missing_gradients(bits):
 
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_after_a_parameter_was_changed_underneath(bits):
+    """``p.data`` of another order in memory (32 bits: the moments follow; 8: refused, their blocks do not), size, device or type, gradients left
+    behind: nothing is launched, parameters, moments and counts stay"""
+    w = torch.randn(6, 5, 4, device="cuda")
+    a, b = torch.nn.Parameter(w.clone()), torch.nn.Parameter(w.clone())
+    g = torch.randn(6, 5, 4, device="cuda")
+    opts = [optim.AdamW([p], **HYP, state_bits=bits, seed=4) for p in (a, b)]
+    for p, o in zip((a, b), opts):
+        p.grad = g.clone()
+        o.step()
+    for order in ((2, 0, 1), (0, 1, 2)):                         # to an order of its own, and back
+        inverse = [order.index(i) for i in range(3)]
+        b.data = b.data.permute(order).contiguous().permute(inverse)
+        assert b.is_contiguous() == (order == (0, 1, 2))
+        if bits == 8 and order != (0, 1, 2):
+            for call in (opts[1].step, opts[1].state_values, lambda: optim.AdamW([b], state_bits=8).load_state_dict(opts[1].state_dict())):
+                with pytest.raises(ValueError):
+                    call()
+            continue
+        for p, o in zip((a, b), opts):
+            o.step(max_norm=1.0)
+        assert torch.equal(a, b) and opts[0].state[a]["step"] == opts[1].state[b]["step"]
+        for x, y in zip(opts[0].state_values(), opts[1].state_values()):
+            assert torch.equal(x[0], y[0]) and y[0].stride() == b.stride()
+    keep = b.detach().clone()
+    before = {k: v.clone() if torch.is_tensor(v) else v for k, v in opts[1].state[b].items()}
+    inner = torch.randn(6, 5, 8, device="cuda")
+    for data in (torch.randn(7, 5, 4, device="cuda"), torch.randn(6, 5, 3, device="cuda"), inner[:, :, :4], inner[:1, :, :4].expand(6, 5, 4), b.data.cpu(), b.data.double(),
+                 b.data.half()):
+        c = torch.nn.Parameter(b.detach().clone())
+        o = optim.AdamW([c], **HYP, state_bits=bits, seed=4)
+        o.load_state_dict(opts[1].state_dict())
+        c.grad = g.clone()
+        saved = data.clone()
+        c.data = data
+        for kw in ({}, {"max_norm": 1.0}):
+            with pytest.raises((ValueError, lib.HoicError)):
+                o.step(**kw)
+        assert torch.equal(data, saved) and o.state[c]["step"] == before["step"] and torch.equal(o.state[c]["exp_avg"], before["exp_avg"])
+        if data.numel() != b.numel() and data.is_cuda:           # a gradient that fits, moments that do not
+            c.grad = torch.ones_like(data)
+            with pytest.raises(ValueError):
+                o.step()
+            if bits == 8:
+                with pytest.raises(ValueError):
+                    o.state_values()
+    assert torch.equal(b.detach(), keep) and torch.equal(opts[1].state[b]["exp_avg"], before["exp_avg"])
+    c = torch.nn.Parameter(torch.randn(5, 6, device="cuda").t())                # an order of its own through a saved state
+    c.grad = torch.randn(6, 5, device="cuda")
+    o = optim.AdamW([c], **HYP, state_bits=bits, seed=4)
+    o.step()
+    d = torch.nn.Parameter(c.detach().clone(memory_format=torch.preserve_format))
+    d.grad = c.grad.clone()
+    q = optim.AdamW([d], **HYP, state_bits=bits, seed=4)
+    q.load_state_dict(copy.deepcopy(o.state_dict()))
+    o.step(); q.step()
+    assert d.stride() == c.stride() and torch.equal(c, d)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_resumes_from_its_state(bits):
     """state_dict / load_state_dict (also through torch.save) and deepcopy continue bit for bit; the moments keep their types"""
     import io
