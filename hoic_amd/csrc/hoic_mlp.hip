@@ -27,6 +27,7 @@
 #include <algorithm>
 #include <string>
 #include <type_traits>
+#include <vector>
 #include "../../include/hoic.h"
 #include "hoic_zfilter_core.h"
 
@@ -1981,6 +1982,25 @@ static int32_t norm_check(const char* who, const void* const* g, const int64_t* 
     if (n[i] < 0 || (n[i] > 0 && !g[i]) || type[i] > HOIC_BF16) { hoic_set_error(std::string(who) + ": a tensor without memory, with a negative size or of another type"); return HOIC_ERR_ARG; }
   return HOIC_OK;
 }
+// tensors that are written share no memory: each element would be taken twice, in any order
+struct Span { uintptr_t at, end; };
+static bool spans_overlap(std::vector<Span>& s) {
+  bool ascending = true;
+  for (size_t i = 1; i < s.size() && ascending; i++) ascending = s[i].at >= s[i - 1].end;
+  if (ascending) return false;
+  std::sort(s.begin(), s.end(), [](const Span& a, const Span& b) { return a.at < b.at; });
+  for (size_t i = 1; i < s.size(); i++) if (s[i].at < s[i - 1].end) return true;
+  return false;
+}
+static int32_t written_check(const char* who, void* const* g, const int64_t* n, const uint8_t* type, int32_t nt) {
+  const int32_t rc = norm_check(who, (const void* const*)g, n, type, nt);
+  if (rc != HOIC_OK) return rc;
+  std::vector<Span> spans;
+  spans.reserve(nt);
+  for (int i = 0; i < nt; i++) if (n[i] > 0) spans.push_back({(uintptr_t)g[i], (uintptr_t)g[i] + (uintptr_t)n[i] * (type[i] == HOIC_F32 ? 4 : 2)});
+  if (spans_overlap(spans)) { hoic_set_error(std::string(who) + ": two tensors in the same memory (their elements would be scaled twice)"); return HOIC_ERR_ARG; }
+  return HOIC_OK;
+}
 extern "C" int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt) {
   if (nt < 0 || (nt > 0 && !n)) return -1;
   const long long chunk = norm_chunk(n, nt);
@@ -2055,7 +2075,7 @@ extern "C" int32_t hoic_grad_norm_partial(const void* const* g, const int64_t* n
   return HOIC_OK;
 }
 extern "C" int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double bound, double* d_buf, float* d_norm, void* stream) {
-  const int32_t rc = norm_check("hoic_clip_grads", (const void* const*)g, n, type, nt);
+  const int32_t rc = written_check("hoic_clip_grads", g, n, type, nt);
   if (rc != HOIC_OK) return rc;
   const long long np = hoic_grad_norm_parts(n, nt);
   if (!d_buf || !d_norm || np == 0 || np > 0x7fffffff || !(bound >= 0.)) { hoic_set_error("hoic_clip_grads: an empty list, no place for the sums, or a bound below 0"); return HOIC_ERR_ARG; }
@@ -2070,7 +2090,7 @@ extern "C" int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8
 }
 
 extern "C" int32_t hoic_scale_list(void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, const float* d_factor, void* stream) {
-  const int32_t rc = norm_check("hoic_scale_list", (const void* const*)g, n, type, nt);
+  const int32_t rc = written_check("hoic_scale_list", g, n, type, nt);
   if (rc != HOIC_OK) return rc;
   if (!d_factor || hoic_grad_norm_parts(n, nt) > 0x7fffffff) { hoic_set_error("hoic_scale_list: no factor, or too large a list"); return HOIC_ERR_ARG; }
   ScaleArgs a;
@@ -2391,6 +2411,10 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
       hoic_set_error("hoic_adamw: a tensor without memory, state (8-bit: aligned to 4 bytes) or step count, or too large"); return HOIC_ERR_ARG;
     }
   }
+  std::vector<Span> spans;
+  spans.reserve(nt);
+  for (int i = 0; i < nt; i++) if (t[i].n > 0) spans.push_back({(uintptr_t)t[i].p, (uintptr_t)t[i].p + (uintptr_t)t[i].n * (x->type == HOIC_F32 ? 4 : 2)});
+  if (spans_overlap(spans)) { hoic_set_error("hoic_adamw: two parameters in the same memory"); return HOIC_ERR_ARG; }
   static_assert(ADAM8_CHUNK == ADAM32_CHUNK, "one chunk size for the launch below");
   hipStream_t st = (hipStream_t)stream;
   AdamArgs a;

@@ -107,15 +107,16 @@ def clip_grad_norm_(parameters, max_norm):
     if not grads:
         return torch.zeros(())
     args, parts = _tensor_list(grads, "clip_grad_norm_")
-    if len({p for p, n in zip(args[0], args[1]) if n}) < sum(1 for n in args[1] if n):
-        raise ValueError("clip_grad_norm_: two gradients in the same memory (each would be scaled twice)")
     dev = grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=dev)
     if parts == 0:
         return norm.zero_()
     buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
     with lib.Launch(dev) as st:
-        lib._chk(lib.load().hoic_clip_grads(*args, bound, buf.data_ptr(), norm.data_ptr(), st), "hoic_clip_grads")
+        rc = lib.load().hoic_clip_grads(*args, bound, buf.data_ptr(), norm.data_ptr(), st)
+    if rc != 0:
+        error = lib.load().hoic_last_error().decode()
+        raise (ValueError if "same memory" in error else lib.HoicError)(f"clip_grad_norm_: {error}")
     torch.autograd.graph.increment_version(grads)
     return norm
 
@@ -314,9 +315,6 @@ class AdamW(torch.optim.Optimizer):
                     lib._chk(L.hoic_grad_norm_partial(*args, buf_ptr, st), "hoic_grad_norm_partial")
             else:
                 norm.zero_()
-        if not capturable:
-            for s in touched:
-                s["step"] += 1
         for (at, gi, dtype), rows in work.items():
             group, dev, n = self.param_groups[gi], torch.device("cuda", at), len(rows) // 10
             lr, (b1, b2) = group["lr"], group["betas"]
@@ -330,6 +328,9 @@ class AdamW(torch.optim.Optimizer):
                                     0 if consts is None else consts.data_ptr(), buf_ptr, norm_ptr, bound or 0.0, parts, group["seed"], 0)
             with lib.Launch(dev) as st:
                 lib._chk(L.hoic_adamw((C.c_int64 * len(rows))(*rows), n, a, st), "hoic_adamw")
+        if not capturable:
+            for s in touched:
+                s["step"] += 1
         torch.autograd.graph.increment_version(params)
         return loss
 

@@ -522,6 +522,53 @@ def test_norm_refusals():
 
 
 # ================================================================================================ AdamW
+def test_lists_that_overlap_are_refused_on_the_host():
+    """any two tensors that are written, in whatever order they are listed; neighbours may touch"""
+    import ctypes as C
+    L = lib.load()
+    base = 1 << 20
+
+    def lists(spans, types):
+        return (C.c_void_p * len(spans))(*[base + at for at, _ in spans]), (C.c_int64 * len(spans))(*[n for _, n in spans]), bytes(types), len(spans)
+
+    cases = [([(0, 4), (0, 4)], (0, 0)), ([(0, 4), (12, 4)], (0, 0)), ([(12, 4), (0, 4)], (0, 0)), ([(0, 5), (8, 1)], (1, 0)), ([(64, 4), (0, 4), (32, 2), (34, 1)], (0, 0, 2, 1)),
+             ([(0, 100), (40, 1), (200, 1)], (2, 0, 1))]
+    for spans, types in cases:
+        assert L.hoic_clip_grads(*lists(spans, types), 1.0, 8, 8, None) == -1 and b"same memory" in L.hoic_last_error()
+        assert L.hoic_scale_list(*lists(spans, types), 8, None) == -1 and b"same memory" in L.hoic_last_error()
+    fields = dict(type=0, state_bits=32, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, weight_decay=0.0, d_lr=0, d_consts=0, d_norm_buf=0, d_norm=0, bound=0.0, norm_parts=0, seed=0,
+                  reserved=0)
+    for type_, spans in ((0, [(0, 4), (12, 4)]), (2, [(12, 2), (6, 4)]), (1, [(0, 1), (0, 1)])):
+        rows = [v for at, n in spans for v in (base + at, 8, 8, 8, 0, 0, n, 1, 0, 0)]
+        assert L.hoic_adamw((C.c_int64 * len(rows))(*rows), len(spans), lib.ADAMW_ARGS.pack(*(fields | dict(type=type_)).values()), None) == -1
+        assert b"same memory" in L.hoic_last_error()
+
+
+@gpu
+def test_clipping_and_adamw_of_views_of_one_buffer():
+    """neighbours in one buffer, listed in any order, are taken; views that share an element are refused and left as they are"""
+    flat, g = torch.randn(64, device="cuda"), torch.randn(64, device="cuda")
+    cuts = [(32, 64), (0, 7), (7, 32)]
+    ps = [torch.nn.Parameter(flat[a:b]) for a, b in cuts]
+    for p, (a, b) in zip(ps, cuts):
+        p.grad = g[a:b]
+    want = g.double() * min(1.0, 0.5 / (float(g.double().norm()) + 1e-6))
+    optim.clip_grad_norm_(ps, 0.5)
+    assert bool(((g.double() - want).abs() <= 2 * 1.001 * U32 * want.abs() + 2.0 ** -149).all())
+    opt, before = optim.AdamW(ps, lr=0.1), flat.clone()
+    opt.step()
+    assert bool((flat != before).all())
+    ps[0].grad = g[31:63]
+    keep = g.clone()
+    with pytest.raises(ValueError, match="same memory"):
+        optim.clip_grad_norm_(ps, 0.1)
+    ps[0].data = flat[31:63]
+    before = flat.clone()
+    with pytest.raises(lib.HoicError, match="same memory"):
+        opt.step()
+    assert torch.equal(g, keep) and torch.equal(flat, before) and all(opt.state[p]["step"] == 1 for p in ps)
+
+
 def random_bits(n, seed, step, ordinal, first=0):
     """the stochastic rounding's 32 bits per element, in NumPy"""
     def mix(x):
