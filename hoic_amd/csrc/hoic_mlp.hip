@@ -1812,6 +1812,7 @@ extern "C" int32_t hoic_policy_loss(const hoic_policy_loss_args* p, void* stream
       || (a.count && !a.d_mean)) {
     hoic_set_error("hoic_policy_loss: missing tensors"); return HOIC_ERR_ARG;
   }
+  if (a.rows > 1ll << 32) { hoic_set_error("hoic_policy_loss: more than 2^32 rows"); return HOIC_ERR_ARG; }      // (counts are in 32 bits per wavefront)
   hipStream_t st = (hipStream_t)stream;
   PolicyLossArgs k;
   k.a = a;
@@ -2177,7 +2178,7 @@ template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw32_
   float cl = 1.f;
   if (a.clip.parts) {
     const double2 f = join_norm(a.clip);
-    if (!(f.x < INFINITY)) return;
+    if (!((float)f.x < INFINITY)) return;      // (as float32, the norm that the caller is shown)
     cl = (float)f.y;
   }
   const AdamConsts c = adam_consts(a, t);
@@ -2313,7 +2314,7 @@ template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw8_k
   double cl = 1.;
   if (a.clip.parts) {
     const double2 f = join_norm(a.clip);
-    if (!(f.x < INFINITY)) return;
+    if (!((float)f.x < INFINITY)) return;      // (as float32, the norm that the caller is shown)
     cl = f.y;
   }
   const AdamConsts c = adam_consts(a, t);

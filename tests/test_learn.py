@@ -427,6 +427,14 @@ def test_policy_loss_entry_point_refuses_on_the_host():
     assert L.hoic_policy_loss_scratch_bytes(0) == 0
 
 
+def test_policy_loss_entry_point_refuses_rows_beyond_its_counts():
+    L = lib.load()
+    at = 64
+    for rows in ((1 << 32) + 1, 1 << 40):
+        args = lib.POLICY_LOSS_ARGS.pack(rows, 4, 0, 0, 0, at, at, at, 0, 0, 4, 4, 0, 0, 0, 4, at, 0, 0, 0, 0, 0.2, 0.2, 0.0, 1.0, 0, 0, 0, at, at, 0, at)
+        assert L.hoic_policy_loss(args, None) == -1 and b"2^32" in L.hoic_last_error()
+
+
 # ================================================================================================ norm and clipping
 def tensor_list(sizes, dtype=torch.float32, seed=0, scale=1.0, device="cuda"):
     g = torch.Generator().manual_seed(seed)
@@ -980,6 +988,22 @@ def test_adamw_skips_a_step_whose_norm_is_not_finite(bits):
     ps[1].grad[3] = 0.0
     opt.step(max_norm=1.0)
     assert all(bool(torch.isfinite(p).all()) for p in ps) and not torch.equal(ps[0].detach(), held[0][0])
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [60, 5 << 20])
+def test_adamw_skips_a_step_whose_norm_is_past_float32(bits, n):
+    """gradients of float32's largest values: the norm is finite in 64 bits and infinite in the float32 that the caller sees -- the step is
+    skipped like any whose ``grad_norm`` is not finite (joined in the step's launch, and before it in a large list)"""
+    p = torch.nn.Parameter(torch.ones(n, device="cuda"))
+    p.grad = torch.full((n,), 3.0e38, device="cuda")
+    opt = optim.AdamW([p], **HYP, state_bits=bits)
+    opt.step(max_norm=1.0)
+    assert math.isinf(float(opt.grad_norm)) and bool((p == 1).all()) and not bool(opt.state[p]["exp_avg"].any()) and not bool(opt.state[p]["exp_avg_sq"].any())
+    p.grad[1:] = 0.0
+    opt.step(max_norm=1.0)
+    assert abs(float(opt.grad_norm) / 3.0e38 - 1) <= 2 * U32 and float(p.detach()[0]) < 1.0
 
 
 @gpu
