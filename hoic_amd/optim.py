@@ -244,10 +244,10 @@ class AdamW(torch.optim.Optimizer):
         bits, capturable = self.defaults["state_bits"], self.defaults["capturable"]
         capturing, state = torch.cuda.is_current_stream_capturing(), self.state
         # rows of the list (hoic_adamw_tensor) per device, group and type
-        ordinal, work, key, rows = -1, {}, None, None
-        params, held, touched, g_ptrs, g_sizes, g_types = [], [], [], [], [], []
+        ordinal, work, rows, params, held, touched = -1, {}, None, [], [], []
         t = d_step = m_scale = v_scale = 0
         for gi, group in enumerate(self.param_groups):
+            rows_at = rows_dtype = None
             for p in group["params"]:
                 ordinal += 1
                 g = p.grad
@@ -276,25 +276,19 @@ class AdamW(torch.optim.Optimizer):
                     if s.get("order") != (None if contiguous else _strides(p)):
                         self._new_order(p, s, capturing)
                         m = s["exp_avg"]
-                if (at, gi, dtype) != key:
+                if at != rows_at or dtype is not rows_dtype:
                     _check(p, "AdamW")
-                    key = (at, gi, dtype)
-                    rows = work.get(key)
-                    if rows is None:
-                        rows = work[key] = []
+                    rows_at, rows_dtype = at, dtype
+                    rows = work.setdefault((at, gi, dtype), [])
                 if capturable:
                     d_step = s["step"].data_ptr()
                 else:
                     t = s["step"] + 1
                 if bits == 8:
                     m_scale, v_scale = s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr()
-                ptr = g.data_ptr()
-                rows += (p.data_ptr(), ptr, m.data_ptr(), s["exp_avg_sq"].data_ptr(), m_scale, v_scale, n, t, d_step, ordinal)
+                rows += (p.data_ptr(), g.data_ptr(), m.data_ptr(), s["exp_avg_sq"].data_ptr(), m_scale, v_scale, n, t, d_step, ordinal)
                 params.append(p)
                 touched.append(s)
-                g_ptrs.append(ptr)
-                g_sizes.append(n)
-                g_types.append(TYPES[dtype])
         self.grad_norm = None
         if not work:
             if bound is not None:
@@ -307,7 +301,12 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW: one norm over gradients on several devices")
             dev = params[0].device
             self.grad_norm = norm = torch.empty((), dtype=torch.float32, device=dev)
-            args, parts = _list_args(g_ptrs, g_sizes, g_types)
+            ptrs, sizes, types = [], [], []
+            for (_, _, dtype), rows in work.items():
+                ptrs += rows[1::10]
+                sizes += rows[6::10]
+                types += [TYPES[dtype]] * (len(rows) // 10)
+            args, parts = _list_args(ptrs, sizes, types)
             if parts:
                 buf = torch.empty(parts + 2, dtype=torch.float64, device=dev)
                 buf_ptr, norm_ptr = buf.data_ptr(), norm.data_ptr()
