@@ -7,7 +7,8 @@ Everything runs on the current stream of the tensors' device and nothing synchro
 """
 from __future__ import annotations
 
-import ctypes as C
+import itertools
+import struct
 
 import torch
 import torch.optim.optimizer as _opt
@@ -44,11 +45,16 @@ def _check(t, what):
         raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
 
 
+def _pack(x):
+    """64-bit integers as a host array (a third of the time of a ctypes array)"""
+    return struct.pack(f"{len(x)}q", *x)
+
+
 def _list_args(ptrs, sizes, types):
     """(pointers, sizes, types, count) of the hoic_grad_norm family, and the number of partial sums"""
     n = len(ptrs)
-    sizes = (C.c_int64 * n)(*sizes)
-    return ((C.c_void_p * n)(*ptrs), sizes, bytes(types), n), lib.load().hoic_grad_norm_parts(sizes, n)
+    sizes = _pack(sizes)
+    return (_pack(ptrs), sizes, bytes(types), n), lib.load().hoic_grad_norm_parts(sizes, n)
 
 
 def _tensor_list(tensors, what):
@@ -326,7 +332,7 @@ class AdamW(torch.optim.Optimizer):
             a = lib.ADAMW_ARGS.pack(TYPES[dtype], bits, lr, b1, b2, group["eps"], group["weight_decay"], lr_ptr,
                                     0 if consts is None else consts.data_ptr(), buf_ptr, norm_ptr, bound or 0.0, parts, group["seed"], 0)
             with lib.Launch(dev) as st:
-                lib._chk(L.hoic_adamw((C.c_int64 * len(rows))(*rows), n, a, st), "hoic_adamw")
+                lib._chk(L.hoic_adamw(_pack(rows), n, a, st), "hoic_adamw")
         if not capturable:
             for s in touched:
                 s["step"] += 1
@@ -343,27 +349,30 @@ class AdamW(torch.optim.Optimizer):
         if bits == 32 and all(s for _, s in states):
             return [s["exp_avg"] for _, s in states], [s["exp_avg_sq"] for _, s in states]
         new = lambda p: torch.empty_like(p, dtype=torch.float32, requires_grad=False)
-        ms, vs, work = [], [], {}
-        first = states[0][0]
-        if bits == 8 and all(s and p.device == first.device and p.is_contiguous() for p, s in states):
-            # one buffer a moment, cut into the parameters' shapes (an allocation a parameter costs more than the launch)
-            params, n = [p for p, _ in states], sum(p.numel() for p, _ in states)
-            ms, vs = (list(torch._C._nn.unflatten_dense_tensors(torch.empty(n, dtype=torch.float32, device=first.device), params)) for _ in range(2))
+        ms, vs, work, ptrs, at = [], [], {}, None, states[0][0].device
+        if bits == 8 and all([s and p.is_contiguous() and p.device == at for p, s in states]):
+            # one buffer, cut into the parameters' shapes (an allocation a parameter costs more than the launch)
+            sizes = [p.numel() for p, _ in states]
+            buf = torch.empty(2 * sum(sizes), dtype=torch.float32, device=at)
+            shape = lambda xs: [x if p.dim() == 1 else x.view(p.shape) for (p, _), x in zip(states, xs)]
+            cut, k = torch.split_with_sizes(buf, sizes + sizes), len(sizes)
+            ms, vs, ptrs = shape(cut[:k]), shape(cut[k:]), [buf.data_ptr() + 4 * x for x in itertools.accumulate(sizes + sizes, initial=0)]
         for i, (p, s) in enumerate(states):
-            if len(ms) <= i:
+            if ptrs is None:
                 ms.append(s["exp_avg"] if s and bits == 32 else new(p) if s else new(p).zero_())
                 vs.append(s["exp_avg_sq"] if s and bits == 32 else new(p) if s else new(p).zero_())
             if s and bits == 8:
-                if s["exp_avg"].numel() != p.numel() or s["exp_avg"].device != p.device or s.get("order") != (None if p.is_contiguous() else _strides(p)):
+                m, dev, n = s["exp_avg"], p.device, p.numel()
+                if m.numel() != n or m.device != dev or s.get("order") != (None if ptrs or p.is_contiguous() else _strides(p)):
                     raise ValueError("AdamW: 8-bit moments of a parameter whose size, device or order in memory has changed since")
-                rows = work.get(p.device)
+                rows = work.get(dev)
                 if rows is None:
-                    rows = work[p.device] = []
-                rows += (ms[i].data_ptr(), vs[i].data_ptr(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), s["exp_avg_scale"].data_ptr(),
-                         s["exp_avg_sq_scale"].data_ptr(), p.numel(), 1, 0, 0)
+                    rows = work[dev] = []
+                rows += (ptrs[i] if ptrs else ms[i].data_ptr(), ptrs[k + i] if ptrs else vs[i].data_ptr(), m.data_ptr(), s["exp_avg_sq"].data_ptr(),
+                         s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr(), n, 1, 0, 0)
         for dev, rows in work.items():
             with lib.Launch(dev) as st:
-                lib._chk(lib.load().hoic_adamw_values((C.c_int64 * len(rows))(*rows), len(rows) // 10, st), "hoic_adamw_values")
+                lib._chk(lib.load().hoic_adamw_values(_pack(rows), len(rows) // 10, st), "hoic_adamw_values")
         return ms, vs
 
 
