@@ -1513,7 +1513,13 @@ template <bool NT = false, class T> __device__ __forceinline__ void store4(T* __
 // Everything per row is in 64 bits: a row whose ratio lies within a float32 rounding of a clip border would otherwise have its
 // whole gradient or none by chance (|l| is 50 and more, so float32 leaves the ratio 1e-5 wide); on this GPU a 64-bit FMA
 // issues at the rate of a float32 one, and the kernel waits for memory.
-// A row is handled by `lpr` lanes of four dimensions each (lpr = the power of two >= dims / 4), a wavefront takes 64 / lpr rows.
+// A row is handled by `lpr` lanes of four dimensions each (lpr = the power of two >= dims / 4), a wavefront takes 64 / lpr rows, so that
+// a wavefront's load of 32 float32 dimensions is one stretch of 1 KB and a row's sums are three DPP steps.
+// Bound: HBM in large batches (524 287 x 32, a log-deviation per row, reference and mask: 91 us, 5.1 TB/s; a copy reaches 4.8), the
+// latency of load -> row sums -> store in an update's (53 248 x 32 shared: 10.3 us, two such steps a workgroup).  At most 1024
+// workgroups of equally many steps, four on each CU: 512 take 12.1 us against 11.9 at 53 248 rows and 118 against 92 at 524 287,
+// 2048 take 13.9 and 90 (twice the partial sums to join).  Dimensions that are no multiple of four are loaded one by one: a vector load where four are
+// left and single ones in the last lane costs both paths in every wavefront (26 dimensions 58.9 against 51.9 us, 33: 121 against 98).
 struct PolicyLossArgs {
   hoic_policy_loss_args a;
   int lpr_log2;
@@ -1553,7 +1559,8 @@ __device__ __forceinline__ double row_sum(double x, int lpr) {
 }
 __device__ __forceinline__ double wave_sum(double x) { return row_sum(x, 64); }
 
-// valid rows of 4096 bytes a workgroup step, 16 a lane
+// valid rows, 4096 bytes a workgroup's step, 16 a lane (in front of a gradient, whose rows are divided by their number: 3.4 us at 524 287 rows, a
+// launch's latency)
 __global__ __launch_bounds__(256) void hoic_count_valid_kernel(const unsigned char* __restrict__ valid, long long rows, long long per_block, int* __restrict__ counts) {
   typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(1)));
   __shared__ int red[4];
@@ -1765,7 +1772,8 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
   }
 }
 
-// sums of the workgroups' parts, a column a wavefront: workgroup 0 the scalars, the others four dimensions each
+// sums of the workgroups' parts, a column a wavefront, all 16 loads of a lane in flight: workgroup 0 the scalars, the others four
+// dimensions each (2.9 us: the latency of one load, the tree and a launch)
 __global__ __launch_bounds__(256) void hoic_policy_loss_finish_kernel(PolicyLossArgs k) {
   const hoic_policy_loss_args& a = k.a;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, j = blockIdx.x == 0 ? a.dims + w : ((int)blockIdx.x - 1) * 4 + w;
@@ -1840,8 +1848,8 @@ extern "C" int32_t hoic_policy_loss(const hoic_policy_loss_args* p, void* stream
 }
 
 // ---------------------------------------------------------------------------------------------- lists of tensors
-// A list's tensors travel in the kernel arguments (<= LIST_MAX a launch), so that a call needs no table in device memory, no
-// copy to it, and can be captured into a graph as it is.  A workgroup takes one chunk of one tensor.
+// A list's tensors travel in the kernel arguments (NORM_MAX or ADAM_MAX a launch, what 4 KB of arguments hold), so that a call needs no
+// table in device memory, no copy to it, and can be captured into a graph as it is.  A workgroup takes one chunk of one tensor.
 template <class E, int MAXT> __device__ __forceinline__ int list_find(const E (&t)[MAXT], int nt, int block) {
   int lo = 0, hi = nt - 1;
   while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (t[mid].first <= block) lo = mid; else hi = mid - 1; }
@@ -1850,7 +1858,7 @@ template <class E, int MAXT> __device__ __forceinline__ int list_find(const E (&
 
 // sqrt(sum g^2) over a list: 64-bit partial sums per workgroup, then joined in fixed order, with the factor
 // min(1, bound / (norm + 1e-6)) beside it -- by a workgroup of its own, or, in lists of few parts, by every workgroup of the launch
-// that uses the factor (Joint): that saves the launch between.
+// that uses the factor (Joint): that saves the launch between (JOIN_LAUNCHES, JOIN_BLOCKS).
 struct Joint { const double* parts; int nparts; double bound; float* norm; };      // parts NULL: no clipping; nparts 0: parts = {norm, factor}
 __device__ __forceinline__ double2 norm_factor(double sum, double bound) {
   const double t = sqrt(sum), c = bound / (t + 1e-6);
@@ -1922,6 +1930,8 @@ template <bool NT, class T> __device__ __forceinline__ double sumsq(const T* g, 
   }
   return s;
 }
+// Bound: HBM (268 M bf16 values, 537 MB: 104 us, 5.2 TB/s; the 64-bit FMA of a value issues as a 32-bit one), a launch's latency in short
+// lists (3.9 M values: 4.3 us).
 template <bool NT> __global__ __launch_bounds__(256) void hoic_sumsq_kernel(NormArgs a) {
   __shared__ double red[4];
   const int t = list_find(a.t, a.nt, blockIdx.x);
@@ -1938,7 +1948,8 @@ __global__ __launch_bounds__(256) void hoic_norm_finish_kernel(Joint j, double* 
   const double2 r = join_norm(j);
   if (threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
 }
-// g *= factor where it is not 1
+// g *= factor where it is not 1.  Bound: HBM (537 MB read and written: 171 us, 6.3 TB/s); short lists wait for the parts' join (3.9 M float32
+// values: 7.2 us).
 struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; Joint clip; const float* factor; };      // factor: in the place of the clipping one
 template <bool NT, class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, const Joint& clip, const float* factor) {
   typedef WideStep<T> W;
@@ -1976,7 +1987,10 @@ static long long norm_chunk(const int64_t* n, int32_t nt) {
   const long long c = (tot + 1023) / 1024;
   return c <= 8192 ? 8192 : (c + NORM_STEP - 1) / NORM_STEP * NORM_STEP;
 }
-#define JOIN_PARTS 2048          // up to so many parts are joined by the workgroups that use them
+// The parts are joined by the workgroups that use them where these are of at most two launches (some 1000 parts and one per tensor): clipping
+// 252 k to 268 M elements in 6 or 8 tensors saves 1.0 to 1.4 us of GPU time that way (4 M: 10.1 against 11.2; and 2.5 us of host time), 1 M in 240 0.7, in
+// 480 (four launches) it loses 1.0.
+#define JOIN_LAUNCHES 2
 static int32_t norm_check(const char* who, const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt) {
   if (nt < 0 || (nt > 0 && (!g || !n || !type))) { hoic_set_error(std::string(who) + ": bad list"); return HOIC_ERR_ARG; }
   for (int i = 0; i < nt; i++)
@@ -2053,7 +2067,7 @@ static void scale_launches(ScaleArgs& a, void* const* g, const int64_t* n, const
 // d_buf = {norm, factor, parts ...}; what a launch that uses the factor is given: the parts, or {norm, factor} after a join
 static Joint norm_join(double* d_buf, long long nparts, double bound, float* d_norm, bool now, hipStream_t st) {
   Joint j = {d_buf + 2, (int)nparts, bound, d_norm};
-  if (nparts <= JOIN_PARTS && !now) return j;
+  if (!now) return j;
   hipLaunchKernelGGL(hoic_norm_finish_kernel, dim3(1), dim3(256), 0, st, j, d_buf);
   return Joint{d_buf, 0, bound, nullptr};
 }
@@ -2084,7 +2098,13 @@ extern "C" int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8
   norm_partial((const void* const*)g, n, type, nt, d_buf + 2, st);
   ScaleArgs a;
   a.factor = nullptr;
-  a.clip = norm_join(d_buf, np, bound, d_norm, false, st);
+  int launches = 0;
+  for (int ty = HOIC_F32; ty <= HOIC_BF16; ty++) {
+    int k = 0;
+    for (int i = 0; i < nt; i++) k += type[i] == ty && n[i] > 0;
+    launches += (k + NORM_MAX - 1) / NORM_MAX;
+  }
+  a.clip = norm_join(d_buf, np, bound, d_norm, launches > JOIN_LAUNCHES, st);
   scale_launches(a, g, n, type, nt, st);
   MCHK(hipGetLastError());
   return HOIC_OK;
@@ -2159,8 +2179,15 @@ __device__ __forceinline__ unsigned wave_max(unsigned x) {
 #undef DPP_MAX
   return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
+// 2048 elements a workgroup: a list of six small tensors (252 k elements) takes 4.7 us, 6.5 with 4096, 9.7 with 8192; 3.9 M elements 17.3 / 16.9 / 16.9,
+// 134 M of bf16 548 / 538 / 599 (8-bit states 383 / 394 / 413).
+// Bound: HBM (134 M bf16 parameters, 2.95 GB: 480 to 500 us, 5.9 TB/s; 3.9 M float32 ones, out of the last-level cache: 17.8 us).
 #define ADAM32_CHUNK 2048
-#define JOIN_BLOCKS 4096         // a launch of more workgroups is given the joined factor
+// Launches of more workgroups (and lists of more than JOIN_LAUNCHES) are given the joined factor.  Norm and step, joined by the workgroups / in
+// front: 32 bits 26.2 / 28.5 us at 2048 workgroups, 43.5 / 46.2 at 4096, 88.2 / 88.4 at 8192; 8 bits 18.5 / 19.5 at 1024, 30.2 / 30.9 at 2048, 38.8 / 38.3
+// at 3072, 46.2 / 44.1 at 4096 (fewer elements in flight to hide it).  100 tensors (three launches): 27.1 / 27.0 and 34.1 / 34.2; 1000: 192 / 176.
+#define JOIN_BLOCKS32 4096
+#define JOIN_BLOCKS8 2048
 template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw32_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; float* m = (float*)a.t[t].m; float* v = (float*)a.t[t].v;
@@ -2291,6 +2318,9 @@ __device__ __forceinline__ unsigned code8_quick(double a, double r, int low, uns
   near = min(near, (t << 15) + 0x8000u);
   return (t >> 17) - (sub ? (unsigned)(1023 + low) * 8u : (unsigned)(1022 + low) * 8u);
 }
+// The step with 8-bit states, a block of 256 elements a wavefront (four a lane: the codes are one 32-bit load, the block's maxima one DPP
+// tree), two blocks' loads in flight.  Bound: 80 VALU operations an element -- 134 M elements take 339 us with float32 parameters (6.3 TB/s) and
+// 317 with bf16 ones (4.2): 2.4 ps an element whatever they weigh.
 template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; unsigned char* m = (unsigned char*)a.t[t].m; unsigned char* v = (unsigned char*)a.t[t].v;
@@ -2364,7 +2394,8 @@ template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw8_k
   }
   for (; again; again &= again - 1) adam8_block<T>(a, t, c, cl, key, i0, ((__ffs(again) - 1) * 4 + wave) * 256, left, lane);
 }
-// the float32 values of 8-bit states: p, g of an entry are the places of m's and v's values
+// the float32 values of 8-bit states: p, g of an entry are the places of m's and v's values (HBM: 134 M elements, 1.35 GB: 215 us, 6.3 TB/s;
+// stores around the caches lose here: 719 against 646 us at 2 GB)
 __global__ __launch_bounds__(256) void hoic_adamw_values_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   float* om = (float*)a.t[t].p; float* ov = (float*)(uintptr_t)a.t[t].g;
@@ -2385,7 +2416,7 @@ __global__ __launch_bounds__(256) void hoic_adamw_values_kernel(AdamArgs a) {
     store4(om + i, l, x); store4(ov + i, l, y);
   }
 }
-// a captured step counts on the device: step += 1, then the constants that depend on it
+// a captured step counts on the device: step += 1, then the constants that depend on it (one thread a tensor: a launch's latency)
 struct AdamCount { int* step[ADAM_MAX]; unsigned ordinal[ADAM_MAX]; int nt, at; double lr; const float* d_lr; double b1, b2, wd; unsigned seed; float* consts; };
 __global__ __launch_bounds__(64) void hoic_adamw_count_kernel(AdamCount a) {
   const int t = threadIdx.x;
@@ -2423,12 +2454,14 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
   a.b1d = x->b1; a.c1d = 1. - x->b1; a.b2d = x->b2; a.c2d = 1. - x->b2; a.consts = x->d_consts;
   a.at = 0;
   long long total = 0, bytes = 0;
+  int some = 0;
   for (int i = 0; i < nt; i++) {
+    some += t[i].n > 0;
     total += (t[i].n + ADAM32_CHUNK - 1) / ADAM32_CHUNK;
     bytes += t[i].n * ((x->type == HOIC_F32 ? 8 : 4) + x->state_bits / 4);          // p, g, m, v
   }
   a.clip = Joint{nullptr, 0, 0., nullptr};
-  if (x->d_norm_buf) a.clip = norm_join(x->d_norm_buf, x->norm_parts, x->bound, x->d_norm, total > JOIN_BLOCKS, st);
+  if (x->d_norm_buf) a.clip = norm_join(x->d_norm_buf, x->norm_parts, x->bound, x->d_norm, total > (x->state_bits == 8 ? JOIN_BLOCKS8 : JOIN_BLOCKS32) || some > JOIN_LAUNCHES * ADAM_MAX, st);
   for (int i = 0; i < nt;) {
     long long blocks = 0;
     AdamCount cnt;
