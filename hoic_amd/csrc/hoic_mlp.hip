@@ -25,6 +25,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
+#include <exception>
 #include <string>
 #include <type_traits>
 #include <vector>
@@ -1999,22 +2000,30 @@ static int32_t norm_check(const char* who, const void* const* g, const int64_t* 
 }
 // tensors that are written share no memory: each element would be taken twice, in any order
 struct Span { uintptr_t at, end; };
-static bool spans_overlap(std::vector<Span>& s) {
+template <class F> static int32_t spans_check(const char* who, int32_t nt, F span) {       // span(i): of tensor i, {0, 0}: an empty one
+  uintptr_t last = 0;
   bool ascending = true;
-  for (size_t i = 1; i < s.size() && ascending; i++) ascending = s[i].at >= s[i - 1].end;
-  if (ascending) return false;
-  std::sort(s.begin(), s.end(), [](const Span& a, const Span& b) { return a.at < b.at; });
-  for (size_t i = 1; i < s.size(); i++) if (s[i].at < s[i - 1].end) return true;
-  return false;
+  for (int i = 0; i < nt && ascending; i++) {
+    const Span s = span(i);
+    if (s.end == s.at) continue;
+    ascending = s.at >= last; last = s.end;
+  }
+  if (ascending) return HOIC_OK;
+  bool twice = false;
+  try {
+    std::vector<Span> s;
+    s.reserve(nt);
+    for (int i = 0; i < nt; i++) { const Span x = span(i); if (x.end != x.at) s.push_back(x); }
+    std::sort(s.begin(), s.end(), [](const Span& a, const Span& b) { return a.at < b.at; });
+    for (size_t i = 1; i < s.size(); i++) twice = twice || s[i].at < s[i - 1].end;
+  } catch (const std::exception&) { hoic_set_error("no host memory for the list"); return HOIC_ERR_ARG; }
+  if (twice) { hoic_set_error(std::string(who) + ": two tensors in the same memory (their elements would be taken twice)"); return HOIC_ERR_ARG; }
+  return HOIC_OK;
 }
 static int32_t written_check(const char* who, void* const* g, const int64_t* n, const uint8_t* type, int32_t nt) {
   const int32_t rc = norm_check(who, (const void* const*)g, n, type, nt);
   if (rc != HOIC_OK) return rc;
-  std::vector<Span> spans;
-  spans.reserve(nt);
-  for (int i = 0; i < nt; i++) if (n[i] > 0) spans.push_back({(uintptr_t)g[i], (uintptr_t)g[i] + (uintptr_t)n[i] * (type[i] == HOIC_F32 ? 4 : 2)});
-  if (spans_overlap(spans)) { hoic_set_error(std::string(who) + ": two tensors in the same memory (their elements would be scaled twice)"); return HOIC_ERR_ARG; }
-  return HOIC_OK;
+  return spans_check(who, nt, [&](int i) { return n[i] > 0 ? Span{(uintptr_t)g[i], (uintptr_t)g[i] + (uintptr_t)n[i] * (type[i] == HOIC_F32 ? 4 : 2)} : Span{0, 0}; });
 }
 extern "C" int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt) {
   if (nt < 0 || (nt > 0 && !n)) return -1;
@@ -2443,10 +2452,8 @@ extern "C" int32_t hoic_adamw(const hoic_adamw_tensor* t, int32_t nt, const hoic
       hoic_set_error("hoic_adamw: a tensor without memory, state (8-bit: aligned to 4 bytes) or step count, or too large"); return HOIC_ERR_ARG;
     }
   }
-  std::vector<Span> spans;
-  spans.reserve(nt);
-  for (int i = 0; i < nt; i++) if (t[i].n > 0) spans.push_back({(uintptr_t)t[i].p, (uintptr_t)t[i].p + (uintptr_t)t[i].n * (x->type == HOIC_F32 ? 4 : 2)});
-  if (spans_overlap(spans)) { hoic_set_error("hoic_adamw: two parameters in the same memory"); return HOIC_ERR_ARG; }
+  const int32_t apart = spans_check("hoic_adamw", nt, [&](int i) { return t[i].n > 0 ? Span{(uintptr_t)t[i].p, (uintptr_t)t[i].p + (uintptr_t)t[i].n * (x->type == HOIC_F32 ? 4 : 2)} : Span{0, 0}; });
+  if (apart != HOIC_OK) return apart;
   static_assert(ADAM8_CHUNK == ADAM32_CHUNK, "one chunk size for the launch below");
   hipStream_t st = (hipStream_t)stream;
   AdamArgs a;

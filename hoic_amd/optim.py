@@ -137,7 +137,8 @@ class AdamW(torch.optim.Optimizer):
     learning rates).
 
     ``step(max_norm=b)`` clips by the norm of all gradients inside the step (the gradients themselves are left alone); the norm is in
-    ``self.grad_norm`` afterwards, and a norm that is not finite leaves parameters and moments as they are.
+    ``self.grad_norm`` afterwards, and a norm that is not finite leaves parameters and moments as they are (the step counts all the same:
+    the host does not wait for the norm).
 
     ``capturable``: the step count lives on the device, so that ``step()`` can be captured into a graph (after one eager step, which
     makes the states) and replayed; ``lr`` may then be a float32 CUDA tensor of one element, read at every replay."""

@@ -347,7 +347,7 @@ int32_t hoic_mlp_rowsum_packed(const void* d_P, int32_t rows, int32_t Cp, float*
  * is asynchronous on `stream`, launches on the current device and can be captured into a HIP graph. */
 enum hoic_type { HOIC_F32 = 0, HOIC_F16 = 1, HOIC_BF16 = 2 };
 /* hoic_policy_loss: the clipped policy loss of a Gaussian policy with a KL term (agent_ppo.py:46-64 with policy_gaussian.py:27-33,
- * distributions.py:11-22; the KL term is PPO's penalty form, which the reference does not have).  Rows m, dimensions j < dims
+ * distributions.py:11-22; the KL term is PPO's penalty form, which the reference does not have).  Rows m (<= 2^32), dimensions j < dims
  * <= 256; s = log_std, l = sum_j log N(act; mean, e^s), r = e^(l - fixed) (fixed NULL: r = 1, the old policy is this one),
  *   S = -min(r adv, clip(r, 1 - clip_lo, 1 + clip_hi) adv),  K = KL(reference || policy),  L = sum over valid rows (S + kl_coef K) / n,
  * n = number of valid rows (valid NULL: all; no valid row: L = 0 and no gradient).  Rows outside `valid` may hold anything.
@@ -383,7 +383,8 @@ int32_t hoic_policy_loss(const hoic_policy_loss_args* a, void* stream);
  * hoic_grad_norm: the norm; d_buf[0..1] = {norm, 1} afterwards.
  * hoic_grad_norm_partial: the parts alone, for hoic_adamw (d_norm_buf, norm_parts) to join.
  * hoic_scale_list: g *= *d_factor (device float; 1 touches nothing).
- * hoic_clip_grads: g *= min(1, bound / (norm + 1e-6)) in place (a factor of 1 touches nothing). */
+ * hoic_clip_grads: g *= min(1, bound / (norm + 1e-6)) in place (a factor of 1 touches nothing).
+ * Tensors that are written share no memory (HOIC_ERR_ARG otherwise; hoic_adamw's parameters too). */
 int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt);
 int32_t hoic_grad_norm(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* d_buf, float* d_norm, void* stream);
 int32_t hoic_grad_norm_partial(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* d_buf, void* stream);
@@ -392,7 +393,7 @@ int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8_t* type, i
 /* hoic_adamw: one AdamW step over nt tensors of one type (in the place of the optimiser step of agent_ppo.py:46-56 / agent_pg.py:18-25;
  * list in HOST memory).  m' = b1 m + (1 - b1) c g, v' = b2 v + (1 - b2) (c g)^2, p' = p - (lr wd p + lr / (1 - b1^t) m' / (sqrt(v' / (1 - b2^t))
  * + eps)).  c = 1 without d_norm_buf; with it c = min(1, bound / (norm + 1e-6)) from the norm_parts parts of hoic_grad_norm_partial
- * (the norm comes back in d_norm), and a norm that is not finite leaves everything as it is.
+ * (the norm comes back in d_norm), and a norm that is not finite in float32 leaves everything as it is.
  *   state_bits 32: m, v float32 [n];  8: m, v bytes [n], m_scale, v_scale float32 [ceil(n / 256)]: blocks of 256 in storage order, a
  *   power-of-two scale each; m sign + e4m3 (bias 7), v e5m3 (bias 15) without sign; rounded up with the probability of the part cut
  *   off by a hash of (seed, t, ordinal, element); 0x7f / 0xff stand for values that are not finite
