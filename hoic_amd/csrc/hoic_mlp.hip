@@ -1892,28 +1892,39 @@ template <> struct wide<__bf16> { typedef b8u type; enum { n = 8 }; };
 template <class T> struct WideStep {
   static constexpr int N = wide<T>::n, SPAN = 256 * N;          // elements of a load, of a workgroup's row of loads
   typename wide<T>::type x[8];
-  // the lane's elements from i on, of which those below i1 exist (the rest read as 0)
+  // the workgroup's elements from i on, of which those below i1 exist (the rest read as 0): whole rows of loads, at most one cut one
   template <bool NT> __device__ __forceinline__ void load(const T* g, long long i, long long i1) {
-    if (i - threadIdx.x * N + 8 * SPAN <= i1) {
+    const int left = i1 - i < 8 * SPAN ? (int)(i1 - i) : 8 * SPAN, lane = threadIdx.x * N;
+    g += i;
+    if (left == 8 * SPAN) {
 #pragma unroll
-      for (int u = 0; u < 8; u++) x[u] = load_as<NT>((const typename wide<T>::type*)(g + i + u * SPAN));
+      for (int u = 0; u < 8; u++) x[u] = load_as<NT>((const typename wide<T>::type*)(g + lane + u * SPAN));
     } else {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
-        const long long at = i + u * SPAN;
-        if (at + N <= i1) { x[u] = *(const typename wide<T>::type*)(g + at); continue; }
-#pragma unroll
-        for (int e = 0; e < N; e++) x[u][e] = at + e < i1 ? g[at + e] : (T)0.f;
+        typename wide<T>::type z = {};
+        x[u] = z;
+        if ((u + 1) * SPAN <= left) x[u] = load_as<NT>((const typename wide<T>::type*)(g + lane + u * SPAN));
       }
+      const int cut = left / SPAN * SPAN + lane;
+      typename wide<T>::type y = {};
+#pragma unroll
+      for (int e = 0; e < N; e++) if (cut + e < left) y[e] = g[cut + e];
+#pragma unroll
+      for (int u = 0; u < 8; u++) if (u == left / SPAN) x[u] = y;
     }
   }
   __device__ __forceinline__ void store(T* g, long long i, long long i1) const {
+    const int left = i1 - i < 8 * SPAN ? (int)(i1 - i) : 8 * SPAN, lane = threadIdx.x * N;
+    g += i;
 #pragma unroll
     for (int u = 0; u < 8; u++) {
-      const long long at = i + u * SPAN;
-      if (at + N <= i1) { *(typename wide<T>::type*)(g + at) = x[u]; continue; }
+      if ((u + 1) * SPAN <= left) {
+        *(typename wide<T>::type*)(g + lane + u * SPAN) = x[u];
+      } else if (u * SPAN < left) {
 #pragma unroll
-      for (int e = 0; e < N; e++) if (at + e < i1) g[at + e] = x[u][e];
+        for (int e = 0; e < N; e++) if (u * SPAN + lane + e < left) g[u * SPAN + lane + e] = x[u][e];
+      }
     }
   }
 };
@@ -1921,7 +1932,7 @@ template <bool NT, class T> __device__ __forceinline__ double sumsq(const T* g, 
   typedef WideStep<T> W;
   double s = 0.;
   W w;
-  for (long long i = i0 + threadIdx.x * W::N; i - threadIdx.x * W::N < i1; i += 8 * W::SPAN) {
+  for (long long i = i0; i < i1; i += 8 * W::SPAN) {
     w.template load<NT>(g, i, i1);
 #pragma unroll
     for (int u = 0; u < 8; u++) {
@@ -1956,7 +1967,7 @@ template <bool NT, class T> __device__ __forceinline__ void scale_list(T* g, lon
   typedef WideStep<T> W;
   W w;
   if (factor && *factor == 1.f) return;
-  long long i = i0 + threadIdx.x * W::N;
+  long long i = i0;
   w.template load<NT>(g, i, i1);               // (on their way while the norm is joined)
   const double f = factor ? (double)*factor : join_norm(clip).y;
   if (f == 1.) return;
@@ -1969,7 +1980,7 @@ template <bool NT, class T> __device__ __forceinline__ void scale_list(T* g, lon
     }
     w.store(g, i, i1);
     i += 8 * W::SPAN;
-    if (i - threadIdx.x * W::N >= i1) break;
+    if (i >= i1) break;
     w.template load<NT>(g, i, i1);
   }
 }
