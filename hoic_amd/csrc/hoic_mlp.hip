@@ -1879,9 +1879,9 @@ __device__ __forceinline__ double2 join_norm(const Joint& j) {
   if (j.norm && blockIdx.x == 0 && threadIdx.x == 0) *j.norm = (float)r.x;
   return r;
 }
-struct NormEntry { const void* g; long long n; int first; };
+struct NormEntry { const void* g; long long n; int first, part; };
 #define NORM_MAX 120
-struct NormArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; double* part; };
+struct NormArgs { NormEntry t[NORM_MAX]; int nt, type, units; long long chunk; double* part; };      // units: parts a workgroup (the second stays 0)
 // Eight loads of 16 bytes a lane, all in flight before the first is used: 8192 elements of 32 bits a workgroup's step, 16384 of 16
 #define NORM_STEP 16384          // elements in whole steps of either kind
 typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(2)));
@@ -1953,7 +1953,8 @@ template <bool NT> __global__ __launch_bounds__(256) void hoic_sumsq_kernel(Norm
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) a.part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+  if (threadIdx.x < a.units && i0 + (threadIdx.x ? a.chunk >> 1 : 0) < a.t[t].n)
+    a.part[a.t[t].part + (blockIdx.x - a.t[t].first) * a.units + threadIdx.x] = threadIdx.x ? 0. : (red[0] + red[1]) + (red[2] + red[3]);
 }
 // parts -> clip = {norm, factor}, norm in float32
 __global__ __launch_bounds__(256) void hoic_norm_finish_kernel(Joint j, double* __restrict__ clip) {
@@ -1962,7 +1963,7 @@ __global__ __launch_bounds__(256) void hoic_norm_finish_kernel(Joint j, double* 
 }
 // g *= factor where it is not 1.  Bound: HBM (537 MB read and written: 171 us, 6.3 TB/s); short lists wait for the parts' join (3.9 M float32
 // values: 7.2 us).
-struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type; long long chunk; Joint clip; const float* factor; };      // factor: in the place of the clipping one
+struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type, units; long long chunk; Joint clip; const float* factor; };      // factor: in the place of the clipping one
 template <bool NT, class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, const Joint& clip, const float* factor) {
   typedef WideStep<T> W;
   W w;
@@ -1991,8 +1992,9 @@ template <bool NT> __global__ __launch_bounds__(256) void hoic_scale_kernel(Scal
   else if (a.type == HOIC_F16) scale_list<NT>((_Float16*)a.t[t].g, i0, i1, a.clip, a.factor);
   else scale_list<NT>((__bf16*)a.t[t].g, i0, i1, a.clip, a.factor);
 }
-// elements a workgroup: whole steps, or one of 8192 in lists too short to fill the chip otherwise; at most ~1024 workgroups (= parts) a list
-// beyond one per tensor
+// elements a part: whole steps, or 8192 in lists too short to fill the chip otherwise (4 M float32 values in 8 tensors clipped in 10.2 us, 11.9
+// with 4096, 10.6 with 16384); at most ~1024 parts a list beyond one per tensor (32 M clipped in 63.0 us, 64.6 with 2048, 62.8 with 512, but 8 M in
+// 14.5, 14.7 and 18.0)
 static long long norm_chunk(const int64_t* n, int32_t nt) {
   long long tot = 0;
   for (int i = 0; i < nt; i++) tot += n[i];
@@ -2052,18 +2054,20 @@ static long long list_bytes(const int64_t* n, const uint8_t* type, int32_t nt) {
   for (int i = 0; i < nt; i++) b += n[i] * (type[i] == HOIC_F32 ? 4 : 2);
   return b;
 }
-// launches over a list, type by type: f(entries so far, blocks) for every NORM_MAX of them
+// launches over a list, type by type: launch(workgroups, parts) for every NORM_MAX tensors of one.  A part is norm_chunk elements of a
+// tensor whatever its type; in short lists a workgroup of 16-bit elements takes two, a whole step of its loads (clipping 8 M bf16 values in
+// 8 tensors 11.5 us, 13.6 with one; 1 M 7.5 / 8.2), one of 32-bit elements one (with two 17.5 us against 14.7, and 8.3 against 7.2).
 template <class A, class F> static void norm_launches(A& a, const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, F launch) {
-  a.chunk = norm_chunk(n, nt);
+  const long long chunk = norm_chunk(n, nt);
   for (int ty = HOIC_F32; ty <= HOIC_BF16; ty++) {
-    a.type = ty; a.nt = 0;
-    long long blocks = 0;
+    a.type = ty; a.nt = 0; a.units = ty != HOIC_F32 && chunk < NORM_STEP ? 2 : 1; a.chunk = chunk * a.units;
+    long long blocks = 0, parts = 0;
     for (int i = 0; i < nt; i++) {
       if (type[i] == ty && n[i] > 0) {
-        a.t[a.nt].g = g[i]; a.t[a.nt].n = n[i]; a.t[a.nt].first = (int)blocks; a.nt++;
-        blocks += (n[i] + a.chunk - 1) / a.chunk;
+        a.t[a.nt].g = g[i]; a.t[a.nt].n = n[i]; a.t[a.nt].first = (int)blocks; a.t[a.nt].part = (int)parts; a.nt++;
+        blocks += (n[i] + a.chunk - 1) / a.chunk; parts += (n[i] + chunk - 1) / chunk;
       }
-      if (blocks && (a.nt == NORM_MAX || i == nt - 1)) { launch(blocks); a.nt = 0; blocks = 0; }
+      if (blocks && (a.nt == NORM_MAX || i == nt - 1)) { launch(blocks, parts); a.nt = 0; blocks = parts = 0; }
     }
   }
 }
@@ -2071,15 +2075,15 @@ static void norm_partial(const void* const* g, const int64_t* n, const uint8_t* 
   NormArgs a;
   a.part = part;
   const bool stream = list_bytes(n, type, nt) > STREAM_BYTES;
-  norm_launches(a, g, n, type, nt, [&](long long blocks) {
+  norm_launches(a, g, n, type, nt, [&](long long blocks, long long parts) {
     if (stream) hipLaunchKernelGGL(hoic_sumsq_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL(hoic_sumsq_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, st, a);
-    a.part += blocks;
+    a.part += parts;
   });
 }
 static void scale_launches(ScaleArgs& a, void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, hipStream_t st) {
   const bool stream = list_bytes(n, type, nt) > STREAM_BYTES;
-  norm_launches(a, (const void* const*)g, n, type, nt, [&](long long blocks) {
+  norm_launches(a, (const void* const*)g, n, type, nt, [&](long long blocks, long long) {
     if (stream) hipLaunchKernelGGL(hoic_scale_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL(hoic_scale_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, st, a);
   });
