@@ -186,6 +186,30 @@ def test_policy_loss_deviations_of_masked_rows_are_not_used(kind, mean):
 
 
 @gpu
+@pytest.mark.parametrize("M", [15, 16, 17, 4095, 4097, 12304, 16383, 16384, 16401, 65535, 65536, 65537, 70001, (1 << 20) + 5])
+def test_policy_loss_counts_the_valid_rows(M):
+    """flags as bool and as bytes of any value, at every alignment, in batches that every workgroup counts by itself and in larger ones: the
+    number is in ``info`` and divides the gradient (advantage 1, ratio 1: each valid row's d_mean is -(a - mean) / sigma^2 / n)"""
+    g = torch.Generator().manual_seed(M)
+    for shift, kind in ((0, "bool"), (1, "bytes"), (7, "bytes"), (3, "one"), (2, "none")):
+        flags = torch.zeros(M + 8, dtype=torch.uint8)
+        if kind == "one":
+            flags[shift + int(torch.randint(M, (), generator=g))] = 128
+        elif kind != "none":
+            keep = torch.rand(M, generator=g) < 0.6
+            flags[shift:shift + M][keep] = torch.randint(1, 256, (int(keep.sum()),), generator=g).to(torch.uint8) if kind == "bytes" else 1
+        n = int((flags[shift:shift + M] != 0).sum())
+        ok = (flags[shift:shift + M] != 0).cuda()
+        valid = flags.cuda()[shift:shift + M]
+        valid = valid.bool() if kind == "bool" else valid
+        mean = torch.zeros(M, 1, device="cuda")
+        o = rl.clipped_policy_loss_grad(mean, torch.zeros(1, device="cuda"), torch.ones(M, 1, device="cuda"), torch.ones(M, device="cuda"), valid=valid)
+        assert float(o.info[3]) == n
+        want = torch.where(ok, torch.full((M,), -1.0 / max(n, 1), device="cuda"), torch.zeros(M, device="cuda"))
+        assert torch.equal(o.d_mean[:, 0], want)
+
+
+@gpu
 def test_policy_loss_strides_and_expanded_rows():
     """row strides that are no multiple of the dimensions, columns that are not adjacent, one row expanded over the batch"""
     base = loss_case(200, 9, per_row=True, seed=11, device="cuda")
