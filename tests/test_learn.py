@@ -1183,6 +1183,44 @@ def test_adamw_unaligned_views_and_a_side_stream(bits):
         assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and torch.equal(flat[[0, 4098, 9000, 9002, 19999]], edges)
 
 
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_learners_on_two_streams(bits):
+    """loss -> gradients -> clipping -> step -> values of two learners, interleaved launch by launch on two streams, and one after the other on
+    one: the same bits (nothing is shared between calls)"""
+    def learner(seed):
+        x = loss_case(20000 if seed else 900, 32, mask=0.3, seed=seed, device="cuda")
+        mu, s = torch.nn.Parameter(x["mean"].nan_to_num(0.0)), torch.nn.Parameter(x["log_std"].clone())
+        return x, mu, s, optim.AdamW([mu, s], lr=1e-3, weight_decay=0.01, state_bits=bits, seed=seed)
+
+    def update(x, mu, s, opt):
+        o = rl.clipped_policy_loss_grad(**{**x, "mean": mu.detach(), "log_std": s.detach()}, kl_coef=0.2, weight=100.0)
+        mu.grad, s.grad = o.d_mean, o.d_log_std
+        norm = optim.clip_grad_norm_([mu, s], 0.7)
+        opt.step(max_norm=0.5)
+        return [o.loss, o.info, norm, opt.grad_norm, *sum(opt.state_values(), [])]
+
+    want = []
+    for seed in (0, 1):
+        w = learner(seed)
+        want.append([[t.clone() for t in update(*w)] for _ in range(6)] + [[w[1].detach(), w[2].detach()]])
+    streams, both = [torch.cuda.Stream(), torch.cuda.Stream()], [learner(0), learner(1)]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(6):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append([t.clone() for t in update(*both[k])])
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        got[k].append([both[k][1].detach(), both[k][2].detach()])
+        for a, b in zip(got[k], want[k]):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y)
+        assert bool(torch.isfinite(got[k][-1][0]).all())
+
+
 def test_rounding_bits_are_uniform():
     """chi-square of the hash's two halves in 256 cells (255 degrees of freedom: mean 255, std 22.6; 6 std allowed), and the
     correlation of neighbours, halves, steps and tensors (2^18 samples: std 2^-9; 6 std allowed)"""
