@@ -1519,8 +1519,8 @@ template <bool NT = false, class T> __device__ __forceinline__ void store4(T* __
 // Bound: HBM in large batches (524 287 x 32, a log-deviation per row, reference and mask: 91 us, 5.1 TB/s; a copy reaches 4.8), the
 // latency of load -> row sums -> store in an update's (53 248 x 32 shared: 10.3 us, two such steps a workgroup).  At most 1024
 // workgroups of equally many steps, four on each CU: 512 take 12.1 us against 11.9 at 53 248 rows and 118 against 92 at 524 287,
-// 2048 take 13.9 and 90 (twice the partial sums to join).  Dimensions that are no multiple of four are loaded one by one: a vector load where four are
-// left and single ones in the last lane costs both paths in every wavefront (26 dimensions 58.9 against 51.9 us, 33: 121 against 98).
+// 2048 take 13.9 and 90 (twice the partial sums to join).  Odd dimensions are loaded one by one: a vector load where four are left and single
+// ones in the last lane costs both paths in every wavefront (33 dimensions 121 against 98 us).
 struct PolicyLossArgs {
   hoic_policy_loss_args a;
   int lpr_log2;
@@ -1612,10 +1612,11 @@ __device__ __forceinline__ void store_log_std_grad(const hoic_policy_loss_args& 
   else if (a.t_std == HOIC_F16) ((_Float16*)a.d_log_std)[j] = (_Float16)(float)x;
   else ((__bf16*)a.d_log_std)[j] = (__bf16)(float)x;
 }
-// SHARED: one row of log-deviations (and of the reference's) for all rows: their terms are made once a dimension.  VEC: dims is a multiple of 4,
-// a lane's four dimensions are one load (else four).  Rows outside the batch read row 0's place and are dropped at the end: short
+// SHARED: one row of log-deviations (and of the reference's) for all rows: their terms are made once a dimension.  VEC: how many of a lane's
+// four dimensions one load takes, 4, 2 or 1 as dims is a multiple (524 288 rows of 26 float32 dimensions 48 us with 2, 55 with 1; 50 bf16 ones 86 / 122;
+// 26 with log-deviations per row 94 / 111).  Rows outside the batch read row 0's place and are dropped at the end: short
 // straight code matters more here than their traffic, a launch of a few rows waits for its instructions first of all.
-template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __launch_bounds__(PL_NT, 4) void hoic_policy_loss_kernel(PolicyLossArgs k) {
+template <class TM, bool SHARED, bool KL, bool GRAD, int VEC> __global__ __launch_bounds__(PL_NT, 4) void hoic_policy_loss_kernel(PolicyLossArgs k) {
   const hoic_policy_loss_args& a = k.a;
   __shared__ double red[PL_NT * 4];          // the dimensions' terms first, the row groups' sums in the end
   __shared__ double tail[4][PL_NT / 64];
@@ -1628,8 +1629,13 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
   for (int e = 0; e < 4; e++) off[e] = e < left ? j + e : 0;
   auto load = [&](const auto* x, long long at) {
     f32x4 r;
-    if (VEC) {
+    if (VEC == 4) {
       r = __builtin_convertvector(*(const typename vec4<std::decay_t<decltype(*x)>>::type*)(x + at + off[0]), f32x4);
+    } else if (VEC == 2) {
+      typedef std::decay_t<decltype(*x)> T;
+      typedef T t2 __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+      const t2 u = *(const t2*)(x + at + off[0]), v = *(const t2*)(x + at + off[2]);
+      r[0] = (float)u[0]; r[1] = (float)u[1]; r[2] = (float)v[0]; r[3] = (float)v[1];
     } else {
 #pragma unroll
       for (int e = 0; e < 4; e++) r[e] = (float)x[at + off[e]];
@@ -1755,8 +1761,12 @@ template <class TM, bool SHARED, bool KL, bool GRAD, bool VEC> __global__ __laun
       if (in) {
         auto store = [&](auto* out, f32x4 v) {
           typedef std::decay_t<decltype(*out)> T;
-          if (VEC) { if (left > 0) *(typename vec4<T>::type*)(out + j) = __builtin_convertvector(v, typename vec4<T>::type); }
-          else {
+          typedef T t2 __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+          if (VEC == 4) { if (left > 0) *(typename vec4<T>::type*)(out + j) = __builtin_convertvector(v, typename vec4<T>::type); }
+          else if (VEC == 2) {
+            if (left > 0) *(t2*)(out + j) = t2{(T)v[0], (T)v[1]};
+            if (left > 2) *(t2*)(out + j + 2) = t2{(T)v[2], (T)v[3]};
+          } else {
 #pragma unroll
             for (int e = 0; e < 4; e++) if (e < left) out[j + e] = (T)v[e];
           }
@@ -1816,8 +1826,9 @@ __global__ __launch_bounds__(256) void hoic_policy_loss_finish_kernel(PolicyLoss
 
 extern "C" int64_t hoic_policy_loss_scratch_bytes(int32_t dims) { return dims <= 0 ? 0 : (int64_t)PL_BLOCKS * (dims + 4) * 8 + PL_COUNTS * 4; }
 template <class TM, bool SHARED, bool KL, bool GRAD> static void launch_policy_loss(const PolicyLossArgs& k, hipStream_t st) {
-  if (k.a.dims % 4 == 0) hipLaunchKernelGGL((hoic_policy_loss_kernel<TM, SHARED, KL, GRAD, true>), dim3(k.nb), dim3(PL_NT), 0, st, k);
-  else hipLaunchKernelGGL((hoic_policy_loss_kernel<TM, SHARED, KL, GRAD, false>), dim3(k.nb), dim3(PL_NT), 0, st, k);
+  if (k.a.dims % 4 == 0) hipLaunchKernelGGL((hoic_policy_loss_kernel<TM, SHARED, KL, GRAD, 4>), dim3(k.nb), dim3(PL_NT), 0, st, k);
+  else if (k.a.dims % 2 == 0) hipLaunchKernelGGL((hoic_policy_loss_kernel<TM, SHARED, KL, GRAD, 2>), dim3(k.nb), dim3(PL_NT), 0, st, k);
+  else hipLaunchKernelGGL((hoic_policy_loss_kernel<TM, SHARED, KL, GRAD, 1>), dim3(k.nb), dim3(PL_NT), 0, st, k);
 }
 template <class TM, bool SHARED, bool KL> static void launch_policy_loss(const PolicyLossArgs& k, hipStream_t st) {
   if (k.a.d_mean) launch_policy_loss<TM, SHARED, KL, true>(k, st); else launch_policy_loss<TM, SHARED, KL, false>(k, st);
