@@ -177,17 +177,21 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW: a parameter whose elements do not fill their memory (an expanded or cut view)")
         super().add_param_group(group)
 
-    def _make_state(self, p, step=0):
+    def _make_state(self, p, step=0, filled=True):
         bits, s = self.defaults["state_bits"], {}
         s["step"] = torch.full((), step, dtype=torch.int32, device=p.device) if self.defaults["capturable"] else step
         if not p.is_contiguous():
             s["order"] = _strides(p)
         for key in ("exp_avg", "exp_avg_sq"):
             if bits == 32:
-                s[key] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+                s[key] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format, requires_grad=False)
             else:
-                s[key] = torch.zeros(p.numel(), dtype=torch.uint8, device=p.device)
-                s[key + "_scale"] = torch.full(((p.numel() + BLOCK - 1) // BLOCK,), _EMPTY_SCALE, dtype=torch.float32, device=p.device)
+                s[key] = torch.empty(p.numel(), dtype=torch.uint8, device=p.device)
+                s[key + "_scale"] = torch.empty((p.numel() + BLOCK - 1) // BLOCK, dtype=torch.float32, device=p.device)
+            if filled:
+                s[key].zero_()
+                if bits == 8:
+                    s[key + "_scale"].fill_(_EMPTY_SCALE)
         return s
 
     def _new_order(self, p, s, capturing):
@@ -218,7 +222,7 @@ class AdamW(torch.optim.Optimizer):
                 continue
             if set(s) - {"step", "order"} != want:
                 raise ValueError(f"a state of {sorted(s)}: this optimiser holds {sorted(want)} (state_bits={self.defaults['state_bits']})")
-            mine = self._make_state(p, int(s["step"]))
+            mine = self._make_state(p, int(s["step"]), filled=False)
             if self.defaults["state_bits"] == 8 and list(s.get("order", ())) != list(mine.get("order", ())):
                 raise ValueError("8-bit moments of a parameter that lay in another order in memory")
             for key in want:
