@@ -7,7 +7,6 @@ Everything runs on the current stream of the tensors' device and nothing synchro
 """
 from __future__ import annotations
 
-import itertools
 import struct
 
 import torch
@@ -353,28 +352,33 @@ class AdamW(torch.optim.Optimizer):
             return [], []
         if bits == 32 and all(s for _, s in states):
             return [s["exp_avg"] for _, s in states], [s["exp_avg_sq"] for _, s in states]
-        new = lambda p: torch.empty_like(p, dtype=torch.float32, requires_grad=False)
-        ms, vs, work, ptrs, at = [], [], {}, None, states[0][0].device
-        if bits == 8 and all([s and p.is_contiguous() and p.device == at for p, s in states]):
+        changed = "AdamW: 8-bit moments of a parameter whose size, device or order in memory has changed since"
+        at, work = states[0][0].get_device(), {}
+        if bits == 8 and all([s and p.is_contiguous() and p.get_device() == at for p, s in states]):
             # one buffer, cut into the parameters' shapes (an allocation a parameter costs more than the launch)
             sizes = [p.numel() for p, _ in states]
-            buf = torch.empty(2 * sum(sizes), dtype=torch.float32, device=at)
-            shape = lambda xs: [x if p.dim() == 1 else x.view(p.shape) for (p, _), x in zip(states, xs)]
-            cut, k = torch.split_with_sizes(buf, sizes + sizes), len(sizes)
-            ms, vs, ptrs = shape(cut[:k]), shape(cut[k:]), [buf.data_ptr() + 4 * x for x in itertools.accumulate(sizes + sizes, initial=0)]
-        for i, (p, s) in enumerate(states):
-            if ptrs is None:
-                ms.append(s["exp_avg"] if s and bits == 32 else new(p) if s else new(p).zero_())
-                vs.append(s["exp_avg_sq"] if s and bits == 32 else new(p) if s else new(p).zero_())
-            if s and bits == 8:
-                m, dev, n = s["exp_avg"], p.device, p.numel()
-                if m.numel() != n or m.device != dev or s.get("order") != (None if ptrs or p.is_contiguous() else _strides(p)):
-                    raise ValueError("AdamW: 8-bit moments of a parameter whose size, device or order in memory has changed since")
-                rows = work.get(dev)
-                if rows is None:
-                    rows = work[dev] = []
-                rows += (ptrs[i] if ptrs else ms[i].data_ptr(), ptrs[k + i] if ptrs else vs[i].data_ptr(), m.data_ptr(), s["exp_avg_sq"].data_ptr(),
-                         s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr(), n, 1, 0, 0)
+            n, k = sum(sizes), len(sizes)
+            buf = torch.empty(2 * n, dtype=torch.float32, device=states[0][0].device)
+            mp, rows = buf.data_ptr(), []
+            for (_, s), size in zip(states, sizes):
+                m = s["exp_avg"]
+                if m.numel() != size or m.get_device() != at or "order" in s:
+                    raise ValueError(changed)
+                rows += (mp, mp + 4 * n, m.data_ptr(), s["exp_avg_sq"].data_ptr(), s["exp_avg_scale"].data_ptr(), s["exp_avg_sq_scale"].data_ptr(), size, 1, 0, 0)
+                mp += 4 * size
+            work[buf.device] = rows
+            out = [x if p.dim() == 1 else x.view(p.shape) for (p, _), x in zip(states + states, torch.split_with_sizes(buf, sizes + sizes))]
+            ms, vs = out[:k], out[k:]
+        else:
+            new = lambda p: torch.empty_like(p, dtype=torch.float32, requires_grad=False)
+            ms = [s["exp_avg"] if s and bits == 32 else new(p) if s else new(p).zero_() for p, s in states]
+            vs = [s["exp_avg_sq"] if s and bits == 32 else new(p) if s else new(p).zero_() for p, s in states]
+            for (p, s), m, v in zip(states, ms, vs):
+                if s and bits == 8:
+                    if s["exp_avg"].numel() != p.numel() or s["exp_avg"].device != p.device or s.get("order") != (None if p.is_contiguous() else _strides(p)):
+                        raise ValueError(changed)
+                    work.setdefault(p.device, []).extend((m.data_ptr(), v.data_ptr(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), s["exp_avg_scale"].data_ptr(),
+                                                          s["exp_avg_sq_scale"].data_ptr(), p.numel(), 1, 0, 0))
         for dev, rows in work.items():
             with lib.Launch(dev) as st:
                 lib._chk(lib.load().hoic_adamw_values(_pack(rows), len(rows) // 10, st), "hoic_adamw_values")
