@@ -266,11 +266,12 @@ class AdamW(torch.optim.Optimizer):
                 dtype, at, n, contiguous = p.dtype, p.get_device(), p.numel(), p.is_contiguous()
                 if g.dtype is not dtype or g.layout is not torch.strided or g.numel() != n or g.get_device() != at:
                     raise ValueError(f"AdamW: a gradient {tuple(g.shape)} {g.dtype} on {g.device} (dense ones only) of a parameter {tuple(p.shape)} {dtype} on {p.device}")
-                if not (contiguous and g.is_contiguous()) and _strides(g) != _strides(p):
-                    if not _dense(p) or g.shape != p.shape:
+                if not (contiguous and g.is_contiguous()):
+                    if not _dense(p) or g.shape != p.shape:          # (dense when it was added, but ``p.data`` may have been replaced since)
                         raise ValueError(f"AdamW: a parameter {tuple(p.shape)} whose elements do not fill their memory, or a gradient of another shape, {tuple(g.shape)}")
-                    g = torch.empty_like(p, requires_grad=False).copy_(g.detach())          # the parameter's order of elements
-                    held.append(g)
+                    if _strides(g) != _strides(p):
+                        g = torch.empty_like(p, requires_grad=False).copy_(g.detach())      # the parameter's order of elements
+                        held.append(g)
                 s = state[p]
                 if not s or capturing:
                     if capturing and not capturable:

@@ -1,0 +1,102 @@
+"""Calls of the learning operators (hoic_amd.rl, hoic_amd.optim) that their documentation allows or has to refuse, beside tests/test_learn.py: what
+must reach no kernel is tested on the CPU, with the entry points replaced by recorders."""
+import copy
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import test_learn as T
+from hoic_amd import lib, optim, rl
+
+gpu = pytest.mark.gpu
+U32 = T.U32
+
+
+class Recorder:
+    """the library with every entry point a recorder of its calls; the gradient lists' sizes are the real ones"""
+
+    def __init__(self):
+        self.calls, self.real = [], lib.load()
+
+    def hoic_grad_norm_parts(self, sizes, n):
+        return self.real.hoic_grad_norm_parts(sizes, n)
+
+    def __getattr__(self, name):
+        return lambda *args: self.calls.append((name, args)) or 0
+
+
+class NoLaunch:
+    def __init__(self, dev):
+        pass
+
+    def __enter__(self):
+        return 0
+
+    def __exit__(self, *exc):
+        pass
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    """optim on CPU tensors that pass for tensors of cuda:0"""
+    r = Recorder()
+    monkeypatch.setattr(lib, "load", lambda: r)
+    monkeypatch.setattr(lib, "Launch", NoLaunch)
+    monkeypatch.setattr(optim, "_check", lambda t, what: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    return r
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("stepped", [False, True])
+def test_adamw_cut_or_expanded_parameters_reach_no_kernel(recorder, bits, stepped):
+    """``p.data`` replaced by a view whose elements do not fill their memory, the gradient a view of the same strides: a kernel that takes the
+    elements in a row would write its neighbours (a cut view) or past the allocation (an expanded one)"""
+    cut = lambda: torch.randn(6, 8)[:, :4]
+    views = [(cut(), cut()), (torch.randn(1, 4).expand(6, 4), torch.randn(1, 4).expand(6, 4)), (torch.randn(6, 1).expand(6, 4), torch.randn(6, 1).expand(6, 4)),
+             (torch.randn(48)[::2].view(6, 4), torch.randn(48)[::2].view(6, 4)), (torch.randn(8, 6).t()[:, ::2], torch.randn(8, 6).t()[:, ::2])]
+    for data, grad in views:
+        p = torch.nn.Parameter(torch.zeros(6, 4)); p.grad = torch.ones(6, 4)
+        opt = optim.AdamW([p], state_bits=bits)
+        if stepped:
+            opt.step()
+            assert [name for name, _ in recorder.calls] == ["hoic_adamw"]
+            recorder.calls.clear()
+        before = {k: v.clone() if torch.is_tensor(v) else v for k, v in opt.state[p].items()} if stepped else {}
+        keep = data.clone()
+        p.grad = None
+        p.data = data
+        p.grad = grad
+        for kw in ({}, {"max_norm": 1.0}):
+            with pytest.raises(ValueError, match="fill their memory"):
+                opt.step(**kw)
+            assert not recorder.calls and torch.equal(data, keep)
+        state = opt.state[p]
+        assert state.keys() == before.keys() and all(torch.equal(state[k], v) if torch.is_tensor(v) else state[k] == v for k, v in before.items())
+    # a gradient of the parameter's strides and number of elements, but of another shape
+    p = torch.nn.Parameter(torch.randn(3, 2))
+    p.grad = torch.zeros(16).as_strided((3, 2), (1, 2))
+    opt = optim.AdamW([p], state_bits=bits)
+    p.data = torch.randn(3, 2).t()
+    with pytest.raises(ValueError, match="another shape"):
+        opt.step()
+    assert not recorder.calls
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_dense_parameters_of_any_order_reach_the_kernel(recorder, bits):
+    """views that fill one stretch of memory are taken as they are, a gradient of another order in a copy of the parameter's"""
+    base, gbase = torch.randn(40), torch.randn(40)
+    p = torch.nn.Parameter(base[7:31].view(4, 6).t()); p.grad = gbase[5:29].view(4, 6).t()
+    optim.AdamW([p], state_bits=bits).step()
+    (name, (rows, n, _, _)), = recorder.calls
+    row = np.frombuffer(rows, np.int64)
+    assert name == "hoic_adamw" and n == 1 and row[0] == p.data_ptr() and row[1] == p.grad.data_ptr() and row[6] == 24
+    recorder.calls.clear()
+    p.grad = torch.randn(6, 4)
+    optim.AdamW([p], state_bits=bits).step()
+    (name, (rows, n, _, _)), = recorder.calls
+    assert np.frombuffer(rows, np.int64)[1] != p.grad.data_ptr()
