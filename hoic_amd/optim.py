@@ -81,6 +81,15 @@ def _bound(max_norm):
     return b
 
 
+def _check_options(group):
+    """options of torch.optim.Adam's / AdamW's groups that the step does not have"""
+    for key in ("maximize", "amsgrad"):
+        if group.get(key):
+            raise ValueError(f"AdamW: {key}=True is not supported")
+    if group.get("weight_decay") and group.get("decoupled_weight_decay") is False:
+        raise ValueError("AdamW: its weight decay is decoupled, these options ask for a coupled one (torch.optim.Adam with weight_decay)")
+
+
 def grad_norm(tensors):
     """sqrt(sum of squares) over a list of tensors (float32 / float16 / bfloat16, any mix, one device) as a float32 scalar on the
     device; 64-bit sums in a fixed order: the same bits in every run."""
@@ -166,6 +175,7 @@ class AdamW(torch.optim.Optimizer):
         for key in ("state_bits", "capturable"):
             if group.get(key, self.defaults[key]) != self.defaults[key]:
                 raise ValueError(f"{key} is one for all groups")
+        _check_options({**self.defaults, **group})
         memory = {p.data_ptr() for g in self.param_groups for p in g["params"]}
         for p in ps:
             _check(p, "AdamW")
@@ -206,9 +216,11 @@ class AdamW(torch.optim.Optimizer):
             s["order"] = _strides(p)
 
     def load_state_dict(self, state_dict):
-        """Also takes the state of a ``torch.optim.Adam`` / ``AdamW`` over the same parameters (``state_bits=32``).  The moments are
-        copied, and keep their own types whatever the parameters' are.  (8-bit ones need parameters in the order in memory that they
-        were made for.)"""
+        """Also takes the state of a ``torch.optim.Adam`` / ``AdamW`` over the same parameters (``state_bits=32``; refused with options that
+        this step does not have: ``maximize``, ``amsgrad``, ``Adam``'s coupled weight decay).  The moments are copied, and keep their own
+        types whatever the parameters' are.  (8-bit ones need parameters in the order in memory that they were made for.)"""
+        for g in state_dict["param_groups"]:
+            _check_options(g)
         old = [p for g in state_dict["param_groups"] for p in g["params"]]
         new = [p for g in self.param_groups for p in g["params"]]
         want = {"exp_avg", "exp_avg_sq"} if self.defaults["state_bits"] == 32 else {"exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale"}

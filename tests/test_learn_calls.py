@@ -100,3 +100,34 @@ def test_adamw_dense_parameters_of_any_order_reach_the_kernel(recorder, bits):
     optim.AdamW([p], state_bits=bits).step()
     (name, (rows, n, _, _)), = recorder.calls
     assert np.frombuffer(rows, np.int64)[1] != p.grad.data_ptr()
+
+
+@pytest.mark.parametrize("stepped", [False, True])
+def test_adamw_refuses_options_that_it_does_not_have(recorder, stepped):
+    """a group of torch's optimisers that maximises, keeps maxima or couples its weight decay is not taken over in silence, with a state or
+    before the first step; one without them is, with its moments"""
+    def foreign(cls, **kw):
+        q = torch.nn.Parameter(torch.randn(5, 3))
+        o = cls([q], lr=0.25, **kw)
+        if stepped:
+            q.grad = torch.randn(5, 3)
+            o.step()
+        return o.state_dict()
+
+    p = torch.nn.Parameter(torch.randn(5, 3))
+    opt = optim.AdamW([p], lr=0.5)
+    for cls, kw, word in ((torch.optim.AdamW, dict(maximize=True), "maximize"), (torch.optim.Adam, dict(maximize=True), "maximize"),
+                          (torch.optim.AdamW, dict(amsgrad=True), "amsgrad"), (torch.optim.Adam, dict(weight_decay=0.1), "decoupled")):
+        with pytest.raises(ValueError, match=word):
+            opt.load_state_dict(foreign(cls, **kw))
+        assert opt.param_groups[0]["lr"] == 0.5 and not opt.state.get(p)
+        group = {k: v for k, v in kw.items()} | ({"decoupled_weight_decay": False} if word == "decoupled" else {})
+        with pytest.raises(ValueError, match=word):
+            opt.add_param_group(dict(params=[torch.nn.Parameter(torch.randn(2))], **group))
+    for cls, kw in ((torch.optim.AdamW, dict(weight_decay=0.1)), (torch.optim.Adam, {})):
+        sd = foreign(cls, **kw)
+        opt.load_state_dict(sd)
+        assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["weight_decay"] == kw.get("weight_decay", 0.0)
+        if stepped:
+            assert opt.state[p]["step"] == 1 and torch.equal(opt.state[p]["exp_avg"], sd["state"][0]["exp_avg"])
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
