@@ -296,11 +296,12 @@ class _ClippedPolicyLoss(torch.autograd.Function):
     rows would underflow unscaled)."""
 
     @staticmethod
-    def forward(ctx, kl_coef, clip, mean, log_std, *rest):
+    def forward(ctx, wanted, kl_coef, clip, mean, log_std, *rest):
+        # wanted: whether a backward call can follow (ctx.needs_input_grad says nothing about the grad mode)
         actions, advantages, fixed, ref_mean, ref_log_std, valid = rest
         x = (mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid)
-        grad = (ctx.needs_input_grad[2] or ctx.needs_input_grad[3]) and mean.dtype == torch.float32
-        loss, info, ctx.count, d_mean, d_log_std, log_probs = _policy_loss_launch(x, kl_coef, 1.0, grad, want_count=not grad)
+        grad = wanted and mean.dtype == torch.float32
+        loss, info, ctx.count, d_mean, d_log_std, log_probs = _policy_loss_launch(x, kl_coef, 1.0, grad, want_count=wanted and not grad)
         ctx.save_for_backward(mean, log_std, *rest)
         ctx.consts, ctx.grads = (kl_coef, clip), (d_mean, d_log_std) if grad else None
         ctx.mark_non_differentiable(*((info,) if log_probs is None else (info, log_probs)))
@@ -324,7 +325,7 @@ class _ClippedPolicyLoss(torch.autograd.Function):
             kl_coef, clip = ctx.consts
             *_, d_mean, d_log_std, _ = _policy_loss_launch((mean, log_std, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid), kl_coef, 1.0,
                                                            True, upstream=g, count=ctx.count)
-        return (None, None, d_mean, d_log_std) + (None,) * 6
+        return (None, None, None, d_mean, d_log_std) + (None,) * 6
 
 
 def _policy_loss_tensors(x, kl_coef):
@@ -382,7 +383,8 @@ def clipped_policy_loss(mean, log_std, actions, advantages, fixed_log_probs=None
         return _policy_loss_tensors(x, kl_coef)
     mean2, log_std2, actions, advantages, fixed, clip, ref_mean, ref_log_std, valid = x
     const = [t.detach() if t is not None and t.requires_grad else t for t in (actions, advantages, fixed, ref_mean, ref_log_std, valid)]
-    return PolicyLoss(*_ClippedPolicyLoss.apply(float(kl_coef), clip, mean2, log_std2, *const))
+    wanted = torch.is_grad_enabled() and (mean2.requires_grad or log_std2.requires_grad)
+    return PolicyLoss(*_ClippedPolicyLoss.apply(wanted, float(kl_coef), clip, mean2, log_std2, *const))
 
 
 def clipped_policy_loss_grad(mean, log_std, actions, advantages, fixed_log_probs=None, clip_epsilon=0.2, *, ref_mean=None, ref_log_std=None,

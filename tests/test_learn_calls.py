@@ -131,3 +131,27 @@ def test_adamw_refuses_options_that_it_does_not_have(recorder, stepped):
         if stepped:
             assert opt.state[p]["step"] == 1 and torch.equal(opt.state[p]["exp_avg"], sd["state"][0]["exp_avg"])
     opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+
+
+@pytest.mark.parametrize("mean", [torch.float32, torch.bfloat16])
+def test_policy_loss_makes_gradients_only_for_a_backward_call(monkeypatch, mean):
+    """a value under no_grad, or of tensors that require no gradient, is a pass without gradients, whether or not leaves stand behind it"""
+    asked = []
+
+    def launch(x, kl_coef, weight, grad, upstream=None, count=None, want_count=False):
+        asked.append((grad, want_count))
+        made = lambda t: torch.zeros_like(t) if grad else None
+        return torch.zeros(()), torch.zeros(4), torch.ones(1, dtype=torch.float64) if want_count else None, made(x[0]), made(x[1]), None
+
+    monkeypatch.setattr(rl, "_on_kernel", lambda t: True)
+    monkeypatch.setattr(rl, "_policy_loss_launch", launch)
+    x = T.loss_case(7, 3, mean={torch.float32: "f32", torch.bfloat16: "bf16"}[mean])
+    direct = mean == torch.float32                    # (gradients of 16-bit means are made in the backward call, which needs the count)
+    for leaves in ((), ("mean",), ("log_std",), ("mean", "log_std")):
+        y = {**x, **{k: x[k].detach().requires_grad_() for k in leaves}}
+        with torch.no_grad():
+            assert not rl.clipped_policy_loss(**y, kl_coef=0.3).loss.requires_grad
+        assert asked.pop() == (False, False) and not asked
+        p = rl.clipped_policy_loss(**y, kl_coef=0.3)
+        assert p.loss.requires_grad == bool(leaves)
+        assert asked.pop() == ((direct, not direct) if leaves else (False, False)) and not asked
