@@ -332,7 +332,8 @@ def _policy_loss_tensors(x, kl_coef):
     """The loss as tensor operations (CPU and float64 tensors; what the kernel computes, row by row)"""
     mean, log_std, actions, advantages, fixed, (lo, hi), ref_mean, ref_log_std, valid = x
     advantages, fixed, valid = (None if t is None else t.reshape(-1) for t in (advantages, fixed, valid))
-    ref_mean, ref_log_std = (None if t is None else t.detach() for t in (ref_mean, ref_log_std))
+    # differentiable in the mean and log_std alone, as the kernel's form
+    actions, advantages, fixed, ref_mean, ref_log_std = (None if t is None else t.detach() for t in (actions, advantages, fixed, ref_mean, ref_log_std))
     if valid is not None:                          # rows outside the batch may hold anything: they are left out, not multiplied by 0
         keep = valid.bool()
         cut = lambda t: t if t is None or (t.shape[0] != keep.shape[0]) else t[keep]

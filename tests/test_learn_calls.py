@@ -155,3 +155,17 @@ def test_policy_loss_makes_gradients_only_for_a_backward_call(monkeypatch, mean)
         p = rl.clipped_policy_loss(**y, kl_coef=0.3)
         assert p.loss.requires_grad == bool(leaves)
         assert asked.pop() == ((direct, not direct) if leaves else (False, False)) and not asked
+
+
+def test_policy_loss_tensor_form_is_differentiable_in_the_policy_alone():
+    """actions, advantages (a value network's, say), old log-probabilities and the reference get no gradient on the CPU either"""
+    others = ("actions", "advantages", "fixed_log_probs", "ref_mean", "ref_log_std")
+    x = {k: v.double() if v is not None and v.dtype != torch.bool else v for k, v in T.loss_case(9, 4, seed=3).items()}
+    want = T.loss_reference(x, kl_coef=0.3)
+    y = {k: v.detach().requires_grad_() if k != "valid" else v for k, v in x.items()}
+    rl.clipped_policy_loss(**y, kl_coef=0.3).loss.backward()
+    assert all(y[k].grad is None for k in others)
+    for k in ("mean", "log_std"):
+        torch.testing.assert_close(y[k].grad, want["d_" + k], rtol=1e-12, atol=1e-13)
+    z = {k: v.detach().requires_grad_(k in others) if k != "valid" else v for k, v in x.items()}
+    assert not rl.clipped_policy_loss(**z, kl_coef=0.3).loss.requires_grad
