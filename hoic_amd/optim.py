@@ -317,6 +317,10 @@ class AdamW(torch.optim.Optimizer):
             if bound is not None:
                 self.grad_norm = torch.zeros(())
             return loss
+        for at, gi, _ in work:               # before any launch: a step is taken by all groups or by none
+            lr = self.param_groups[gi]["lr"]
+            if isinstance(lr, torch.Tensor) and (not capturable or lr.get_device() != at or lr.dtype != torch.float32 or lr.numel() != 1):
+                raise ValueError("lr: a float, or with capturable=True a float32 tensor of one element on the parameters' device")
         L = lib.load()
         buf_ptr = norm_ptr = parts = 0
         if bound is not None:
@@ -342,8 +346,6 @@ class AdamW(torch.optim.Optimizer):
             lr, (b1, b2) = group["lr"], group["betas"]
             lr_ptr = 0
             if isinstance(lr, torch.Tensor):
-                if not capturable or lr.device != dev or lr.dtype != torch.float32 or lr.numel() != 1:
-                    raise ValueError("lr: a float, or with capturable=True a float32 tensor of one element on the parameters' device")
                 lr, lr_ptr = 0.0, lr.data_ptr()
             consts = torch.empty(4 * n, dtype=torch.float32, device=dev) if capturable else None
             a = lib.ADAMW_ARGS.pack(TYPES[dtype], bits, lr, b1, b2, group["eps"], group["weight_decay"], lr_ptr,

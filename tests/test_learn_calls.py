@@ -169,3 +169,20 @@ def test_policy_loss_tensor_form_is_differentiable_in_the_policy_alone():
         torch.testing.assert_close(y[k].grad, want["d_" + k], rtol=1e-12, atol=1e-13)
     z = {k: v.detach().requires_grad_(k in others) if k != "valid" else v for k, v in x.items()}
     assert not rl.clipped_policy_loss(**z, kl_coef=0.3).loss.requires_grad
+
+
+def test_adamw_checks_every_group_before_the_first_launch(recorder):
+    """a learning rate that the second group cannot use: nothing is launched, no step counted, so that the corrected call takes one step"""
+    ps = [torch.nn.Parameter(torch.randn(4)) for _ in range(2)]
+    for p in ps:
+        p.grad = torch.randn(4)
+    opt = optim.AdamW([dict(params=[p]) for p in ps])
+    for lr in (torch.tensor(0.1), torch.zeros(2), torch.tensor(0.1, dtype=torch.float64)):
+        opt.param_groups[1]["lr"] = lr
+        for kw in ({}, {"max_norm": 1.0}):
+            with pytest.raises(ValueError, match="lr"):
+                opt.step(**kw)
+            assert not recorder.calls
+    opt.param_groups[1]["lr"] = 0.1
+    opt.step()
+    assert [name for name, _ in recorder.calls] == ["hoic_adamw"] * 2 and all(opt.state[p]["step"] == 1 for p in ps)
