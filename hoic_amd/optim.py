@@ -176,14 +176,13 @@ class AdamW(torch.optim.Optimizer):
             if group.get(key, self.defaults[key]) != self.defaults[key]:
                 raise ValueError(f"{key} is one for all groups")
         _check_options({**self.defaults, **group})
-        memory = {p.data_ptr() for g in self.param_groups for p in g["params"]}
         for p in ps:
             _check(p, "AdamW")
-            if p.numel() and p.data_ptr() in memory:
-                raise ValueError("AdamW: two parameters in the same memory")
-            memory.add(p.data_ptr())
             if not _dense(p):
                 raise ValueError("AdamW: a parameter whose elements do not fill their memory (an expanded or cut view)")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in [p for g in self.param_groups for p in g["params"]] + ps if p.numel())
+        if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+            raise ValueError("AdamW: two parameters in the same memory")
         super().add_param_group(group)
 
     def _make_state(self, p, step=0, filled=True):

@@ -186,3 +186,19 @@ def test_adamw_checks_every_group_before_the_first_launch(recorder):
     opt.param_groups[1]["lr"] = 0.1
     opt.step()
     assert [name for name, _ in recorder.calls] == ["hoic_adamw"] * 2 and all(opt.state[p]["step"] == 1 for p in ps)
+
+
+def test_adamw_refuses_parameters_that_overlap_in_any_group(recorder):
+    """views that share some elements, in one group or in two, of one type or of two: an element would be stepped twice; neighbours are taken"""
+    flat = torch.randn(64)
+    make = lambda a, b, dtype=torch.float32: torch.nn.Parameter(flat[a:b].view(dtype))
+    for first, second in (((0, 8), (7, 12)), ((7, 12), (0, 8)), ((0, 8), (0, 8)), ((0, 32), (4, 5)), ((4, 5), (0, 32))):
+        for dtype in (torch.float32, torch.bfloat16):
+            with pytest.raises(ValueError, match="same memory"):
+                optim.AdamW([make(*first), make(*second, dtype)])
+            opt = optim.AdamW([make(*first)])
+            with pytest.raises(ValueError, match="same memory"):
+                opt.add_param_group(dict(params=make(*second, dtype)))
+            assert len(opt.param_groups) == 1
+    opt = optim.AdamW([make(8, 16), make(0, 8), make(8, 8)])
+    opt.add_param_group(dict(params=[make(16, 20, torch.bfloat16), make(16, 16)]))
