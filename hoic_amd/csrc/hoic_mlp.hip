@@ -1891,7 +1891,9 @@ template <class E, int MAXT> __device__ __forceinline__ int list_find(const E (&
 // that uses the factor (Joint): that saves the launch between (JOIN_LAUNCHES, JOIN_BLOCKS).
 struct Joint { const double* parts; int nparts; double bound; float* norm; };      // parts NULL: no clipping; nparts 0: parts = {norm, factor}
 __device__ __forceinline__ double2 norm_factor(double sum, double bound) {
-  const double t = sqrt(sum), c = bound / (t + 1e-6);
+  double t = sqrt(sum);
+  if ((float)t == INFINITY) t = INFINITY;        // (as float32, the norm that the caller is shown: the factor is then 0)
+  const double c = bound / (t + 1e-6);
   return make_double2(t, c > 1. ? 1. : c);       // (a NaN norm leaves a NaN factor)
 }
 // all of a 256-lane workgroup: {norm, factor}
@@ -2258,7 +2260,7 @@ template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw32_
   float cl = 1.f;
   if (a.clip.parts) {
     const double2 f = join_norm(a.clip);
-    if (!((float)f.x < INFINITY)) return;      // (as float32, the norm that the caller is shown)
+    if (!(f.x < INFINITY)) return;
     cl = (float)f.y;
   }
   const AdamConsts c = adam_consts(a, t);
@@ -2397,7 +2399,7 @@ template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw8_k
   double cl = 1.;
   if (a.clip.parts) {
     const double2 f = join_norm(a.clip);
-    if (!((float)f.x < INFINITY)) return;      // (as float32, the norm that the caller is shown)
+    if (!(f.x < INFINITY)) return;
     cl = f.y;
   }
   const AdamConsts c = adam_consts(a, t);

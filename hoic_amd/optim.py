@@ -114,7 +114,7 @@ def grad_norm(tensors):
 def clip_grad_norm_(parameters, max_norm):
     """``torch.nn.utils.clip_grad_norm_`` (norm 2) on this package's kernels: the gradients times min(1, max_norm / (norm + 1e-6)) in
     place, the norm before clipping returned as a float32 scalar on the device.  A factor of 1 reads and writes nothing; a norm
-    that is not finite gives the factor that the formula gives (0 or NaN)."""
+    that is not finite in float32 gives the factor that the formula gives (0 or NaN)."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     bound = _bound(max_norm)

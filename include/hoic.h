@@ -383,7 +383,8 @@ int32_t hoic_policy_loss(const hoic_policy_loss_args* a, void* stream);
  * hoic_grad_norm: the norm; d_buf[0..1] = {norm, 1} afterwards.
  * hoic_grad_norm_partial: the parts alone, for hoic_adamw (d_norm_buf, norm_parts) to join.
  * hoic_scale_list: g *= *d_factor (device float; 1 touches nothing).
- * hoic_clip_grads: g *= min(1, bound / (norm + 1e-6)) in place (a factor of 1 touches nothing).
+ * hoic_clip_grads: g *= min(1, bound / (norm + 1e-6)) in place (a factor of 1 touches nothing; a norm past float32's range counts as
+ * infinite: factor 0).
  * Tensors that are written share no memory (HOIC_ERR_ARG otherwise; hoic_adamw's parameters too). */
 int64_t hoic_grad_norm_parts(const int64_t* n, int32_t nt);
 int32_t hoic_grad_norm(const void* const* g, const int64_t* n, const uint8_t* type, int32_t nt, double* d_buf, float* d_norm, void* stream);

@@ -202,3 +202,22 @@ def test_adamw_refuses_parameters_that_overlap_in_any_group(recorder):
             assert len(opt.param_groups) == 1
     opt = optim.AdamW([make(8, 16), make(0, 8), make(8, 8)])
     opt.add_param_group(dict(params=[make(16, 20, torch.bfloat16), make(16, 16)]))
+
+
+@gpu
+@pytest.mark.parametrize("n", [60, 5 << 20])
+def test_clipping_by_a_norm_past_float32(n):
+    """gradients whose norm float32 cannot hold: the norm that is shown is infinite, and the factor is that norm's, 0, as torch's own clipping
+    gives; a norm just inside the range still gives its quotient (lists joined by the scaling launch and in front of it)"""
+    for parts in (1, min(n, 300)):
+        g = torch.full((n // parts * parts,), 3e38, device="cuda")
+        ps = [torch.nn.Parameter(torch.empty_like(x)) for x in g.split(n // parts)]
+        for p, x in zip(ps, g.split(n // parts)):
+            p.grad = x
+        assert math.isinf(float(optim.clip_grad_norm_(ps, 40.0))) and not bool(g.any())
+        g.zero_()
+        g[::g.numel() // 4][:4] = -1.5e38               # norm 3e38
+        norm = float(optim.clip_grad_norm_(ps, 3e37))
+        assert abs(norm / 3e38 - 1) <= 4 * U32 and bool(torch.isfinite(g).all())
+        # the value 1.5e38 (half a unit off), the factor 0.1 and the product: three roundings
+        assert bool(((g[::g.numel() // 4][:4].double() / -1.5e37 - 1).abs() <= 3.01 * U32).all()) and int((g != 0).sum()) == 4
