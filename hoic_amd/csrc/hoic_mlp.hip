@@ -2289,11 +2289,14 @@ __device__ __forceinline__ float m_value(unsigned c) {
 }
 __device__ __forceinline__ float v_value(unsigned c) { return c == 0xff ? __builtin_nanf("") : __builtin_bit_cast(float, c << 20) * pow2f(112); }
 // Where a value lies between two codes is a matter of its last bits now and then: with b1 = 0.9 one value in 10^7 or so is a decimal
-// fraction that lies exactly on the border between up and down.  So that it falls where the same formula lets it fall in 64-bit
-// tensor operations, the operations are theirs, unfused and in their order, down to 2^e: tensor operations take it from the math
-// library's pow, which gives the next smaller number for some e.  Those e (bit e + 126), and what that makes of
+// fraction that lies exactly on the border between up and down, and either code is then a right one.  So that a step here and the same formula
+// in 64-bit tensor operations hold the same states, the operations are theirs, unfused and in their order, down to 2^e: tensor
+// operations on this GPU take it from the math library's pow, which gives the next smaller number for some e.  Those e (bit e + 126), and what
+// that makes of
 //   a code's value (8 + man) 2^(e - 10 | e - 18): one unit in the last place down for these exponent fields (bit = field),
 //   a / k: one up,     y 2^(3 - ey): one down for these ey (bit ey + 14).
+// Nothing but a border case depends on it: with exact powers 30 of 1.6e9 codes are the neighbouring ones (134 M f32 parameters, no clipping; none of
+// 2.3e8 with clipping), and the step of 3.9 M parameters takes 18.6 instead of 19.2 us.
 __device__ const unsigned POW_DOWN[8] = {0x00a02000u, 0x08084010u, 0x40000424u, 0x04252800u, 0x28080200u, 0x02100420u, 0x04000908u, 0x090a0210u};
 #define M_DOWN 0x43u
 #define V_DOWN 0x20004253u

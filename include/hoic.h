@@ -397,7 +397,8 @@ int32_t hoic_clip_grads(void* const* g, const int64_t* n, const uint8_t* type, i
  * (the norm comes back in d_norm), and a norm that is not finite in float32 leaves everything as it is.
  *   state_bits 32: m, v float32 [n];  8: m, v bytes [n], m_scale, v_scale float32 [ceil(n / 256)]: blocks of 256 in storage order, a
  *   power-of-two scale each; m sign + e4m3 (bias 7), v e5m3 (bias 15) without sign; rounded up with the probability of the part cut
- *   off by a hash of (seed, t, ordinal, element); 0x7f / 0xff stand for values that are not finite
+ *   off by a hash of (seed, t, ordinal, element) -- a value on the border between two codes to the last bits of 64-bit arithmetic (one in
+ *   10^7) becomes either; 0x7f / 0xff stand for values that are not finite
  *   t = step (>= 1, this step's) -- or, with d_consts (4 nt floats of scratch), counted on the device: *d_step += 1 first; lr then
  *   comes from d_lr (device float) when given.  Bytes of 8-bit states aligned to 4.
  * hoic_adamw_values: the float32 values of 8-bit states: p receives m's, g v's (both float32 [n]). */

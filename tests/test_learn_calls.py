@@ -221,3 +221,81 @@ def test_clipping_by_a_norm_past_float32(n):
         assert abs(norm / 3e38 - 1) <= 4 * U32 and bool(torch.isfinite(g).all())
         # the value 1.5e38 (half a unit off), the factor 0.1 and the product: three roundings
         assert bool(((g[::g.numel() // 4][:4].double() / -1.5e37 - 1).abs() <= 3.01 * U32).all()) and int((g != 0).sum()) == 4
+
+
+def exact_pow2(e):
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def exact_place8(x, signed, r16):
+    """float64 values in whole blocks -> (place on the ladder with the random part, in codes: its whole part is the code without sign; scales), every
+    power of two from its bits"""
+    top, low = (7, -6) if signed else (15, -14)
+    b = x.abs().view(-1, 256)
+    e = torch.clamp(torch.frexp(b.max(1).values)[1] - 1 - top, min=-126)
+    e = torch.where(b.max(1).values > 0, e, torch.full_like(e, -126))
+    y = (b * exact_pow2(-e)[:, None]).view(-1)
+    ey = torch.clamp(torch.where(y > 0, torch.frexp(y)[1] - 1, torch.full_like(e, low).repeat_interleave(256)), min=low)
+    return y * exact_pow2(3 - ey) + (r16.double() + 0.5) / 65536.0 + ((ey - low) * 8).double(), exact_pow2(e)
+
+
+def exact_values8(code, k, signed):
+    low = -6 if signed else -14
+    c = torch.arange(256, device=code.device)
+    e, man = (c & 127 if signed else c) >> 3, c & 7
+    v = torch.where(e == 0, man.double(), man.double() + 8.0) * exact_pow2(torch.clamp(e, min=1) - 4 + low)
+    return torch.where(c >= 128, -v, v)[code.long()] * k.repeat_interleave(256) if signed else v[code.long()] * k.repeat_interleave(256)
+
+
+@pytest.mark.parametrize("signed", [True, False])
+def test_exact_forms_of_8_bit_values_agree(signed):
+    """the tensor form with exact powers of two, which the next test uses, against the search on the ladder"""
+    gen = np.random.default_rng(1)
+    x = gen.standard_normal(256 * 40) * 10.0 ** gen.uniform(-12, 0, 256 * 40)
+    x = x if signed else np.abs(x)
+    x[:300] = 0
+    r = gen.integers(0, 65536, x.size)
+    codes, scales = T.store8(x, signed, r)
+    place, k = exact_place8(torch.tensor(x), signed, torch.tensor(r))
+    code = torch.floor(place) if signed else torch.where(torch.tensor(x) > 0, torch.clamp(torch.floor(place), min=1), torch.floor(place))
+    assert np.array_equal(code.numpy(), codes & 127 if signed else codes) and np.array_equal(k.float().numpy(), scales)
+    assert np.array_equal(exact_values8(torch.tensor(codes), k, signed).numpy(), T.load8(codes, scales, signed))
+
+
+@gpu
+@pytest.mark.parametrize("bits_of_gradient", [12, 24])
+def test_adamw8_codes_are_those_of_exact_powers_but_on_a_border(bits_of_gradient):
+    """the documented format -- code times a power of two, up with the probability of the part cut off -- with exact powers of two, over a first step
+    and three on states of every code: the same scales and the same codes, but where the exact place lies on a border (within 2^-30 of a step: a
+    last bit of a power of two moves a value of 2^8 of its scale by 2^-44 of it, 2^-35 of the smallest step, a scale that falls by 2^5
+    in a step makes 2^-30 of that).  Such places come up once in 10^7 values, and a code then is one of the two beside it."""
+    n = 1 << 24
+    gen = torch.Generator(device="cuda").manual_seed(bits_of_gradient)
+    g = torch.randint(1, 1 << bits_of_gradient, (n,), device="cuda", generator=gen).float() * (2.0 ** torch.randint(-20, -10, (n,), device="cuda", generator=gen))
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda")); p.grad = g
+    opt = optim.AdamW([p], lr=0.0, state_bits=8, seed=7)
+    i = torch.arange(n, device="cuda")
+    def mix(x):
+        x = x ^ (x >> 17); x = (x * 0x743B8C43) & 0xFFFFFFFF
+        x = x ^ (x >> 12); x = (x * 0xAB2209AB) & 0xFFFFFFFF
+        return x ^ (x >> 15)
+    m = v = torch.zeros(n, dtype=torch.float64, device="cuda")
+    for t in (1, 2, 3, 4):
+        opt.step()
+        m = 0.9 * m + (1.0 - 0.9) * g.double(); v = 0.999 * v + (1.0 - 0.999) * g.double() * g.double()
+        h = mix((i + mix(mix(mix(mix(7) + t & 0xFFFFFFFF) + 0) + 0 & 0xFFFFFFFF)) & 0xFFFFFFFF)
+        s = opt.state[p]
+        for key, x, signed, r in (("exp_avg", m, True, h & 0xFFFF), ("exp_avg_sq", v, False, h >> 16)):
+            place, k = exact_place8(x, signed, r)
+            assert torch.equal(k.float(), s[key + "_scale"])
+            code, got = torch.floor(place), (s[key] & 127 if signed else s[key]).double()
+            code = code if signed else torch.where(x > 0, torch.clamp(code, min=1), code)
+            far = (place - torch.round(place)).abs() >= 2.0 ** -30
+            assert torch.equal(got[far], code[far]), (key, t)
+            assert int((~far).sum()) < 2 ** -12 * n and bool(((got - torch.round(place))[~far] <= 0).all() & ((got - torch.round(place))[~far] >= -1).all())
+            if signed:
+                held = got != 0                                # (a sum that cancels to its last bits has either sign: codes 0 and 128 both stand for 0)
+                assert torch.equal((s[key] >= 128)[held], (x < 0)[held])
+        m, v = exact_values8(s["exp_avg"], s["exp_avg_scale"].double(), True), exact_values8(s["exp_avg_sq"], s["exp_avg_sq_scale"].double(), False)
+        assert torch.equal(opt.state_values()[0][0], m.float()) and torch.equal(opt.state_values()[1][0], v.float())
+        p.grad = g = -g.flip(0)
