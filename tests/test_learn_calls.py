@@ -299,3 +299,135 @@ def test_adamw8_codes_are_those_of_exact_powers_but_on_a_border(bits_of_gradient
         m, v = exact_values8(s["exp_avg"], s["exp_avg_scale"].double(), True), exact_values8(s["exp_avg_sq"], s["exp_avg_sq_scale"].double(), False)
         assert torch.equal(opt.state_values()[0][0], m.float()) and torch.equal(opt.state_values()[1][0], v.float())
         p.grad = g = -g.flip(0)
+
+
+# ================================================================================================ the learner's head step with a KL term
+def head_case(rows, seed=5, trainable=True):
+    from hoic_amd.config import Config
+    from hoic_amd.rl import PolicyGaussian
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=gen)
+    pol = PolicyGaussian(Config("box_future5_light_add_geom"), 32, 617).cuda()
+    with torch.no_grad():
+        pol.action_log_std.add_(rn(1, 32) * 0.2)
+        pol.action_mean.weight.mul_(3.0)
+    pol.action_log_std.requires_grad_(trainable)
+    h = rn(rows, 512)
+    actions = pol.action_mean(h).detach() + torch.exp(pol.action_log_std.detach()) * rn(rows, 32)
+    before = copy.deepcopy(pol)
+    with torch.no_grad():
+        before.action_mean.weight.add_(rn(32, 512) * 2e-4)
+        before.action_log_std.add_(rn(1, 32) * 0.01)
+        fixed, old = before.get_log_prob(None, actions, hidden=h), dict(mean=before.action_mean(h), log_std=before.action_log_std.clone())
+    return pol, h, actions, rn(rows, 1), fixed, old
+
+
+def head_reference(pol, h, actions, adv, fixed, old, kl_coef, weight, clip=0.2):
+    """float64 autograd: (loss, weight * its gradients of hidden, weight, bias, log_std; log-probabilities, ratio)"""
+    pol64, h64 = copy.deepcopy(pol).double(), h.double().requires_grad_()
+    pol64.action_log_std.requires_grad_(True)
+    mu, s, a = pol64.action_mean(h64), pol64.action_log_std, actions.double()
+    logp = (-((a - mu) ** 2) / (2 * torch.exp(2 * s)) - s - 0.5 * math.log(2 * math.pi)).sum(1, keepdim=True)
+    ratio = torch.exp(logp - (logp.detach() if fixed is None else fixed.double()))
+    mu0, s0 = (mu.detach(), s.detach()) if fixed is None else (old["mean"].double(), old["log_std"].double())
+    kl = (s - s0 + (torch.exp(2 * s0) + (mu - mu0) ** 2) / (2 * torch.exp(2 * s)) - 0.5).sum(1, keepdim=True)
+    loss = (-torch.min(ratio * adv.double(), torch.clamp(ratio, 1 - clip, 1 + clip) * adv.double()) + kl_coef * kl).mean()
+    g = torch.autograd.grad(weight * loss, (h64, pol64.action_mean.weight, pol64.action_mean.bias, s))
+    return loss.item(), g, logp.detach(), ratio.detach().reshape(-1)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [53248, 1003])
+@pytest.mark.parametrize("weight", [1.0, 0.75])
+@pytest.mark.parametrize("trainable", [True, False])
+def test_kl_head_step_matches_float64(rows, weight, trainable):
+    """mlp.ppo_kl_head_step against float64 autograd, epoch 0 and a later one: value, gradients of the hidden activation and of every
+    parameter of the head, log-probabilities.  Its head kernels are ppo_head_step's, and so are the tolerances (tests/test_mlp.py: float32 head
+    forward and backward; rows next to a clip border may fall either way); the loss between them is in 64 bits."""
+    from hoic_amd import mlp as M
+    pol, h, actions, adv, fixed, given = head_case(rows, trainable=trainable)
+    def close(a, b, rel, what):
+        err, mag = float((a.double() - b).abs().max()), float(b.abs().max())
+        assert err <= rel * mag + 1e-12, f"{what}: {err:.3e} against magnitude {mag:.3e}"
+    for first in (True, False):
+        old = {} if first else dict(given)
+        pol.action_mean.weight.grad = pol.action_mean.bias.grad = pol.action_log_std.grad = None
+        loss, dh, lp = M.ppo_kl_head_step(h, pol, actions, adv, None if first else fixed, 0.2, 0.7, old, weight)
+        want, (g_h, g_w, g_b, g_s), logp, ratio = head_reference(pol, h, actions, adv, None if first else fixed, given, 0.7, weight)
+        assert abs(float(loss) - want) <= 2e-5 * max(1.0, abs(want))
+        near = ((ratio - 0.8).abs() < 1e-5) | ((ratio - 1.2).abs() < 1e-5)
+        if first:
+            close(lp, logp, 2e-6, "log-probabilities")
+            assert lp.shape == (rows, 1) and torch.equal(old["log_std"], pol.action_log_std) and old["log_std"].data_ptr() != pol.action_log_std.data_ptr()
+            close(old["mean"], pol.double().action_mean(h.double()).detach(), 1e-5, "means of epoch 0"); pol.float()
+        else:
+            assert lp is fixed and set(old) == {"mean", "log_std"}
+            assert 0.05 < float(((ratio < 0.8) | (ratio > 1.2)).double().mean()) < 0.95 and float(near.double().mean()) < 1e-3
+        close(dh[~near], g_h[~near], 5e-5, "d loss / d hidden")
+        tol = 5e-4 if bool(near.any()) else 5e-5
+        close(pol.action_mean.weight.grad, g_w, tol, "action_mean.weight.grad")
+        close(pol.action_mean.bias.grad, g_b, tol, "action_mean.bias.grad")
+        if trainable:
+            close(pol.action_log_std.grad, g_s, tol, "action_log_std.grad")
+            assert pol.action_log_std.grad.shape == pol.action_log_std.shape
+        else:
+            assert pol.action_log_std.grad is None
+
+
+@gpu
+def test_kl_head_step_without_kl_is_the_head_step():
+    """kl_coef 0: value, gradients and log-probabilities of ppo_head_step, whose loss kernel is in float32 (twice the tolerances against float64)"""
+    from hoic_amd import mlp as M
+    pol, h, actions, adv, fixed, old = head_case(4099, seed=9)
+    near = head_reference(pol, h, actions, adv, fixed, old, 0.0, 1.0)[3]
+    near = ((near - 0.8).abs() < 1e-5) | ((near - 1.2).abs() < 1e-5)
+    out = []
+    for step in (lambda f: M.ppo_kl_head_step(h, pol, actions, adv, f, 0.2, 0.0, {} if f is None else old, 0.75), lambda f: M.ppo_head_step(h, pol, actions, adv, f, 0.2, 0.75)):
+        for f in (None, fixed):
+            loss, dh, lp = step(f)
+            out.append([loss, dh[~near] if f is not None else dh, lp] + [p.grad.clone() for p in (pol.action_mean.weight, pol.action_mean.bias, pol.action_log_std)])
+    for k in range(2):
+        tol = 1e-3 if k and bool(near.any()) else 1e-4
+        for a, b, rel in zip(out[k], out[2 + k], (4e-5, 1e-4, 4e-6, tol, tol, tol)):
+            assert float((a.double() - b.double()).abs().max()) <= rel * max(float(b.abs().max()), 1.0 if rel == 4e-5 else 0.0) + 1e-12
+
+
+def learner_run(streams=1, overlap=False, optimizer="AdamW", kl_coef=0.5, fix_std=False):
+    from hoic_amd.agent import PPOLearner
+    torch.manual_seed(0)
+    cfg = T.learner_config([512, 256, 256], kl_coef=kl_coef, policy_optimizer=optimizer, value_optimizer=optimizer, policy_weightdecay=0.01, value_weightdecay=0.01, fix_std=fix_std)
+    L = PPOLearner(cfg, 617, 32, torch.device("cuda"), update_dtype="f16x3", strict_reference=False, update_streams=streams)
+    L.overlap_value_update = overlap
+    start = [p.detach().clone() for n in ("policy", "value") for p in getattr(L, n + "_net").parameters()]
+    for seed in (5, 6):
+        L.update_params(T.learner_batch(16, 256, 617, 32, torch.float32, "cuda", seed=seed))
+    L.finish_update()
+    torch.cuda.synchronize()
+    return start, [p.detach().clone() for n in ("policy", "value") for p in getattr(L, n + "_net").parameters()], L
+
+
+@gpu
+@pytest.mark.parametrize("optimizer", ["AdamW", "AdamW8bit"])
+def test_learner_update_with_kl_is_the_same_on_any_streams(optimizer):
+    """one stream, the value chain on a side stream, each chain's small kernels on a stream of its own, the value phase behind the policy's: the same
+    kernels on the same operands in the same order within a chain, so the same bits after two updates, losses included"""
+    _, want, L = learner_run(1, optimizer=optimizer)
+    for streams, overlap in ((2, False), (3, False), (3, True)):
+        _, got, K = learner_run(streams, overlap, optimizer=optimizer)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), (streams, overlap)
+        assert K.last_losses == L.last_losses
+
+
+@gpu
+@pytest.mark.parametrize("fix_std", [False, True])
+def test_learner_update_with_kl_through_autograd_heads(monkeypatch, fix_std):
+    """heads and losses through autograd (what runs where the heads do not fit the fused kernels): the same update as the fused form to float32
+    rounding -- Adam's quotients carry a gradient's relative error, 5e-5 by the head step's tests, into the step, and small gradients' signs: a
+    hundredth of the way moved allowed"""
+    from hoic_amd import mlp as M
+    start, fused, L = learner_run(fix_std=fix_std)
+    monkeypatch.setattr(M, "FORCE_AUTOGRAD_HEADS", True)
+    _, plain, K = learner_run(fix_std=fix_std)
+    dist = lambda x, y: math.sqrt(sum(float(((a.double() - b.double()) ** 2).sum()) for a, b in zip(x, y)))
+    assert 0.0 < dist(fused, start) and dist(fused, plain) <= 1e-2 * dist(fused, start)
+    assert abs(L.last_losses[1] - K.last_losses[1]) <= 1e-4 * max(1.0, abs(L.last_losses[1]))
