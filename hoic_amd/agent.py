@@ -186,6 +186,14 @@ class PPOLearner:
         fused = {"fused": True} if (cuda and fused_adam) else {}
         return torch.optim.Adam(net.parameters(), lr=lr, weight_decay=weight_decay, **fused)
 
+    def _clip(self, params, bound):
+        """agent_handmimic.py:67's clipping for the optimisers that do not clip inside their step: hoic_amd.optim.clip_grad_norm_ (two launches, the
+        norm in 64 bits) for float32 networks on the GPU, torch's otherwise"""
+        if params[0].is_cuda and params[0].dtype == torch.float32:
+            from .optim import clip_grad_norm_
+            return clip_grad_norm_(params, bound)
+        return torch.nn.utils.clip_grad_norm_(params, bound)
+
     # ------------------------------------------------------------------ update (agent_pg.py:39-55, agent_ppo.py:16-64)
     def _allreduce_start(self, params):
         """Start the gradient all-reduce of one network (one flat buffer) without waiting for it."""
@@ -553,7 +561,7 @@ class PPOLearner:
                 self.optimizer_policy.step(max_norm=40 if clip else None)
             else:
                 if clip:
-                    torch.nn.utils.clip_grad_norm_(pparams, 40)
+                    self._clip(pparams, 40)
                 self.optimizer_policy.step()
             if self._engines is not None:
                 self._engines[1].weights_changed()

@@ -431,3 +431,37 @@ def test_learner_update_with_kl_through_autograd_heads(monkeypatch, fix_std):
     dist = lambda x, y: math.sqrt(sum(float(((a.double() - b.double()) ** 2).sum()) for a, b in zip(x, y)))
     assert 0.0 < dist(fused, start) and dist(fused, plain) <= 1e-2 * dist(fused, start)
     assert abs(L.last_losses[1] - K.last_losses[1]) <= 1e-4 * max(1.0, abs(L.last_losses[1]))
+
+
+@gpu
+@pytest.mark.parametrize("update_dtype", ["f16x3", "f32"])
+@pytest.mark.parametrize("scale,strict", [(1.0, True), (1e5, True), (1e5, False)])
+def test_learner_clips_with_its_own_kernels(monkeypatch, update_dtype, scale, strict):
+    """Adam on the GPU: the policy's gradient through optim.clip_grad_norm_ (once a run as the reference does, or every step), as torch clips it:
+    the same gradient where the norm is under the bound, a factor of float32 roundings beside torch's above it (its norm: some 10 roundings
+    of partial norms, the factor and the product two more: under 16 U32)"""
+    from hoic_amd import agent as A
+    torch.manual_seed(0)
+    L = A.PPOLearner(T.learner_config([512, 256, 256], policy_lr=1e-3), 617, 32, torch.device("cuda"), update_dtype=update_dtype, strict_reference=strict)
+    norms, own, theirs = [], optim.clip_grad_norm_, torch.nn.utils.clip_grad_norm_
+
+    def both(params, bound):
+        twins = [torch.nn.Parameter(torch.empty_like(p)) for p in params]
+        for q, p in zip(twins, params):
+            q.grad = None if p.grad is None else p.grad.clone()
+        norms.append(float(own(params, bound)))
+        want = float(theirs(twins, bound))
+        assert bound == 40 and abs(norms[-1] - want) <= 16 * U32 * want
+        for q, p in zip(twins, params):
+            if p.grad is not None:
+                assert torch.equal(p.grad, q.grad) if want < 39.9 else bool(((p.grad - q.grad).abs() <= 16 * U32 * q.grad.abs() + 2.0 ** -149).all())
+        return norms[-1]
+
+    monkeypatch.setattr(optim, "clip_grad_norm_", both)
+    monkeypatch.setattr(torch.nn.utils, "clip_grad_norm_", None)
+    b = T.learner_batch(16, 256, 617, 32, torch.float32, "cuda")
+    monkeypatch.setattr(A, "estimate_advantages", lambda *a, **k: tuple(x * s for x, s in zip(rl.estimate_advantages(*a, **k), (scale, 1.0))))
+    for _ in range(2):
+        L.update_params(b)
+    L.finish_update()
+    assert len(norms) == (1 if strict else 10) and (norms[0] > 40) == (scale > 1)
