@@ -70,8 +70,8 @@ __device__ __forceinline__ void gelu_pair(float z, float& g, float& dg) {
   g = z * Phi;
   dg = fmaf(z * 0.39894228040143268f, e, Phi);
 }
-// The same pair for TWO values at once on the packed float32 pipe (v_pk_fma_f32 / v_pk_mul_f32: two IEEE operations per
-// instruction).  Constants folded: t = 1 / (1 + (p / sqrt 2) |z|), exp(-z^2 / 2) = exp2(-(z sqrt(log2(e) / 2))^2).
+// The same pair for TWO values at once (one instruction each: this unit is built without the packed float32 ones, see the Makefile).
+// Constants folded: t = 1 / (1 + (p / sqrt 2) |z|), exp(-z^2 / 2) = exp2(-(z sqrt(log2(e) / 2))^2).
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void gelu_pair2(f2 z, f2& g, f2& dg) {
@@ -228,10 +228,10 @@ __device__ __forceinline__ void gemm_epilogue(const GemmArgs& a, f32x16 (&acc)[T
 // float32 copy directly, the packed row-major output after an exchange inside each group of 8 lanes (lane q of a group
 // writes dword q of the 32-byte H8L8 group: q < 4 the hi halves of columns 2q, 2q + 1, q >= 4 the lo halves).  No
 // transposed output in this form (the weight-gradient kernel below reads row-major operands).
-// Round 6: the arithmetic runs two rows at a time on the packed float32 pipe (v_pk_fma_f32 / v_pk_mul_f32: consecutive
-// accumulator registers are consecutive rows of one column), the hi | lo word of an element is two v_fma_mix (the output
-// scale folded in), and every access is base (SGPR pair) + one 32-bit byte offset shared by the output arrays -- 21 issue
-// slots per element where the scalar form took 41 (profiles/r06_experiments.json "epilogue_diet").
+// The arithmetic takes two rows at a time (consecutive accumulator registers are consecutive rows of one column), the hi | lo word of an element
+// is two v_fma_mix (the output scale folded in), and every access is base (SGPR pair) + one 32-bit byte offset shared by the output
+// arrays: 3 664 VALU instructions in the forward kernel, 4 783 before (2 851 with packed float32 instructions, which this unit does without: the
+// time is that of the output bytes in each form).
 template <int EPI, int TM, int TN>
 __device__ __forceinline__ void gemm_epilogue_mn(const GemmArgs& a, f32x16 (&acc)[TM][TN], int mb, int nb, int lane) {
   const int l31 = lane & 31, hf = lane >> 5;
@@ -1534,7 +1534,8 @@ struct PolicyLossArgs {
 // itself / in front: 257 x 32 8.1 / 10.1 us, 20 000 10.3 / 11.9, 53 248 15.9 / 15.8 (and 2.5 us of host time), 100 000 23.0 / 21.6, 524 288 78 / 57.
 #define PL_COUNT_ALL 65536
 
-// e^x to 2e-13: 2^k (1 + r + ... + r^10 / 10!), |r| <= ln 2 / 2; the next term is r^11 / 11! < 2.2e-13.  (A relative 2e-13 of a row's terms
+// e^x to 2e-13: 2^k (1 + r + ... + r^10 / 10!), r = x - k ln 2 with ln 2 in two parts, its first 32 bits (whose product with k is exact) and the
+// rest (Cody and Waite, Software Manual for the Elementary Functions, 1980), |r| <= ln 2 / 2; the next term is r^11 / 11! < 2.2e-13.  (A relative 2e-13 of a row's terms
 // moves its ratio by 1e-11.)  A NaN stays one; infinities are for exp_row.
 __device__ __forceinline__ double exp_terms(double x) {
   const double k = __builtin_rint(x * 1.4426950408889634074);
