@@ -1773,7 +1773,7 @@ template <class TM, bool SHARED, bool KL, bool GRAD, int VEC> __global__ __launc
           }
         };
         store((TM*)a.d_mean + row * a.ld_dmean, SHARED && !ok ? zero4 : g);      // (0 also beside a shared deviation that is no number)
-        if (row_ls) { if (a.t_std == HOIC_F32) store((float*)a.d_log_std + row * a.dims, gs); else store((TM*)a.d_log_std + row * a.dims, gs); }
+        if constexpr (!SHARED) if (row_ls) { if (a.t_std == HOIC_F32) store((float*)a.d_log_std + row * a.dims, gs); else store((TM*)a.d_log_std + row * a.dims, gs); }
       }
     }
   }
