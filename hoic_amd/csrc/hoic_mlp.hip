@@ -1480,14 +1480,23 @@ template <> struct vec4<float> { typedef f4u type; };
 template <> struct vec4<_Float16> { typedef h4u type; };
 template <> struct vec4<__bf16> { typedef b4u type; };
 
-// NT: around the caches, for lists that would only push one another out of them (STREAM_BYTES below)
-template <bool NT, class V> __device__ __forceinline__ V load_as(const V* x) { return NT ? __builtin_nontemporal_load(x) : *x; }
-template <bool NT, class V> __device__ __forceinline__ void store_as(V* x, V v) { if (NT) __builtin_nontemporal_store(v, x); else *x = v; }
+struct word { typedef unsigned type; };
+
+// NT: around the caches, for lists that would only push one another out of them (STREAM_BYTES below).  The vector's type comes by a trait W: deduced
+// from a pointer it would lose its alignment, and the compiler would take any view of a tensor for one aligned to 16 bytes.
+template <bool NT, class W, class T> __device__ __forceinline__ typename W::type load_as(const T* x) {
+  const typename W::type* v = (const typename W::type*)x;
+  return NT ? __builtin_nontemporal_load(v) : *v;
+}
+template <bool NT, class W, class T> __device__ __forceinline__ void store_as(T* x, typename W::type r) {
+  typename W::type* v = (typename W::type*)x;
+  if (NT) __builtin_nontemporal_store(r, v); else *v = r;
+}
 // four elements from x on, of which the first `left` exist (the rest read as 0)
 template <bool NT = false, class T> __device__ __forceinline__ f32x4 load4(const T* __restrict__ x, int left) {
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
   if (left >= 4) {
-    r = __builtin_convertvector(load_as<NT>((const typename vec4<T>::type*)x), f32x4);
+    r = __builtin_convertvector(load_as<NT, vec4<T>>(x), f32x4);
   } else {
     if (left > 0) r.x = (float)x[0];
     if (left > 1) r.y = (float)x[1];
@@ -1497,7 +1506,7 @@ template <bool NT = false, class T> __device__ __forceinline__ f32x4 load4(const
 }
 template <bool NT = false, class T> __device__ __forceinline__ void store4(T* __restrict__ x, int left, f32x4 r) {
   if (left >= 4) {
-    store_as<NT>((typename vec4<T>::type*)x, __builtin_convertvector(r, typename vec4<T>::type));
+    store_as<NT, vec4<T>>(x, __builtin_convertvector(r, typename vec4<T>::type));
   } else {
     if (left > 0) x[0] = (T)r.x;
     if (left > 1) x[1] = (T)r.y;
@@ -1930,13 +1939,13 @@ template <class T> struct WideStep {
     g += i;
     if (left == 8 * SPAN) {
 #pragma unroll
-      for (int u = 0; u < 8; u++) x[u] = load_as<NT>((const typename wide<T>::type*)(g + lane + u * SPAN));
+      for (int u = 0; u < 8; u++) x[u] = load_as<NT, wide<T>>(g + lane + u * SPAN);
     } else {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
         typename wide<T>::type z = {};
         x[u] = z;
-        if ((u + 1) * SPAN <= left) x[u] = load_as<NT>((const typename wide<T>::type*)(g + lane + u * SPAN));
+        if ((u + 1) * SPAN <= left) x[u] = load_as<NT, wide<T>>(g + lane + u * SPAN);
       }
       const int cut = left / SPAN * SPAN + lane;
       typename wide<T>::type y = {};
@@ -2397,7 +2406,7 @@ template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw8_k
     const long long ob = (u * 4 + wave) * 256, i = i0 + ob + lane * 4;
     if (ob + 256 > left) continue;
     pp[u] = load4<NT>(p + i, 4); gg[u] = load4<NT>(g + i, 4);
-    cm[u] = load_as<NT>((const unsigned*)(m + i)); cv[u] = load_as<NT>((const unsigned*)(v + i));
+    cm[u] = load_as<NT, word>(m + i); cv[u] = load_as<NT, word>(v + i);
     km[u] = ms[(i0 + ob) >> 8]; kv[u] = vs[(i0 + ob) >> 8];
   }
   double cl = 1.;
@@ -2447,7 +2456,7 @@ template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw8_k
     f32x4 pu = pp[u];
 #pragma unroll
     for (int e = 0; e < 4; e++) pu[e] = adam_param(pu[e], mf[e], vf[e], c, a.eps);
-    store_as<NT>((unsigned*)(m + i), om); store_as<NT>((unsigned*)(v + i), ov);
+    store_as<NT, word>(m + i, om); store_as<NT, word>(v + i, ov);
     store4<NT>(p + i, 4, pu);
     if (lane == 0) { ms[blk] = pow2f(em); vs[blk] = pow2f(ev); }
   }

@@ -465,3 +465,30 @@ def test_learner_clips_with_its_own_kernels(monkeypatch, update_dtype, scale, st
         L.update_params(b)
     L.finish_update()
     assert len(norms) == (1 if strict else 10) and (norms[0] > 40) == (scale > 1)
+
+
+def test_kernels_claim_no_alignment_that_views_lack(tmp_path):
+    """the compiler's own check of the unit's vector accesses: a view of a tensor is aligned to one element, so that a load or store that goes by
+    a wider type's alignment is an error (here a piece of code that does, to see that the check is on)"""
+    import os
+    import re
+    import shutil
+    import subprocess
+    from conftest import ROOT
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("no hipcc")
+    csrc = os.path.join(ROOT, "hoic_amd", "csrc")
+    assert re.search(r"^GEMMFLAGS .*-Werror=align-mismatch", open(os.path.join(csrc, "Makefile")).read(), re.M)
+    check = lambda path: subprocess.run([hipcc, "-std=c++17", "--offload-arch=gfx950", "--cuda-device-only", "-fsyntax-only", "-Werror=align-mismatch", path],
+                                        capture_output=True, text=True)
+    bad = tmp_path / "bad.hip"
+    bad.write_text("""#include <hip/hip_runtime.h>
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+template <class V> __device__ V get(const V* x) { return *x; }
+__global__ void k(const float* x, float* y) { y[0] = get((const f4u*)x).x; }
+""")
+    r = check(str(bad))
+    assert r.returncode != 0 and "align-mismatch" in r.stderr
+    r = check(os.path.join(csrc, "hoic_mlp.hip"))
+    assert r.returncode == 0, r.stderr[-2000:]
