@@ -218,6 +218,10 @@ class AdamW(torch.optim.Optimizer):
         """Also takes the state of a ``torch.optim.Adam`` / ``AdamW`` over the same parameters (``state_bits=32``; refused with options that
         this step does not have: ``maximize``, ``amsgrad``, ``Adam``'s coupled weight decay).  The moments are copied, and keep their own
         types whatever the parameters' are.  (8-bit ones need parameters in the order in memory that they were made for.)"""
+        state_dict = dict(state_dict)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         for g in state_dict["param_groups"]:
             _check_options(g)
         old = [p for g in state_dict["param_groups"] for p in g["params"]]
@@ -241,12 +245,19 @@ class AdamW(torch.optim.Optimizer):
                 mine[key].copy_(s[key] if s[key].shape == mine[key].shape else s[key].reshape(mine[key].shape))
             states[p] = mine
         fixed = {k: self.defaults[k] for k in ("state_bits", "capturable")}
-        super().load_state_dict({**state_dict, "state": {}})
+        hooks = self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks
+        self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = {}, {}
+        try:                        # (the base class would bring the moments to the parameters' types; its hooks run here, around the whole call)
+            super().load_state_dict({**state_dict, "state": {}})
+        finally:
+            self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = hooks
         for g in self.param_groups:
             for key, value in self.defaults.items():
                 g.setdefault(key, value)
             g.update(fixed)
         self.state.update(states)
+        for hook in hooks[1].values():
+            hook(self)
 
     def step(self, closure=None, *, max_norm=None):
         if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _opt._global_optimizer_pre_hooks

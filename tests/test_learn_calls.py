@@ -492,3 +492,30 @@ __global__ void k(const float* x, float* y) { y[0] = get((const f4u*)x).x; }
     assert r.returncode != 0 and "align-mismatch" in r.stderr
     r = check(os.path.join(csrc, "hoic_mlp.hip"))
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_adamw_load_hooks_see_and_change_the_whole_state(recorder):
+    """a hook before loading may hand over another state, one behind it finds the moments in place, each runs once"""
+    ps = [torch.nn.Parameter(torch.randn(6)) for _ in range(2)]
+    for p in ps:
+        p.grad = torch.randn(6)
+    opt = optim.AdamW(ps[:1], lr=0.25)
+    opt.step()
+    opt.state[ps[0]]["exp_avg"].fill_(3.0)
+    other, seen = optim.AdamW(ps[1:], lr=0.5), []
+
+    def before(o, sd):
+        seen.append("before")
+        moments = {k: {**s, "exp_avg": s["exp_avg"] * 2} for k, s in sd["state"].items()}
+        return {"state": moments, "param_groups": [{**g, "lr": 0.125} for g in sd["param_groups"]]}
+
+    def after(o):
+        seen.append(float(o.state[ps[1]]["exp_avg"][0]))
+
+    handles = other.register_load_state_dict_pre_hook(before), other.register_load_state_dict_post_hook(after)
+    other.load_state_dict(opt.state_dict())
+    assert seen == ["before", 6.0] and other.param_groups[0]["lr"] == 0.125 and other.state[ps[1]]["step"] == 1
+    for h in handles:
+        h.remove()
+    other.load_state_dict(opt.state_dict())
+    assert seen == ["before", 6.0] and other.param_groups[0]["lr"] == 0.25 and float(other.state[ps[1]]["exp_avg"][0]) == 3.0
