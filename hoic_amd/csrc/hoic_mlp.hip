@@ -1860,6 +1860,9 @@ extern "C" int32_t hoic_policy_loss(const hoic_policy_loss_args* p, void* stream
       || (a.count && !a.d_mean)) {
     hoic_set_error("hoic_policy_loss: missing tensors"); return HOIC_ERR_ARG;
   }
+  if (a.ld_mean < 0 || a.ld_act < 0 || a.ld_std < 0 || a.ld_ref_mean < 0 || a.ld_ref_std < 0 || (a.d_mean && a.rows > 1 && a.ld_dmean < a.dims)) {
+    hoic_set_error("hoic_policy_loss: row strides of at least 0, the gradient's of at least dims (its rows would be written over one another)"); return HOIC_ERR_ARG;
+  }
   if (a.rows > 1ll << 32) { hoic_set_error("hoic_policy_loss: more than 2^32 rows"); return HOIC_ERR_ARG; }      // (counts are in 32 bits per wavefront)
   hipStream_t st = (hipStream_t)stream;
   PolicyLossArgs k;

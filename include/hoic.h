@@ -351,7 +351,7 @@ enum hoic_type { HOIC_F32 = 0, HOIC_F16 = 1, HOIC_BF16 = 2 };
  * <= 256; s = log_std, l = sum_j log N(act; mean, e^s), r = e^(l - fixed) (fixed NULL: r = 1, the old policy is this one),
  *   S = -min(r adv, clip(r, 1 - clip_lo, 1 + clip_hi) adv),  K = KL(reference || policy),  L = sum over valid rows (S + kl_coef K) / n,
  * n = number of valid rows (valid NULL: all; no valid row: L = 0 and no gradient).  Rows outside `valid` may hold anything.
- *   mean, ref_mean  t_mean, row strides ld_* in elements;  act  t_mean or float32;
+ *   mean, ref_mean  t_mean, row strides ld_* in elements (>= 0; ld_dmean >= dims);  act  t_mean or float32;
  *   log_std, ref_log_std  float32 or t_mean, row stride 0: one row shared by all;  ref_* both or neither
  *   adv, fixed [rows] float32;  valid [rows] bytes
  *   d_mean  NULL: value only;  else weight * upstream * dL/dmean (t_mean; upstream: device scalar, NULL = 1)

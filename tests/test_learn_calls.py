@@ -519,3 +519,15 @@ def test_adamw_load_hooks_see_and_change_the_whole_state(recorder):
         h.remove()
     other.load_state_dict(opt.state_dict())
     assert seen == ["before", 6.0] and other.param_groups[0]["lr"] == 0.25 and float(other.state[ps[1]]["exp_avg"][0]) == 3.0
+
+
+def test_policy_loss_entry_point_refuses_strides_that_it_cannot_take():
+    """negative row strides, and a gradient whose rows would be written over one another: refused before any launch"""
+    L = lib.load()
+    names = ("rows dims t_mean t_act t_std mean act log_std ref_mean ref_log_std ld_mean ld_act ld_std ld_ref_mean ld_ref_std ld_dmean adv fixed valid upstream count "
+             "clip_lo clip_hi kl_coef weight d_mean d_log_std log_probs loss info n_out scratch").split()
+    at = 64
+    good = dict.fromkeys(names, 0) | dict(rows=4, dims=4, mean=at, act=at, log_std=at, adv=at, loss=at, info=at, scratch=at, ld_mean=4, ld_act=4, ld_dmean=4)
+    changes = [{k: -1} for k in ("ld_mean", "ld_act", "ld_std", "ld_ref_mean", "ld_ref_std")] + [dict(d_mean=at, ld_dmean=k) for k in (3, 0, -4)]
+    for change in changes:
+        assert L.hoic_policy_loss(lib.POLICY_LOSS_ARGS.pack(*(good | change).values()), None) == -1 and b"strides" in L.hoic_last_error(), change
