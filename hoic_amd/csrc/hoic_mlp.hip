@@ -1526,7 +1526,7 @@ template <bool NT = false, class T> __device__ __forceinline__ void store4(T* __
 // A row is handled by `lpr` lanes of four dimensions each (lpr = the power of two >= dims / 4), a wavefront takes 64 / lpr rows, so that
 // a wavefront's load of 32 float32 dimensions is one stretch of 1 KB and a row's sums are three DPP steps.
 // Bound: HBM in large batches (524 287 x 32, a log-deviation per row, reference and mask: 94 us at best, 97 in the median, 4.9 TB/s; a copy
-// reaches 4.8), the latency of load -> row sums -> store in an update's (53 248 x 32 shared: 10.6 / 11.2 us, two such steps a workgroup).  At most 1024
+// reaches 4.8), the latency of load -> row sums -> store in an update's (53 248 x 32 shared: 10.6 / 11.3 us, two such steps a workgroup).  At most 1024
 // workgroups of equally many steps, four on each CU: 512 take 12.1 us against 11.9 at 53 248 rows and 118 against 92 at 524 287,
 // 2048 take 13.9 and 90 (twice the partial sums to join).  Odd dimensions are loaded one by one: a vector load where four are left and single
 // ones in the last lane costs both paths in every wavefront (33 dimensions 121 against 98 us).
@@ -1598,7 +1598,7 @@ __device__ __forceinline__ int count_valid(const unsigned char* __restrict__ val
   }
   return c;
 }
-// valid rows, in front of a large gradient (whose rows are divided by their number): 3.5 us at best, 3.9 in the median at 524 287 rows, a launch's latency
+// valid rows, in front of a large gradient (whose rows are divided by their number): 3.2 us at best, 4.0 in the median at 524 287 rows, a launch's latency
 __global__ __launch_bounds__(256) void hoic_count_valid_kernel(const unsigned char* __restrict__ valid, long long rows, long long per_block, int* __restrict__ counts) {
   __shared__ int red[4];
   const long long r0 = (long long)blockIdx.x * per_block, r1 = r0 + per_block < rows ? r0 + per_block : rows;
@@ -1812,7 +1812,7 @@ template <class TM, bool SHARED, bool KL, bool GRAD, int VEC> __global__ __launc
 }
 
 // sums of the workgroups' parts, a column a wavefront, all 16 loads of a lane in flight: workgroup 0 the scalars, the others four
-// dimensions each (2.0 to 2.7 us at best, 3.2 in the median: the latency of one load, the tree and a launch)
+// dimensions each (2.2 us at best, 3.0 in the median at 32 dimensions: the latency of one load, the tree and a launch)
 __global__ __launch_bounds__(256) void hoic_policy_loss_finish_kernel(PolicyLossArgs k) {
   const hoic_policy_loss_args& a = k.a;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, j = blockIdx.x == 0 ? a.dims + w : ((int)blockIdx.x - 1) * 4 + w;
@@ -1986,8 +1986,8 @@ template <bool NT, class T> __device__ __forceinline__ double sumsq(const T* g, 
   }
   return s;
 }
-// Bound: HBM (268 M bf16 values, 537 MB: 103 us at best, 105 in the median, 5.1 TB/s; the 64-bit FMA of a value issues as a 32-bit one), a
-// launch's latency in short lists (3.9 M values: 3.9 / 5.6 us).
+// Bound: HBM (268 M bf16 values, 537 MB: 104 us at best, 105 in the median, 5.1 TB/s; the 64-bit FMA of a value issues as a 32-bit one), a
+// launch's latency in short lists (3.9 M values: 3.9 / 5.4 us).
 template <bool NT> __global__ __launch_bounds__(256) void hoic_sumsq_kernel(NormArgs a) {
   __shared__ double red[4];
   const int t = list_find(a.t, a.nt, blockIdx.x);
@@ -2005,8 +2005,8 @@ __global__ __launch_bounds__(256) void hoic_norm_finish_kernel(Joint j, double* 
   const double2 r = join_norm(j);
   if (threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
 }
-// g *= factor where it is not 1.  Bound: HBM (537 MB read and written: 170 us at best, 172 in the median, 6.2 TB/s); short lists wait for the parts'
-// join (3.9 M float32 values: 7.0 / 7.4 us).
+// g *= factor where it is not 1.  Bound: HBM (537 MB read and written: 170 us at best, 173 in the median, 6.2 TB/s); short lists wait for the parts'
+// join (3.9 M float32 values: 6.8 / 7.1 us).
 struct ScaleArgs { NormEntry t[NORM_MAX]; int nt, type, units; long long chunk; Joint clip; const float* factor; };      // factor: in the place of the clipping one
 template <bool NT, class T> __device__ __forceinline__ void scale_list(T* g, long long i0, long long i1, const Joint& clip, const float* factor) {
   typedef WideStep<T> W;
@@ -2249,8 +2249,8 @@ __device__ __forceinline__ unsigned wave_max(unsigned x) {
 }
 // 2048 elements a workgroup: a list of six small tensors (252 k elements) takes 4.7 us, 6.5 with 4096, 9.7 with 8192; 3.9 M elements 17.3 / 16.9 / 16.9,
 // 134 M of bf16 548 / 538 / 599 (8-bit states 383 / 394 / 413).
-// Bound: HBM (134 M bf16 parameters, 2.95 GB: 493 us at best, 511 in the median, 5.8 TB/s; 3.9 M float32 ones, out of the last-level cache, with
-// the norm's join: 17.6 / 18.1 us).
+// Bound: HBM (134 M bf16 parameters, 2.95 GB: 496 us at best, 518 in the median, 5.7 TB/s; 3.9 M float32 ones, out of the last-level cache, with
+// the norm's join: 17.6 / 17.8 us).
 #define ADAM32_CHUNK 2048
 // Launches of more workgroups (and lists of more than JOIN_LAUNCHES) are given the joined factor.  Norm and step, joined by the workgroups / in
 // front: 32 bits 26.2 / 28.5 us at 2048 workgroups, 43.5 / 46.2 at 4096, 88.2 / 88.4 at 8192; 8 bits 18.5 / 19.5 at 1024, 30.2 / 30.9 at 2048, 38.8 / 38.3
@@ -2391,9 +2391,9 @@ __device__ __forceinline__ unsigned code8_quick(double a, double r, int low, uns
   return (t >> 17) - (sub ? (unsigned)(1023 + low) * 8u : (unsigned)(1022 + low) * 8u);
 }
 // The step with 8-bit states, a block of 256 elements a wavefront (four a lane: the codes are one 32-bit load, the block's maxima one DPP
-// tree), two blocks' loads in flight.  Bound: 80 VALU operations an element -- 134 M elements take 347 us at best with float32 parameters, 378 to
-// 405 in the median of three boxes (16 bytes each: 5.3 to 5.7 TB/s), and 338 / 381 with bf16 ones (10 bytes): 2.5 ps an element at best, whatever
-// they weigh.  3.9 M elements, 1 909 workgroups: 19.4 / 20.0 us, with the norm's join 22.0 / 23.1.
+// tree), two blocks' loads in flight.  Bound: 80 VALU operations an element -- 134 M elements take 352 us at best and 389 in the
+// median with float32 parameters (16 bytes each: 5.5 TB/s), 338 / 367 with bf16 ones (10 bytes): 2.5 to 2.6 ps an element at best, whatever they
+// weigh.  3.9 M elements, 1 909 workgroups: 19.4 / 19.8 us, with the norm's join 21.9 / 23.0.
 template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw8_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   T* p = (T*)a.t[t].p; const T* g = (const T*)a.t[t].g; unsigned char* m = (unsigned char*)a.t[t].m; unsigned char* v = (unsigned char*)a.t[t].v;
@@ -2467,8 +2467,8 @@ template <class T, bool NT> __global__ __launch_bounds__(256) void hoic_adamw8_k
   }
   for (; again; again &= again - 1) adam8_block<T>(a, t, c, cl, key, i0, ((__ffs(again) - 1) * 4 + wave) * 256, left, lane);
 }
-// the float32 values of 8-bit states: p, g of an entry are the places of m's and v's values (HBM: 134 M elements, 1.35 GB: 219 us at best,
-// 241 in the median, 5.6 TB/s; stores around the caches lose here: 719 against 646 us at 2 GB)
+// the float32 values of 8-bit states: p, g of an entry are the places of m's and v's values (HBM: 134 M elements, 1.35 GB: 216 us at best,
+// 242 in the median, 5.6 TB/s; stores around the caches lose here: 719 against 646 us at 2 GB)
 __global__ __launch_bounds__(256) void hoic_adamw_values_kernel(AdamArgs a) {
   const int t = list_find(a.t, a.nt, blockIdx.x);
   float* om = (float*)a.t[t].p; float* ov = (float*)(uintptr_t)a.t[t].g;
