@@ -380,7 +380,7 @@ int32_t hoic_policy_loss(const hoic_policy_loss_args* a, void* stream);
 /* The norm of a list of gradients (the learner clips the policy's at 40: agent_handmimic.py:67).  The lists are HOST arrays: nt
  * pointers to contiguous tensors, their sizes and types (enum hoic_type, one byte each), not all empty.  Sums in 64 bits in a fixed
  * order.  d_buf: hoic_grad_norm_parts(n, nt) + 2 doubles of scratch; d_norm: the norm in float32.
- * hoic_grad_norm: the norm; d_buf[0..1] = {norm, 1} afterwards.
+ * hoic_grad_norm: the norm; d_buf[0..1] = {norm, 1} afterwards (a norm that is not finite in float32: no factor).
  * hoic_grad_norm_partial: the parts alone, for hoic_adamw (d_norm_buf, norm_parts) to join.
  * hoic_scale_list: g *= *d_factor (device float; 1 touches nothing).
  * hoic_clip_grads: g *= min(1, bound / (norm + 1e-6)) in place (a factor of 1 touches nothing; a norm past float32's range counts as
